@@ -365,6 +365,66 @@ int rbq_pack_results(const float* dist_dev, const int64_t* ids_dev, int64_t n, u
 int rbq_merge_result_keys(const uint64_t* keys_dev, int32_t parts, int64_t nq, int32_t k, float* out_dist_dev,
                           int64_t* out_ids_dev, void* stream);
 
+/* ---- operators of the read encoder ----------------------------------------------------------
+ * The layers that make the vectors an index holds, and the loss they are trained with, forward and
+ * backward.  No index handle: they run on the current device, on `stream`, without allocating or
+ * synchronising; matrices are dense and row-major.  Each needs the workspace that its _workspace call
+ * reports for the same arguments on the same device (0: none, NULL allowed); a workspace may be reused by later calls of
+ * the same stream, not by calls that can overlap.  Buffers of 16-bit types and workspaces start on
+ * 16-byte boundaries.  rbq_check_op_errors reports what a kernel found wrong. */
+#define RBQ_F16 0
+#define RBQ_BF16 1
+#define RBQ_F32 2
+#define RBQ_ACT_NONE 0
+#define RBQ_ACT_RELU 1
+#define RBQ_ACT_GELU 2 /* z * Phi(z), the exact (erf) form */
+
+/* y [m, n] = act(x [m, k] w [n, k]^T + bias [n]) + residual [m, n]; bias and residual may be NULL.
+ * dtype RBQ_F16 or RBQ_BF16 for every matrix; products are summed in fp32 and y is rounded once.
+ * m < 2^31 - 128.  Replaces CustomLinearFn / MyLinear (src/neurosamble/kernels/layers.py:23-75)
+ * and the encoder's nn.Linear + activation + residual sums (model/signal_encoder.py:51-180). */
+int rbq_linear_workspace(int64_t m, int32_t k, int32_t n, int32_t dtype, int32_t act, int32_t backward, int64_t* bytes);
+int rbq_linear(const void* x_dev, const void* w_dev, const void* bias_dev, const void* residual_dev, void* y_dev, int64_t m,
+               int32_t k, int32_t n, int32_t dtype, int32_t act, void* workspace_dev, int64_t workspace_bytes, void* stream);
+/* Gradients from g [m, n] = dL/dy: dz = g * act'(x w^T + bias), recomputed; dx = dz w, dw = dz^T x,
+ * dbias = column sums of dz (each may be NULL).  The residual's gradient is g itself.  dz is rounded
+ * to dtype as the operand of both products; all sums are fp32 and each output is rounded once. */
+int rbq_linear_backward(const void* g_dev, const void* x_dev, const void* w_dev, const void* bias_dev, void* dx_dev,
+                        void* dw_dev, void* dbias_dev, int64_t m, int32_t k, int32_t n, int32_t dtype, int32_t act,
+                        void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/* Layer norm of rows [rows, d]: y = (x - mean) * rstd * w + b, rstd = 1 / sqrt(var + eps) with the
+ * biased variance; mean and rstd [rows] fp32 are outputs (the backward pass reads them).  dtype of x
+ * and y: RBQ_F16, RBQ_BF16 or RBQ_F32; param_dtype of w and b: the same, or RBQ_F32.  The encoder's
+ * nn.LayerNorm (model/signal_encoder.py:51-180). */
+int rbq_layer_norm(const void* x_dev, const void* w_dev, const void* b_dev, void* y_dev, float* mean_dev, float* rstd_dev,
+                   int64_t rows, int32_t d, float eps, int32_t dtype, int32_t param_dtype, void* stream);
+/* Gradients from g [rows, d]; dx, and dw and db (param_dtype), may be NULL. */
+int rbq_layer_norm_backward_workspace(int64_t rows, int32_t d, int64_t* bytes);
+int rbq_layer_norm_backward(const void* g_dev, const void* x_dev, const void* w_dev, const float* mean_dev,
+                            const float* rstd_dev, void* dx_dev, void* dw_dev, void* db_dev, int64_t rows, int32_t d,
+                            int32_t dtype, int32_t param_dtype, void* workspace_dev, int64_t workspace_bytes, void* stream);
+
+/* Softmax loss of queries q [n, d] against a bank [v, d]: with s_ij = scale * <q_i, k_j>,
+ *   lse_i = log sum_j e^{s_ij},  loss_i = lse_i - s_{i, target_i}   (fp32 [n]),
+ * the logits never stored.  A row whose target lies outside [0, v) is ignored: loss 0, no gradient.
+ * dtype RBQ_F16 or RBQ_BF16; scale > 0.  Replaces gathered_infonce_loss
+ * (src/neurosamble/harness/_ddp_common.py:71-84) after its all-gather. */
+int rbq_softmax_loss_workspace(int64_t n, int64_t v, int32_t d, int32_t dtype, int32_t backward, int64_t* bytes);
+int rbq_softmax_loss(const void* q_dev, const void* bank_dev, const int64_t* target_dev, int64_t n, int64_t v, int32_t d,
+                     float scale, int32_t dtype, float* loss_dev, float* lse_dev, void* workspace_dev,
+                     int64_t workspace_bytes, void* stream);
+/* Gradients of sum_i g_i loss_i (g [n] fp32) from the forward pass's loss and lse: dq [n, d] and
+ * dbank [v, d] (either may be NULL), in pieces of the bank.  The gradient of the logits is rounded to
+ * dtype as the operand of both products, relative to the largest |g_i|. */
+int rbq_softmax_loss_backward(const float* g_dev, const void* q_dev, const void* bank_dev, const int64_t* target_dev,
+                              const float* loss_dev, const float* lse_dev, int64_t n, int64_t v, int32_t d, float scale,
+                              int32_t dtype, void* dq_dev, void* dbank_dev, void* workspace_dev, int64_t workspace_bytes,
+                              void* stream);
+/* Synchronises the current device and returns RBQ_ERR_CUDA if a kernel of rbq_linear* or
+ * rbq_softmax_loss* gave up on a wait since the last call (their results are then invalid). */
+int rbq_check_op_errors(void);
+
 /* ---- fault injection (tests) --------------------------------------------------------------- */
 /* Host-side: the (after+1)-th device allocation the library makes from now on fails with
  * RBQ_ERR_OOM exactly as a failed cudaMalloc would (one shot; after < 0 turns it off).  Used to

@@ -42,6 +42,7 @@ class IndexInfo(ctypes.Structure):
 SHARD_POLICIES = {"round_robin": 0, "balanced": 1}
 KMEANS_KINDS = {"balanced": 0, "lloyd": 1}
 RAW_STORES = {"device": 0, "host": 1}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2}
 
 
 # name -> argtypes (all functions return int status unless listed in _RESTYPES)
@@ -91,6 +92,16 @@ SIGNATURES = {
     "rbq_merge_results": [_P, _P, _I32, _I64, _I32, _P, _P, _P],
     "rbq_pack_results": [_P, _P, _I64, _P, _P],
     "rbq_merge_result_keys": [_P, _I32, _I64, _I32, _P, _P, _P],
+    "rbq_linear_workspace": [_I64, _I32, _I32, _I32, _I32, _I32, ctypes.POINTER(_I64)],
+    "rbq_linear": [_P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _P],
+    "rbq_linear_backward": [_P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I32, _P, _I64, _P],
+    "rbq_layer_norm": [_P, _P, _P, _P, _P, _P, _I64, _I32, _F32, _I32, _I32, _P],
+    "rbq_layer_norm_backward_workspace": [_I64, _I32, ctypes.POINTER(_I64)],
+    "rbq_layer_norm_backward": [_P, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _P, _I64, _P],
+    "rbq_softmax_loss_workspace": [_I64, _I64, _I32, _I32, _I32, ctypes.POINTER(_I64)],
+    "rbq_softmax_loss": [_P, _P, _P, _I64, _I64, _I32, _F32, _I32, _P, _P, _P, _I64, _P],
+    "rbq_softmax_loss_backward": [_P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _F32, _I32, _P, _P, _P, _I64, _P],
+    "rbq_check_op_errors": [],
     "rbq_debug_fail_alloc": [_I64],
     "rbq_gen_mixture": [_P, _I64, _I32, _I32, _F32, _I32, _I32, _U64, _P],
     "rbq_gen_queries": [_P, _I64, _I32, _P, _I64, _F32, _I32, _U64, _P, _P],

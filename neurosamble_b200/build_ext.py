@@ -9,14 +9,16 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "librbq.so")
 
-SOURCES = ["rbq_host_math.cpp", "rbq_build.cu", "rbq_search.cu", "rbq_coarse_tc.cu", "rbq_capi.cu"]
-HEADERS = ["rbq_internal.cuh", os.path.join("..", "..", "include", "rbq.h")]
+SOURCES = ["rbq_host_math.cpp", "rbq_build.cu", "rbq_search.cu", "rbq_coarse_tc.cu", "rbq_gemm.cu", "rbq_norm.cu",
+           "rbq_capi.cu"]
+HEADERS = ["rbq_internal.cuh", "rbq_tc.cuh", os.path.join("..", "..", "include", "rbq.h")]
 
 # -fmad=false: no FMA contraction anywhere, so every expression is evaluated as written and
 # the results match the CPU oracle bit for bit.  IEEE division / sqrt stay on (no fast math).
@@ -57,12 +59,12 @@ def build(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
         return LIB
     os.makedirs(OUT_DIR, exist_ok=True)
-    objs = []
     nvcc = _nvcc()
     env = dict(os.environ)
     env.pop("CXX", None)
     env.pop("CC", None)
-    for src in SOURCES:
+
+    def compile_one(src: str) -> str:
         obj = os.path.join(OUT_DIR, os.path.splitext(src)[0] + ".o")
         extra = os.environ.get("RBQ_NVCC_EXTRA", "").split()
         cmd = [nvcc, *NVCC_FLAGS, *extra, "-c", os.path.join(CSRC, src), "-o", obj]
@@ -72,7 +74,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True, env=env)
-        objs.append(obj)
+        return obj
+
+    with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 1)) as pool:
+        objs = list(pool.map(compile_one, SOURCES))
     tmp = LIB + ".tmp"
     # Static CUDA runtime: the library does not bind to whichever libcudart the host process
     # (e.g. PyTorch) loaded first; device pointers and streams are shared through the driver.

@@ -13,6 +13,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <initializer_list>
 #include <mutex>
 #include <new>
 #include <string>
@@ -2506,6 +2507,224 @@ int rbq_gen_queries(const float* X_dev, int64_t n, int32_t D, float* Q_dev, int6
   return guarded([&] {
     RBQ_CHECK(X_dev && Q_dev && n >= 1 && D >= 1 && nq >= 0, RBQ_ERR_INVALID, "bad generator arguments");
     launch_gen_queries(X_dev, n, D, Q_dev, nq, sigma, normalize, seed, 20u, src_rows_dev, as_stream(stream));
+  });
+}
+
+// ---- operators of the read encoder --------------------------------------------------------
+
+namespace {
+using rbq::Error;
+
+void check_type(int32_t dtype, bool f32_too)
+{
+  RBQ_CHECK(dtype == RBQ_F16 || dtype == RBQ_BF16 || (f32_too && dtype == RBQ_F32), RBQ_ERR_INVALID,
+            f32_too ? "dtype must be RBQ_F16, RBQ_BF16 or RBQ_F32" : "dtype must be RBQ_F16 or RBQ_BF16");
+}
+void check_aligned(std::initializer_list<const void*> ps)
+{
+  for (const void* p : ps)
+    RBQ_CHECK((reinterpret_cast<uintptr_t>(p) & 15u) == 0, RBQ_ERR_INVALID, "buffers must start on 16-byte boundaries");
+}
+void check_workspace(const void* ws, int64_t bytes, int64_t need)
+{
+  RBQ_CHECK(need <= 0 || (ws != nullptr && bytes >= need), RBQ_ERR_INVALID,
+            "workspace of " + std::to_string(bytes) + " bytes, " + std::to_string(need) + " are needed");
+}
+void check_linear(int64_t m, int32_t k, int32_t n, int32_t dtype, int32_t act)
+{
+  check_type(dtype, false);
+  RBQ_CHECK(act == RBQ_ACT_NONE || act == RBQ_ACT_RELU || act == RBQ_ACT_GELU, RBQ_ERR_INVALID, "unknown activation");
+  RBQ_CHECK(m >= 0 && m < (1ll << 31) - 128 && k >= 1 && n >= 1 && k <= (1 << 24) && n <= (1 << 24), RBQ_ERR_INVALID,
+            "linear: bad sizes");
+}
+void check_norm(int64_t rows, int32_t d)
+{
+  RBQ_CHECK(rows >= 0 && d >= 1 && d <= (1 << 24) && rows <= (1ll << 40), RBQ_ERR_INVALID, "layer norm: bad sizes");
+}
+void check_norm_types(int32_t dtype, int32_t param_dtype)
+{
+  check_type(dtype, true);
+  RBQ_CHECK(param_dtype == dtype || param_dtype == RBQ_F32, RBQ_ERR_INVALID,
+            "param_dtype must be dtype or RBQ_F32");
+}
+void check_loss(int64_t n, int64_t v, int32_t d, int32_t dtype)
+{
+  check_type(dtype, false);
+  RBQ_CHECK(n >= 0 && n < (1ll << 31) - 128 && v >= 1 && v < (1ll << 31) - 256 && d >= 1 && d <= (1 << 20),
+            RBQ_ERR_INVALID, "softmax loss: bad sizes");
+}
+void check_scale(float scale)
+{
+  RBQ_CHECK(scale > 0.0f && scale <= 1e30f, RBQ_ERR_INVALID, "softmax loss: scale must be positive and finite");
+}
+size_t type_bytes(int32_t dtype) { return dtype == RBQ_F32 ? 4 : 2; }
+}  // namespace
+
+int rbq_linear_workspace(int64_t m, int32_t k, int32_t n, int32_t dtype, int32_t act, int32_t backward, int64_t* bytes)
+{
+  return guarded([&] {
+    RBQ_CHECK(bytes, RBQ_ERR_INVALID, "null argument");
+    check_linear(m, k, n, dtype, act);
+    *bytes = m == 0 ? 0
+             : backward
+                 ? launch_linear_backward(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, m, k, n, dtype,
+                                          act, nullptr, false, nullptr)
+                 : launch_linear(nullptr, nullptr, nullptr, nullptr, nullptr, m, k, n, dtype, act, nullptr, false,
+                                 nullptr);
+  });
+}
+
+int rbq_linear(const void* x_dev, const void* w_dev, const void* bias_dev, const void* residual_dev, void* y_dev, int64_t m,
+               int32_t k, int32_t n, int32_t dtype, int32_t act, void* workspace_dev, int64_t workspace_bytes, void* stream)
+{
+  return guarded([&] {
+    Range nvtx_range("rbq_linear");
+    check_linear(m, k, n, dtype, act);
+    if (m == 0) return;
+    RBQ_CHECK(x_dev && w_dev && y_dev, RBQ_ERR_INVALID, "null buffer");
+    check_aligned({x_dev, w_dev, residual_dev, y_dev, workspace_dev});
+    check_workspace(workspace_dev, workspace_bytes,
+                    launch_linear(x_dev, w_dev, bias_dev, residual_dev, y_dev, m, k, n, dtype, act, nullptr, false, nullptr));
+    launch_linear(x_dev, w_dev, bias_dev, residual_dev, y_dev, m, k, n, dtype, act, workspace_dev, true, as_stream(stream));
+  });
+}
+
+int rbq_linear_backward(const void* g_dev, const void* x_dev, const void* w_dev, const void* bias_dev, void* dx_dev,
+                        void* dw_dev, void* dbias_dev, int64_t m, int32_t k, int32_t n, int32_t dtype, int32_t act,
+                        void* workspace_dev, int64_t workspace_bytes, void* stream)
+{
+  return guarded([&] {
+    Range nvtx_range("rbq_linear_backward");
+    check_linear(m, k, n, dtype, act);
+    cudaStream_t s = as_stream(stream);
+    if (m == 0) {  // empty sums
+      if (dw_dev) RBQ_CUDA(cudaMemsetAsync(dw_dev, 0, (size_t)n * k * 2, s));
+      if (dbias_dev) RBQ_CUDA(cudaMemsetAsync(dbias_dev, 0, (size_t)n * 2, s));
+      return;
+    }
+    RBQ_CHECK(g_dev && x_dev && w_dev, RBQ_ERR_INVALID, "null buffer");
+    check_aligned({g_dev, x_dev, w_dev, dx_dev, dw_dev, workspace_dev});
+    check_workspace(workspace_dev, workspace_bytes,
+                    launch_linear_backward(g_dev, x_dev, w_dev, bias_dev, dx_dev, dw_dev, dbias_dev, m, k, n, dtype, act,
+                                           nullptr, false, nullptr));
+    launch_linear_backward(g_dev, x_dev, w_dev, bias_dev, dx_dev, dw_dev, dbias_dev, m, k, n, dtype, act, workspace_dev,
+                           true, s);
+  });
+}
+
+int rbq_layer_norm(const void* x_dev, const void* w_dev, const void* b_dev, void* y_dev, float* mean_dev, float* rstd_dev,
+                   int64_t rows, int32_t d, float eps, int32_t dtype, int32_t param_dtype, void* stream)
+{
+  return guarded([&] {
+    Range nvtx_range("rbq_layer_norm");
+    check_norm(rows, d);
+    check_norm_types(dtype, param_dtype);
+    RBQ_CHECK(eps >= 0.0f && eps <= 1e30f, RBQ_ERR_INVALID, "layer norm: eps must be finite and not negative");
+    if (rows == 0) return;
+    RBQ_CHECK(x_dev && w_dev && b_dev && y_dev && mean_dev && rstd_dev, RBQ_ERR_INVALID, "null buffer");
+    launch_layer_norm(x_dev, w_dev, b_dev, y_dev, mean_dev, rstd_dev, rows, d, eps, dtype, param_dtype, as_stream(stream));
+  });
+}
+
+int rbq_layer_norm_backward_workspace(int64_t rows, int32_t d, int64_t* bytes)
+{
+  return guarded([&] {
+    RBQ_CHECK(bytes, RBQ_ERR_INVALID, "null argument");
+    check_norm(rows, d);
+    *bytes = rows == 0 ? 0 : layer_norm_workspace(rows, d);
+  });
+}
+
+int rbq_layer_norm_backward(const void* g_dev, const void* x_dev, const void* w_dev, const float* mean_dev,
+                            const float* rstd_dev, void* dx_dev, void* dw_dev, void* db_dev, int64_t rows, int32_t d,
+                            int32_t dtype, int32_t param_dtype, void* workspace_dev, int64_t workspace_bytes, void* stream)
+{
+  return guarded([&] {
+    Range nvtx_range("rbq_layer_norm_backward");
+    check_norm(rows, d);
+    check_norm_types(dtype, param_dtype);
+    cudaStream_t s = as_stream(stream);
+    if (rows == 0) {
+      if (dw_dev) RBQ_CUDA(cudaMemsetAsync(dw_dev, 0, (size_t)d * type_bytes(param_dtype), s));
+      if (db_dev) RBQ_CUDA(cudaMemsetAsync(db_dev, 0, (size_t)d * type_bytes(param_dtype), s));
+      return;
+    }
+    RBQ_CHECK(g_dev && x_dev && w_dev && mean_dev && rstd_dev, RBQ_ERR_INVALID, "null buffer");
+    if (!dx_dev && !dw_dev && !db_dev) return;
+    if (dw_dev || db_dev) {
+      check_aligned({workspace_dev});
+      check_workspace(workspace_dev, workspace_bytes, layer_norm_workspace(rows, d));
+    }
+    launch_layer_norm_backward(g_dev, x_dev, w_dev, mean_dev, rstd_dev, dx_dev, dw_dev, db_dev,
+                               static_cast<float*>(workspace_dev), rows, d, dtype, param_dtype, s);
+  });
+}
+
+int rbq_softmax_loss_workspace(int64_t n, int64_t v, int32_t d, int32_t dtype, int32_t backward, int64_t* bytes)
+{
+  return guarded([&] {
+    RBQ_CHECK(bytes, RBQ_ERR_INVALID, "null argument");
+    check_loss(n, v, d, dtype);
+    *bytes = n == 0 ? 0
+             : backward ? launch_softmax_loss_backward(nullptr, nullptr, nullptr, nullptr, nullptr, nullptr, n, v, d, 1.0f,
+                                                       dtype, nullptr, nullptr, nullptr, false, nullptr)
+                        : launch_softmax_loss(nullptr, nullptr, nullptr, n, v, d, 1.0f, dtype, nullptr, nullptr, nullptr,
+                                              false, nullptr);
+  });
+}
+
+int rbq_softmax_loss(const void* q_dev, const void* bank_dev, const int64_t* target_dev, int64_t n, int64_t v, int32_t d,
+                     float scale, int32_t dtype, float* loss_dev, float* lse_dev, void* workspace_dev,
+                     int64_t workspace_bytes, void* stream)
+{
+  return guarded([&] {
+    Range nvtx_range("rbq_softmax_loss");
+    check_loss(n, v, d, dtype);
+    check_scale(scale);
+    if (n == 0) return;
+    RBQ_CHECK(q_dev && bank_dev && target_dev && loss_dev && lse_dev, RBQ_ERR_INVALID, "null buffer");
+    check_aligned({q_dev, bank_dev, workspace_dev});
+    check_workspace(workspace_dev, workspace_bytes,
+                    launch_softmax_loss(q_dev, bank_dev, target_dev, n, v, d, scale, dtype, loss_dev, lse_dev, nullptr, false,
+                                        nullptr));
+    launch_softmax_loss(q_dev, bank_dev, target_dev, n, v, d, scale, dtype, loss_dev, lse_dev, workspace_dev, true,
+                        as_stream(stream));
+  });
+}
+
+int rbq_softmax_loss_backward(const float* g_dev, const void* q_dev, const void* bank_dev, const int64_t* target_dev,
+                              const float* loss_dev, const float* lse_dev, int64_t n, int64_t v, int32_t d, float scale,
+                              int32_t dtype, void* dq_dev, void* dbank_dev, void* workspace_dev, int64_t workspace_bytes,
+                              void* stream)
+{
+  return guarded([&] {
+    Range nvtx_range("rbq_softmax_loss_backward");
+    check_loss(n, v, d, dtype);
+    check_scale(scale);
+    cudaStream_t s = as_stream(stream);
+    if (n == 0) {
+      if (dbank_dev) RBQ_CUDA(cudaMemsetAsync(dbank_dev, 0, (size_t)v * d * 2, s));
+      return;
+    }
+    RBQ_CHECK(g_dev && q_dev && bank_dev && target_dev && loss_dev && lse_dev, RBQ_ERR_INVALID, "null buffer");
+    if (!dq_dev && !dbank_dev) return;
+    check_aligned({q_dev, bank_dev, dq_dev, dbank_dev, workspace_dev});
+    check_workspace(workspace_dev, workspace_bytes,
+                    launch_softmax_loss_backward(g_dev, q_dev, bank_dev, target_dev, loss_dev, lse_dev, n, v, d, scale, dtype,
+                                                 dq_dev, dbank_dev, nullptr, false, nullptr));
+    launch_softmax_loss_backward(g_dev, q_dev, bank_dev, target_dev, loss_dev, lse_dev, n, v, d, scale, dtype, dq_dev,
+                                 dbank_dev, workspace_dev, true, s);
+  });
+}
+
+int rbq_check_op_errors(void)
+{
+  return guarded([&] {
+    RBQ_CUDA(cudaDeviceSynchronize());
+    const int code = take_op_error();
+    if (code)
+      throw Error{RBQ_ERR_CUDA, "a tensor-core pipeline wait timed out on the device (code " + std::to_string(code) +
+                                    "); results of the affected operator are invalid"};
   });
 }
 

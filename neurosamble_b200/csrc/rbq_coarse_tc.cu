@@ -27,6 +27,7 @@
 #include <mutex>
 
 #include "rbq_internal.cuh"
+#include "rbq_tc.cuh"
 
 namespace rbq {
 namespace {
@@ -38,9 +39,6 @@ constexpr int kTcThreads = 256;
 constexpr int kTcStageBytes = (kTcM + kTcN) * 128;  // A chunk (16 KB) + B chunk (32 KB)
 constexpr int kTcStages = 3;
 constexpr int kTcEpiPitch = 33;  // floats per row of a warp's 32 x 32 epilogue tile (bank-conflict free)
-constexpr uint32_t kWaitLimit = 1u << 26;           // bounded mbarrier polling
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
 // 64-bit shared-memory matrix descriptor (K-major, 128-byte swizzle): start address, leading
 // byte offset (unused for this layout, 16 B), stride byte offset (1024 B between 8-row atoms),
@@ -60,69 +58,12 @@ __device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr)
 constexpr uint32_t kTcIdesc = (1u << 4) | (2u << 7) | (2u << 10) | ((uint32_t)(kTcN >> 3) << 17) |
                               ((uint32_t)(kTcM >> 4) << 24);
 
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count)
-{
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count));
-}
-
-// Polls mbarrier phase `parity`; false if it did not complete within kWaitLimit polls.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity)
-{
-  for (uint32_t it = 0; it < kWaitLimit; ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (ok) return true;
-  }
-  return false;
-}
-
 __device__ __forceinline__ void tc_mma(uint32_t dtmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc)
 {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
       " tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n}" ::"r"(dtmem),
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc));
-}
-
-__device__ __forceinline__ void tc_commit(uint32_t bar)
-{
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-
-// 32 consecutive fp32 accumulator columns of the warp's 32 TMEM lanes.
-__device__ __forceinline__ void tc_ld32(uint32_t taddr, float (&v)[32])
-{
-  uint32_t r[32];
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
-      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-        "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-        "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-      : "r"(taddr));
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes)
-{
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
-// 2-D tile load of the tensor map's box at element coordinates (x, y) into shared memory.
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar)
-{
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::
-          "r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
-      : "memory");
 }
 
 __global__ void __launch_bounds__(kTcThreads, 1) coarse_tc_kernel(const __grid_constant__ CUtensorMap tmQ,
@@ -286,27 +227,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) coarse_tc_kernel(const __grid_c
 constexpr int kFtThreads = 192;
 constexpr int kFtStages = 4;
 constexpr int kFtProducerWarp = 4, kFtMmaWarp = 5;
-
-__device__ __forceinline__ void mbar_arrive(uint32_t bar)
-{
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-// mbar_wait that also gives up as soon as another role has reported a failure.
-__device__ __forceinline__ bool mbar_wait_or_fail(uint32_t bar, uint32_t parity, volatile int* fail)
-{
-  for (uint32_t it = 0; it < kWaitLimit; ++it) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (ok) return true;
-    if ((it & 1023u) == 1023u && *fail) return false;
-  }
-  return false;
-}
 
 // Ascending bitonic sort of the 32 * KPL keys a warp holds in registers: element e = lane * KPL + j
 // lives in k[j] of lane `lane`.  Partners closer than KPL are in the same lane; farther ones are
@@ -877,6 +797,8 @@ __global__ void __launch_bounds__(kLsThreads, N == 128 ? 2 : 1) list_scan_tc_ker
   }
 }
 
+}  // namespace
+
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no link-time libcuda).
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder()
 {
@@ -892,6 +814,8 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder()
   RBQ_CHECK(fn != nullptr, RBQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
   return fn;
 }
+
+namespace {
 
 // Row-major fp32 [rows, dp] matrix, box = [box_rows, 32 values], 128-byte swizzle, zero fill.
 CUtensorMap row_major_map(const float* ptr, int64_t rows, int dp, int box_rows)

@@ -1,0 +1,1229 @@
+// Matrix products on the 5th-generation tensor cores (tcgen05, sm_100a) with the epilogues of the
+// read encoder's operators: the linear layer y = act(x w^T + b) + residual and its gradients, and
+// the softmax loss of embeddings against a bank, whose logits never leave the SM.
+//
+//   D[M, N] = sum_k A[m, k] B[n, k]     A, B fp16 or bf16, fp32 accumulators in tensor memory
+//
+// Either operand may be stored with k contiguous ("K-major": x, w, q, the bank) or with its own
+// rows contiguous ("MN-major": the same matrices inside a gradient, where the sum runs over the
+// stored rows); the tensor cores read both, so no operand is ever transposed in memory.
+//
+// CTA (320 threads, persistent over output tiles of 128 x BN): warp 8 streams 64-wide k-blocks of A
+// and B by TMA into a ring of shared-memory stages (128-byte swizzle, zero fill past the edges), warp 9
+// issues the MMAs into one of two accumulators (2 x BN of the 512 TMEM columns), and two warpgroups
+// take the finished accumulators in turn, so that the epilogue of one tile runs beside the MMAs of
+// the next.  In an epilogue thread r owns output row r (TMEM lane r).  Output and input tiles of the
+// epilogue pass through 128-byte swizzled staging rows: by TMA where the matrix allows it (rows a
+// multiple of 16 bytes apart), else by coalesced loads and stores of the warp that owns the rows.
+//
+// Long sums with few output tiles (weight gradients) are split along k: every split writes its own
+// fp32 slab and a second kernel adds the slabs in their order, so results do not depend on timing.
+//
+// Every mbarrier wait is bounded: on time-out the kernel records a code in g_op_err, all roles stop
+// touching memory, copies in flight are waited for (bounded), TMEM is freed and the kernel returns.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <type_traits>
+
+#include "rbq_internal.cuh"
+#include "rbq_tc.cuh"
+
+namespace rbq {
+namespace {
+
+constexpr int kBM = 128;       // output rows of a tile (TMEM lanes)
+constexpr int kBK = 64;        // reduction values per stage: one 128-byte row of 16-bit values
+constexpr int kThreads = 320;  // two epilogue warpgroups, the loader warp, the MMA warp
+constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kStageOut = kBM * 128;          // one staging buffer: 128 rows of 128 bytes
+constexpr uint32_t kOpWaitLimit = 1u << 22;   // polls; each suspends for up to some microseconds
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kGradScale = 16384.0f;        // power of two, see GradRows
+
+__device__ int g_op_err;
+
+enum Epilogue {
+  kEpiLinear,  // out = act(alpha * acc + bias) + extra
+  kEpiActGrad, // out = extra * act'(acc + bias)
+  kEpiSlab,    // fp32 slab of a split along k, written or added to
+  kEpiLse,     // per row and tile: max and sum of exp of the scaled logits, without the target's
+  kEpiProb,    // out = gradient of the loss with respect to the logits, scaled
+};
+
+struct GemmArgs {
+  int64_t M = 0;
+  int N = 0;
+  int tiles_m = 0, tiles_n = 0, splits = 1, kblocks = 0;
+  int m_fast = 0;        // tile order: rows of tiles vary fastest, else columns
+  int a_mn = 0, b_mn = 0;  // operand stored with its rows contiguous
+  uint32_t idesc = 0;
+  // epilogue matrices
+  int io_tma = 1;        // staging moves by TMA; else by the warps from / to the pointers below
+  const void* bias = nullptr;   // [N]
+  const void* extra = nullptr;  // [M, N]
+  void* out = nullptr;          // [M, N]
+  int has_extra = 0;
+  int64_t ld_extra = 0, ld_out = 0;  // of the warps' own moves
+  float alpha = 1.0f;
+  const float* alpha_dev = nullptr;  // further factor held on the device
+  int act = RBQ_ACT_NONE;
+  int slab_rows = 0;     // rows between slabs
+  int slab_add = 0;      // add to what the slab holds
+  // softmax loss: rows are queries, columns bank rows col0 + n
+  float c2 = 0.0f;       // scale * log2(e)
+  int64_t col0 = 0;
+  const int64_t* target = nullptr;   // [M]
+  float2* partial = nullptr;         // [tiles_n, M] (max, sum), base 2
+  const float4* rows = nullptr;      // [M] GradRows
+};
+
+// What the gradient of a row's logits needs: lse in base 2, the row's weight w = g_i / max|g| times
+// kGradScale (0: the row takes no part) and the value at the target, expm1(-loss) * w.
+//   d loss_i / d s_ij = p_ij - [j = t_i],   p_ij - 1 = expm1(-loss_i) at the target
+// The gradient of the logits is rounded to the operands' 16 bits, since it is the operand of the two
+// products that follow.  |p - 1| <= 1, so with |w| <= 2^14 nothing overflows in fp16 and
+// probabilities down to 2^-28 keep all 11 bits; the factor max|g| * scale / 2^14 returns in fp32.
+struct GradRows {
+  float lse2, w, at_target, unused;
+};
+
+__device__ __forceinline__ float ex2(float x)
+{
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Shared-memory matrix descriptor, 128-byte swizzle.  K-major: 8-row atoms 1024 bytes apart (stride
+// offset).  MN-major: an atom is 64 values of the rows by 8 of k; the next 8 of k are 1024 bytes
+// on (stride offset), the next 64 rows one whole k-block on, kBK * 128 bytes (leading offset).
+__device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, int mn)
+{
+  const uint32_t lead = mn ? kBK * 128u : 16u;
+  return (uint64_t)((saddr >> 4) & 0x3FFFu) | (uint64_t)(lead >> 4) << 16 | (uint64_t)(1024u >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+// Bounded wait that gives up once any role has failed.
+__device__ __forceinline__ bool op_wait(uint32_t bar, uint32_t parity, volatile int* fail)
+{
+  for (uint32_t it = 0; it < kOpWaitLimit; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 255u) == 255u && *fail) return false;
+  }
+  return false;
+}
+
+__device__ __forceinline__ void fail_with(volatile int* fail, int code)
+{
+  *fail = 1;
+  atomicExch(&g_op_err, code);
+}
+
+__device__ __forceinline__ void group_sync(int wg) { asm volatile("bar.sync %0, 128;" ::"r"(wg + 1) : "memory"); }
+
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y)
+{
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_add_2d(const CUtensorMap* map, uint32_t src, int x, int y)
+{
+  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+
+template <typename T>
+struct Pack;
+template <>
+struct Pack<__half> {
+  static __device__ __forceinline__ uint32_t two(float a, float b)
+  {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 get(uint32_t u)
+  {
+    return __half22float2(*reinterpret_cast<__half2*>(&u));
+  }
+  static __device__ __forceinline__ float one(__half h) { return __half2float(h); }
+  static __device__ __forceinline__ __half from(float f) { return __float2half_rn(f); }
+};
+template <>
+struct Pack<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t two(float a, float b)
+  {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t*>(&h);
+  }
+  static __device__ __forceinline__ float2 get(uint32_t u)
+  {
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+  }
+  static __device__ __forceinline__ float one(__nv_bfloat16 h) { return __bfloat162float(h); }
+  static __device__ __forceinline__ __nv_bfloat16 from(float f) { return __float2bfloat16_rn(f); }
+};
+
+// act(z) and act'(z); GELU is z * Phi(z), its slope Phi(z) + z * phi(z).
+template <int ACT>
+__device__ __forceinline__ float act_of(float z)
+{
+  if (ACT == RBQ_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
+  if (ACT == RBQ_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+  return z;
+}
+template <int ACT>
+__device__ __forceinline__ float act_slope(float z)
+{
+  if (ACT == RBQ_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+  if (ACT == RBQ_ACT_GELU)
+    return fmaf(z * 0.39894228f, __expf(-0.5f * z * z), 0.5f * (1.0f + erff(z * 0.70710678f)));
+  return 1.0f;
+}
+
+struct Tile {
+  int m, n, split;
+};
+__device__ __forceinline__ Tile tile_at(const GemmArgs& a, int t)
+{
+  Tile r;
+  const int per = a.tiles_m * a.tiles_n;
+  r.split = t / per;
+  const int i = t - r.split * per;
+  if (a.m_fast) {
+    r.n = i / a.tiles_m;
+    r.m = i - r.n * a.tiles_m;
+  } else {
+    r.m = i / a.tiles_n;
+    r.n = i - r.m * a.tiles_n;
+  }
+  return r;
+}
+__device__ __forceinline__ int k_begin(const GemmArgs& a, int split)
+{
+  return (int)((int64_t)a.kblocks * split / a.splits);
+}
+
+template <int EPI, int BN>
+struct Shape {
+  static constexpr int kOperands = kBM * 128 + BN * 128;
+  static constexpr bool kStaged = EPI != kEpiLse;  // the loss's forward pass writes no tile
+  static constexpr int kStages = kStaged ? (BN == 256 ? 3 : 5) : (BN == 256 ? 4 : 6);
+  static constexpr int kOutBytes = kStaged ? 4 * kStageOut : 0;  // two buffers per warpgroup
+  static constexpr int kBytes = kStages * kOperands + kOutBytes + 2 * BN * 4 + 1024;
+};
+
+// The warp's 32 staging rows <-> a matrix whose rows no TMA can address, 64 columns from `col`.
+template <typename T, bool LOAD>
+__device__ __forceinline__ void move_rows(unsigned char* buf, T* mat, int64_t row0, int64_t M, int64_t ld, int col, int N,
+                                          int warp_row, int lane)
+{
+#pragma unroll 4
+  for (int r = 0; r < 32; ++r) {
+    const int row = warp_row + r;
+    if (row0 + row >= M) break;
+    T* at = reinterpret_cast<T*>(buf + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4);
+    T* g = mat + (row0 + row) * ld + col + lane * 2;
+    const int left = N - col - lane * 2;
+    if (LOAD) {
+      at[0] = left > 0 ? g[0] : T(0.0f);
+      at[1] = left > 1 ? g[1] : T(0.0f);
+    } else {
+      if (left > 0) g[0] = at[0];
+      if (left > 1) g[1] = at[1];
+    }
+  }
+}
+
+template <int EPI, typename T, int BN, int ACT>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmO,
+                const __grid_constant__ GemmArgs a)
+{
+  using S = Shape<EPI, BN>;
+  extern __shared__ unsigned char gemm_smem_raw[];
+  unsigned char* base = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~(uintptr_t)1023);
+  unsigned char* staging = base + S::kStages * S::kOperands;
+  float* s_bias = reinterpret_cast<float*>(staging + S::kOutBytes);  // [2][BN]
+  __shared__ __align__(8) unsigned long long s_full[S::kStages], s_empty[S::kStages], s_done[2], s_free[2], s_x[4];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_fail;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                 "r"((uint32_t)(2 * BN)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  if (tid == 0) {
+    for (int i = 0; i < S::kStages; ++i) {
+      mbar_init(smem_u32(&s_full[i]), 1);
+      mbar_init(smem_u32(&s_empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&s_done[i]), 1);
+      mbar_init(smem_u32(&s_free[i]), 4);  // one arrival per epilogue warp
+    }
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&s_x[i]), 1);
+    s_fail = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = s_tmem;
+  volatile int* fail = &s_fail;
+  const int total = a.tiles_m * a.tiles_n * a.splits;
+
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmA)) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmB)) : "memory");
+      int c = 0;  // k-block, counted over the CTA's whole run: stage c % kStages
+      bool ok = true;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+        const Tile tl = tile_at(a, t);
+        const int m0 = tl.m * kBM, n0 = tl.n * BN;
+        for (int kb = k_begin(a, tl.split), ke = k_begin(a, tl.split + 1); kb < ke; ++kb, ++c) {
+          const int st = c % S::kStages;
+          if (c >= S::kStages && !op_wait(smem_u32(&s_empty[st]), (uint32_t)((c / S::kStages - 1) & 1), fail)) {
+            fail_with(fail, 1);
+            ok = false;
+            break;
+          }
+          const uint32_t full = smem_u32(&s_full[st]);
+          const uint32_t sa = smem_u32(base + st * S::kOperands), sb = sa + kBM * 128;
+          mbar_expect_tx(full, (uint32_t)S::kOperands);
+          const int k0 = kb * kBK;
+          if (a.a_mn) {
+#pragma unroll
+            for (int j = 0; j < kBM / 64; ++j) tma_load_2d(sa + j * kBK * 128, &tmA, m0 + j * 64, k0, full);
+          } else {
+            tma_load_2d(sa, &tmA, k0, m0, full);
+          }
+          if (a.b_mn) {
+#pragma unroll
+            for (int j = 0; j < BN / 64; ++j) tma_load_2d(sb + j * kBK * 128, &tmB, n0 + j * 64, k0, full);
+          } else {
+            tma_load_2d(sb, &tmB, k0, n0, full);
+          }
+        }
+      }
+      // Copies in flight after a failure land before the CTA's shared memory goes away.
+      if (*fail)
+        for (int i = (c > S::kStages ? c - S::kStages : 0); i < c; ++i)
+          mbar_wait(smem_u32(&s_full[i % S::kStages]), (uint32_t)((i / S::kStages) & 1));
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    if (lane == 0) {
+      const uint32_t a_step = a.a_mn ? 16 * 128 : 32, b_step = a.b_mn ? 16 * 128 : 32;  // 16 values of k
+      int c = 0, i = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++i) {
+        const int acc = i & 1;
+        if (i >= 2 && !op_wait(smem_u32(&s_free[acc]), (uint32_t)(((i >> 1) - 1) & 1), fail)) {
+          fail_with(fail, 2);
+          break;
+        }
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const int split = t / (a.tiles_m * a.tiles_n);
+        const int kb0 = k_begin(a, split), ke = k_begin(a, split + 1);
+        for (int kb = kb0; kb < ke; ++kb, ++c) {
+          const int st = c % S::kStages;
+          if (!op_wait(smem_u32(&s_full[st]), (uint32_t)((c / S::kStages) & 1), fail)) {
+            fail_with(fail, 3);
+            ok = false;
+            break;
+          }
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t sa = smem_u32(base + st * S::kOperands), sb = sa + kBM * 128;
+#pragma unroll
+          for (int ks = 0; ks < kBK / 16; ++ks)
+            mma_f16(tmem + acc * BN, operand_desc(sa + ks * a_step, a.a_mn), operand_desc(sb + ks * b_step, a.b_mn),
+                    a.idesc, (kb > kb0 || ks > 0) ? 1u : 0u);
+          tc_commit(smem_u32(&s_empty[st]));
+        }
+        if (ok) tc_commit(smem_u32(&s_done[acc]));
+      }
+      // MMAs still running after a failure end before TMEM is freed: the last commit follows them.
+      if (*fail && c > 0)
+        mbar_wait(smem_u32(&s_empty[(c - 1) % S::kStages]), (uint32_t)(((c - 1) / S::kStages) & 1));
+    }
+    __syncwarp();
+  } else {
+    const int wg = warp >> 2, quarter = warp & 3;
+    const int gt = tid & 127;  // thread of the warpgroup = accumulator lane = output row
+    const bool leader = gt == 0;
+    unsigned char* bufs = staging + wg * 2 * kStageOut;
+    float* bias = s_bias + wg * BN;
+    const uint32_t acc_addr = tmem + wg * BN + ((uint32_t)(quarter * 32) << 16);
+    constexpr int kSub = EPI == kEpiSlab ? 32 : 64;  // columns of one 128-byte staging row
+    bool dead = false;  // a wait failed: keep the barriers in step, touch nothing
+    int c = 0;          // staging tile, counted over the warpgroup's run: buffer c & 1
+
+    // The extra input of staging tile c arrives by TMA one tile ahead.
+    auto load_extra = [&](int cc, int t, int s) {
+      const Tile tl = tile_at(a, t);
+      const uint32_t bar = smem_u32(&s_x[wg * 2 + (cc & 1)]);
+      mbar_expect_tx(bar, (uint32_t)kStageOut);
+      tma_load_2d(smem_u32(bufs + (cc & 1) * kStageOut), &tmX, tl.n * BN + s * 64, tl.m * kBM, bar);
+    };
+    const bool extra_tma = (EPI == kEpiLinear || EPI == kEpiActGrad) && a.has_extra && a.io_tma;
+    int loaded = 0;  // extra tiles asked for (leader)
+    if (extra_tma && leader) {
+      const int t = blockIdx.x + wg * gridDim.x;
+      if (t < total) {
+        load_extra(0, t, 0);
+        loaded = 1;
+      }
+    }
+
+    for (int i = wg, t = blockIdx.x + wg * gridDim.x; t < total; i += 2, t += 2 * gridDim.x) {
+      const Tile tl = tile_at(a, t);
+      const int64_t m0 = (int64_t)tl.m * kBM;
+      const int n0 = tl.n * BN;
+      const int64_t row = m0 + gt;
+      if ((EPI == kEpiLinear || EPI == kEpiActGrad) && a.bias != nullptr) {
+        group_sync(wg);  // the last tile's values have been used
+        for (int j = gt; j < BN; j += 128)
+          bias[j] = n0 + j < a.N ? Pack<T>::one(reinterpret_cast<const T*>(a.bias)[n0 + j]) : 0.0f;
+        group_sync(wg);
+      }
+      if (!dead) {
+        const bool ok = op_wait(smem_u32(&s_done[wg]), (uint32_t)((i >> 1) & 1), fail);
+        if (!__all_sync(0xffffffffu, ok)) {
+          if (lane == 0) fail_with(fail, 4);
+          dead = true;
+        }
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+
+      if (EPI == kEpiLse) {
+        const int64_t trow = row < a.M ? __ldg(a.target + row) - a.col0 - n0 : -1;
+        float m = -INFINITY, l = 0.0f;
+        if (!dead) {
+#pragma unroll 1
+          for (int j = 0; j < BN / 32; ++j) {
+            float v[32];
+            tc_ld32(acc_addr + j * 32, v);
+            const int64_t tj = trow - j * 32;
+            if (__any_sync(0xffffffffu, (uint64_t)tj < 32u)) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = e == tj ? -INFINITY : v[e];
+            }
+            if (n0 + j * 32 + 32 > a.N) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = n0 + j * 32 + e < a.N ? v[e] : -INFINITY;
+            }
+            float top = v[0];
+#pragma unroll
+            for (int e = 1; e < 32; ++e) top = fmaxf(top, v[e]);
+            const float mn = fmaxf(m, top * a.c2);
+            const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing but masked logits so far
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sum += ex2(fmaf(v[e], a.c2, -ref));
+            l = fmaf(l, ex2(m - ref), sum);
+            m = mn;
+          }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&s_free[wg]));
+        if (!dead && row < a.M) a.partial[(int64_t)tl.n * a.M + row] = make_float2(m, l);
+        continue;
+      }
+
+      GradRows gr{};
+      int64_t trow = -1;
+      if (EPI == kEpiProb && row < a.M) {
+        const float4 q = __ldg(a.rows + row);
+        gr = GradRows{q.x, q.y, q.z, q.w};
+        trow = __ldg(a.target + row) - a.col0 - n0;
+      }
+      float alpha = a.alpha;
+      if (a.alpha_dev != nullptr) alpha *= __ldg(a.alpha_dev);
+      const int subs = min(BN / kSub, (a.N - n0 + kSub - 1) / kSub);
+#pragma unroll 1
+      for (int s = 0; s < subs; ++s, ++c) {
+        unsigned char* buf = bufs + (c & 1) * kStageOut;
+        const int col = n0 + s * kSub;
+        if (extra_tma) {
+          // ask for the next tile's extra input: its buffer's last store has been read
+          if (leader && !dead) {
+            int nt = t, ns = s + 1;
+            if (ns == subs) nt = t + 2 * gridDim.x, ns = 0;
+            if (nt < total) {
+              asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+              load_extra(c + 1, nt, ns);
+              ++loaded;
+            }
+          }
+          if (!dead) {
+            const bool ok = op_wait(smem_u32(&s_x[wg * 2 + (c & 1)]), (uint32_t)((c >> 1) & 1), fail);
+            if (!__all_sync(0xffffffffu, ok)) {
+              if (lane == 0) fail_with(fail, 5);
+              dead = true;
+            }
+          }
+        } else if (a.io_tma) {
+          if (leader) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          group_sync(wg);  // the buffer's last store has been read
+        } else if ((EPI == kEpiLinear || EPI == kEpiActGrad) && a.has_extra) {
+          if (!dead)
+            move_rows<T, true>(buf, reinterpret_cast<T*>(const_cast<void*>(a.extra)), m0, a.M, a.ld_extra, col,
+                               a.N, quarter * 32, lane);
+          __syncwarp();
+        }
+        if (!dead) {
+#pragma unroll
+          for (int h = 0; h < kSub / 32; ++h) {
+            float v[32];
+            tc_ld32(acc_addr + s * kSub + h * 32, v);
+            if (EPI == kEpiSlab) {
+              float4* at = reinterpret_cast<float4*>(buf + gt * 128);
+#pragma unroll
+              for (int u = 0; u < 8; ++u)
+                at[u ^ (gt & 7)] = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
+              continue;
+            }
+            uint4* at = reinterpret_cast<uint4*>(buf + gt * 128);
+            if (EPI == kEpiProb) {
+              const int64_t tj = trow - s * 64 - h * 32;
+#pragma unroll
+              for (int e = 0; e < 32; ++e) v[e] = ex2(fmaf(v[e], a.c2, -gr.lse2)) * gr.w;
+              if (gr.w == 0.0f) {  // a row that takes no part, whatever its logits
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+              }
+              if ((uint64_t)tj < 32u) {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) v[e] = e == tj ? gr.at_target : v[e];
+              }
+            }
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const int slot = (h * 4 + u) ^ (gt & 7);
+              if (EPI == kEpiLinear || EPI == kEpiActGrad) {
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (EPI == kEpiActGrad || a.has_extra) x = at[slot];
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float2 xe = Pack<T>::get(xs[e]);
+                  float& v0 = v[u * 8 + e * 2];
+                  float& v1 = v[u * 8 + e * 2 + 1];
+                  float b0 = 0.0f, b1 = 0.0f;
+                  if (a.bias != nullptr) {
+                    const float2 b = *reinterpret_cast<const float2*>(bias + s * 64 + h * 32 + u * 8 + e * 2);
+                    b0 = b.x, b1 = b.y;
+                  }
+                  const float z0 = fmaf(v0, alpha, b0), z1 = fmaf(v1, alpha, b1);
+                  if (EPI == kEpiActGrad) {
+                    v0 = xe.x * act_slope<ACT>(z0);
+                    v1 = xe.y * act_slope<ACT>(z1);
+                  } else {
+                    v0 = act_of<ACT>(z0) + xe.x;
+                    v1 = act_of<ACT>(z1) + xe.y;
+                  }
+                }
+              }
+              const float* w = v + u * 8;
+              at[slot] = make_uint4(Pack<T>::two(w[0], w[1]), Pack<T>::two(w[2], w[3]), Pack<T>::two(w[4], w[5]),
+                                    Pack<T>::two(w[6], w[7]));
+            }
+          }
+        }
+        if (s + 1 == subs) {  // the accumulator has been read
+          asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&s_free[wg]));
+        }
+        if (EPI == kEpiSlab || a.io_tma) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          group_sync(wg);
+          if (leader && !dead && !*fail) {
+            const int y = EPI == kEpiSlab ? tl.split * a.slab_rows + (int)m0 : (int)m0;
+            if (EPI == kEpiSlab && a.slab_add)
+              tma_add_2d(&tmO, smem_u32(buf), col, y);
+            else
+              tma_store_2d(&tmO, smem_u32(buf), col, y);
+          }
+        } else {
+          __syncwarp();
+          if (!dead)
+            move_rows<T, false>(buf, reinterpret_cast<T*>(a.out), m0, a.M, a.ld_out, col, a.N, quarter * 32, lane);
+          __syncwarp();
+        }
+      }
+    }
+    if (leader) {
+      // after a failure: extra inputs in flight land before the shared memory goes away
+      if (*fail && loaded > 0)
+        for (int k = (loaded > 2 ? loaded - 2 : 0); k < loaded; ++k)
+          mbar_wait(smem_u32(&s_x[wg * 2 + (k & 1)]), (uint32_t)((k >> 1) & 1));
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(2 * BN)));
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Small kernels around the products.
+// ---------------------------------------------------------------------------------------
+
+// Rows of `cols` 16-bit values -> rows `ld` apart (ld a multiple of 8, so that TMA can address them).
+__global__ void pad_rows_kernel(const uint16_t* __restrict__ src, int64_t rows, int cols, int ld,
+                                uint16_t* __restrict__ dst)
+{
+  const int64_t total = rows * ld;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / ld;
+    const int c = (int)(i - r * ld);
+    dst[i] = c < cols ? src[r * cols + c] : (uint16_t)0;
+  }
+}
+
+// out[m, n] = alpha * sum over slabs in ascending order; slab rows are ld (multiple of 4) apart.
+template <typename T>
+__global__ void add_slabs_kernel(const float* __restrict__ slabs, int splits, int64_t slab_stride, int64_t rows, int cols,
+                                 int ld, float alpha, const float* __restrict__ alpha_dev, T* __restrict__ out)
+{
+  if (alpha_dev != nullptr) alpha *= __ldg(alpha_dev);
+  const int quads = ld / 4;
+  const int64_t total = rows * quads;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t r = i / quads;
+    const int c = (int)(i - r * quads) * 4;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int s = 0; s < splits; ++s) {
+      const float4 v = *reinterpret_cast<const float4*>(slabs + s * slab_stride + r * ld + c);
+      sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+    }
+    T* o = out + r * cols + c;
+    const float e[4] = {sum.x, sum.y, sum.z, sum.w};
+    if ((cols & 3) == 0) {
+      *reinterpret_cast<uint2*>(o) =
+          make_uint2(Pack<T>::two(alpha * e[0], alpha * e[1]), Pack<T>::two(alpha * e[2], alpha * e[3]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < cols) o[j] = Pack<T>::from(alpha * e[j]);
+    }
+  }
+}
+
+// Column sums of Z [rows, cols] (rows ld apart, ld a multiple of 8): block y sums its share of the
+// rows into part[y][cols]; a second kernel adds the parts in their order.
+constexpr int kColThreads = 256, kColGroup = 32;  // 32 lanes of 8 columns, 8 rows at a time
+template <typename T>
+__global__ void __launch_bounds__(kColThreads) column_sums_kernel(const T* __restrict__ Z, int64_t rows, int cols, int64_t ld,
+                                                                  float* __restrict__ part)
+{
+  __shared__ float s_sum[kColThreads / kColGroup][kColGroup * 8 + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c0 = (blockIdx.x * kColGroup + lane) * 8;
+  const int64_t r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
+  float sum[8] = {};
+  if (c0 < cols) {
+#pragma unroll 4
+    for (int64_t r = r0 + warp; r < r1; r += kColThreads / kColGroup) {
+      const uint4 v = *reinterpret_cast<const uint4*>(Z + r * ld + c0);
+      const uint32_t u[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 f = Pack<T>::get(u[e]);
+        sum[2 * e] += f.x;
+        sum[2 * e + 1] += f.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s_sum[warp][lane * 8 + e] = sum[e];
+  __syncthreads();
+  const int c = blockIdx.x * kColGroup * 8 + threadIdx.x;
+  if (c < cols) {
+    float t = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kColThreads / kColGroup; ++w) t += s_sum[w][threadIdx.x];
+    part[(int64_t)blockIdx.y * cols + c] = t;
+  }
+}
+template <typename T>
+__global__ void add_parts_kernel(const float* __restrict__ part, int parts, int cols, T* __restrict__ out)
+{
+  const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+  __shared__ float s_sum[8][33];
+  float t = 0.0f;
+  if (c < cols)
+    for (int p = w; p < parts; p += 8) t += part[(int64_t)p * cols + c];
+  s_sum[w][threadIdx.x & 31] = t;
+  __syncthreads();
+  if (w == 0 && c < cols) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) t += s_sum[i][threadIdx.x];
+    out[c] = Pack<T>::from(t);
+  }
+}
+
+// Softmax loss of 32 rows per block from the tiles' (max, sum) pairs.  Warp w first gathers every
+// 32nd tile of all 32 rows (lane = row), then finishes row w.  The target's logit is a dot product of
+// its own: with rest = log sum_{j != t} e^{s_j}, the loss log(1 + e^{rest - s_t}) of a row that has
+// learnt its target is a small number that lse - s_t would lose.  The few values per row are held in
+// 64 bits.
+template <typename T>
+__global__ void __launch_bounds__(1024) loss_rows_kernel(const float2* __restrict__ partial, int tiles, int64_t n,
+                                                         const T* __restrict__ q, int64_t ldq, const T* __restrict__ bank,
+                                                         int64_t ldb, int d, int64_t v, const int64_t* __restrict__ target,
+                                                         float scale, float* __restrict__ loss, float* __restrict__ lse)
+{
+  __shared__ float s_m[32][33], s_l[32][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t r0 = (int64_t)blockIdx.x * 32;
+  float m = -INFINITY, l = 0.0f;
+  if (r0 + lane < n) {
+    for (int t = warp; t < tiles; t += 32) {
+      const float2 p = partial[(int64_t)t * n + r0 + lane];
+      const float mn = fmaxf(m, p.x), ref = mn == -INFINITY ? 0.0f : mn;
+      l = l * ex2(m - ref) + p.y * ex2(p.x - ref);
+      m = mn;
+    }
+  }
+  s_m[warp][lane] = m;
+  s_l[warp][lane] = l;
+  __syncthreads();
+  const int64_t row = r0 + warp;
+  if (row >= n) return;
+  m = s_m[lane][warp];
+  l = s_l[lane][warp];
+  float top = m;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float ref = top == -INFINITY ? 0.0f : top;
+  l *= ex2(m - ref);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  const int64_t t = target[row];
+  const bool valid = t >= 0 && t < v;
+  double dot = 0.0;
+  if (valid)
+    for (int j = lane; j < d; j += 32)
+      dot += (double)Pack<T>::one(q[row * ldq + j]) * (double)Pack<T>::one(bank[t * ldb + j]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+  if (lane == 0) {
+    const double rest = (double)top * 0.69314718055994531 + log((double)l);  // -inf: no other row
+    double out = 0.0, total = rest;
+    if (valid) {
+      const double own = (double)scale * dot, u = rest - own;
+      out = fmax(u, 0.0) + log1p(exp(-fabs(u)));
+      if (u != u) out = u;
+      total = own + out;
+    }
+    loss[row] = (float)out;
+    lse[row] = (float)total;
+  }
+}
+
+// Largest finite |g| of the rows that take part, and the factor that the gradients return by.
+__global__ void __launch_bounds__(1024) grad_top_kernel(const float* __restrict__ g, const int64_t* __restrict__ target,
+                                                        int64_t n, int64_t v, float scale, float* __restrict__ out)
+{
+  __shared__ float s_top[32];
+  float top = 0.0f;
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    const int64_t t = target[i];
+    if (t >= 0 && t < v) top = fmaxf(top, fabsf(g[i]));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 32; ++w) top = fmaxf(top, s_top[w]);
+    out[0] = top;
+    out[1] = top * scale / kGradScale;
+  }
+}
+__global__ void grad_rows_kernel(const float* __restrict__ g, const int64_t* __restrict__ target,
+                                 const float* __restrict__ loss, const float* __restrict__ lse, int64_t n, int64_t v,
+                                 const float* __restrict__ top, float4* __restrict__ rows)
+{
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const int64_t t = target[i];
+  const float big = top[0];
+  float w = 0.0f;
+  if (t >= 0 && t < v && g[i] != 0.0f) w = g[i] / big * kGradScale;
+  rows[i] = make_float4(lse[i] * kLog2e, w, w == 0.0f ? 0.0f : expm1f(-loss[i]) * w, 0.0f);
+}
+
+// ---------------------------------------------------------------------------------------
+// Host side.
+// ---------------------------------------------------------------------------------------
+int sm_count()
+{
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  RBQ_CUDA(cudaGetDevice(&dev));
+  if (dev < 64 && (n = known[dev].load()) > 0) return n;
+  RBQ_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < 64) known[dev].store(n);
+  return n;
+}
+
+constexpr int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// A row-major matrix [rows, cols] with rows ld values apart.
+struct Matrix {
+  const void* p;
+  int64_t rows, cols, ld;
+};
+
+CUtensorMap tile_map(const void* p, CUtensorMapDataType type, int esize, int64_t rows, int64_t cols, int64_t ld, int box_cols,
+                     int box_rows)
+{
+  CUtensorMap m;
+  // The encoder is a driver call and wants the device's context bound to this host thread, which
+  // a thread that has made no runtime call yet (autograd's) lacks.
+  thread_local int bound = -1;
+  int dev = 0;
+  RBQ_CUDA(cudaGetDevice(&dev));
+  if (bound != dev) {
+    RBQ_CUDA(cudaSetDevice(dev));
+    bound = dev;
+  }
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * esize};
+  const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = tensor_map_encoder()(&m, type, 2, const_cast<void*>(p), dims, strides, box, estr,
+                                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  RBQ_CHECK(r == CUDA_SUCCESS, RBQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
+  return m;
+}
+
+template <typename T>
+constexpr CUtensorMapDataType map_type()
+{
+  return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+template <int EPI, typename T, int BN, int ACT>
+void launch_gemm(GemmArgs& a, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tx, const CUtensorMap& to,
+                 cudaStream_t s)
+{
+  using S = Shape<EPI, BN>;
+  static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit has been raised
+  int dev = 0;
+  RBQ_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !(ready.load() >> dev & 1)) {
+    RBQ_CUDA(cudaFuncSetAttribute(gemm_kernel<EPI, T, BN, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
+    if (dev < 64) ready.fetch_or(1ull << dev);
+  }
+  const int64_t total = (int64_t)a.tiles_m * a.tiles_n * a.splits;
+  const int grid = (int)std::min<int64_t>(total, sm_count());
+  gemm_kernel<EPI, T, BN, ACT><<<grid, kThreads, S::kBytes, s>>>(ta, tb, tx, to, a);
+  RBQ_LAUNCHED();
+}
+
+// One product.  A is [M, K] (or [K, M] with a_mn), B [N, K] (or [K, N] with b_mn).
+template <int EPI, typename T, int ACT = RBQ_ACT_NONE>
+void gemm(GemmArgs a, Matrix A, bool a_mn, Matrix B, bool b_mn, int bn, const CUtensorMap* tx, const CUtensorMap* to,
+          cudaStream_t s)
+{
+  a.M = a_mn ? A.cols : A.rows;
+  a.N = (int)(b_mn ? B.cols : B.rows);
+  const int64_t K = a_mn ? A.rows : A.cols;
+  a.a_mn = a_mn;
+  a.b_mn = b_mn;
+  const int64_t tm = ceil_div(a.M, kBM), tn = ceil_div(a.N, bn), kb = ceil_div(K, kBK);
+  RBQ_CHECK(tm * tn * a.splits < (1ll << 31) && kb < (1 << 30) && K < (1ll << 31) && a.M < (1ll << 31) - 128,
+            RBQ_ERR_INVALID, "matrix product: sizes too large");
+  a.tiles_m = (int)tm;
+  a.tiles_n = (int)tn;
+  a.kblocks = (int)kb;
+  a.m_fast = tm <= tn;  // the operand with fewer tiles stays in L2 while the other streams by once
+  const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  a.idesc = (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
+            ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
+  const CUtensorMap ta = tile_map(A.p, map_type<T>(), 2, A.rows, A.cols, A.ld, 64, a_mn ? kBK : kBM);
+  const CUtensorMap tb = tile_map(B.p, map_type<T>(), 2, B.rows, B.cols, B.ld, 64, b_mn ? kBK : bn);
+  const CUtensorMap& x = tx ? *tx : ta;
+  const CUtensorMap& o = to ? *to : ta;
+  if (bn == 256)
+    launch_gemm<EPI, T, 256, ACT>(a, ta, tb, x, o, s);
+  else
+    launch_gemm<EPI, T, 128, ACT>(a, ta, tb, x, o, s);
+}
+
+// Tile width: 256 columns feed the tensor cores with the fewest operand bytes; 128 where the product
+// has too few tiles to fill the SMs or no more columns.
+int tile_width(int64_t M, int64_t N, int splits = 1)
+{
+  if (N <= 128) return 128;
+  return ceil_div(M, kBM) * ceil_div(N, 256) * splits >= sm_count() ? 256 : 128;
+}
+
+// Splits along k of a slab product: the smallest estimated time, in units of one k-block's MMAs (about
+// 0.3 us on a tile).  A split costs its share of the k-blocks, about 8 units to fill and drain, and
+// 0.15 units a tile for writing its slab and reading it back.
+int plan_splits(int64_t tiles, int64_t kblocks, int most)
+{
+  const int sms = sm_count();
+  int best = 1;
+  double cost = 1e300;
+  for (int s = 1; s <= most && s <= kblocks; ++s) {
+    const double c = (double)ceil_div(tiles * s, sms) * ((double)ceil_div(kblocks, s) + 8.0) + 0.15 * tiles * s;
+    if (c < cost * 0.999) cost = c, best = s;
+  }
+  return best;
+}
+
+// Carves aligned pieces out of the caller's workspace; with no workspace it only counts.
+struct Carver {
+  char* base;
+  int64_t used = 0;
+  explicit Carver(void* p) : base(static_cast<char*>(p)) {}
+  template <typename U>
+  U* take(int64_t count)
+  {
+    U* p = base ? reinterpret_cast<U*>(base + used) : nullptr;
+    used += round_up(std::max<int64_t>(count, 1) * (int64_t)sizeof(U), 1024);
+    return p;
+  }
+};
+
+void pad_rows(const void* src, int64_t rows, int cols, int ld, void* dst, cudaStream_t s)
+{
+  const int64_t blocks = std::min<int64_t>(ceil_div(rows * ld, 256), (int64_t)sm_count() * 16);
+  pad_rows_kernel<<<(unsigned)blocks, 256, 0, s>>>(static_cast<const uint16_t*>(src), rows, cols, ld,
+                                                   static_cast<uint16_t*>(dst));
+  RBQ_LAUNCHED();
+}
+
+// The matrix itself where TMA can address its rows, else a padded copy in the workspace.
+Matrix addressable(const void* p, int64_t rows, int cols, Carver& ws, bool run, cudaStream_t s)
+{
+  if (cols % 8 == 0) return Matrix{p, rows, cols, cols};
+  const int ld = (int)round_up(cols, 8);
+  uint16_t* copy = ws.take<uint16_t>(rows * ld);
+  if (run) pad_rows(p, rows, cols, ld, copy, s);
+  return Matrix{copy, rows, cols, ld};
+}
+
+// out[M, N] = alpha * A B^T through slabs (or at once where one split is best), dense rows.
+// `slabs` of slab_floats(): null to let the caller count.
+struct SlabPlan {
+  int bn, splits;
+  int64_t rows, ld;  // of a slab
+  int64_t floats() const { return (int64_t)splits * rows * ld; }
+};
+SlabPlan plan_slabs(int64_t M, int N, int64_t K)
+{
+  SlabPlan p;
+  p.bn = N <= 128 ? 128 : 256;
+  p.splits = plan_splits(ceil_div(M, kBM) * ceil_div(N, p.bn), ceil_div(K, kBK), 64);
+  p.rows = round_up(M, kBM);
+  p.ld = round_up(N, 4);
+  while (p.splits > 1 && p.splits * p.rows >= (1ll << 31)) --p.splits;
+  return p;
+}
+template <typename T>
+void slab_gemm(const SlabPlan& p, Matrix A, bool a_mn, Matrix B, bool b_mn, float* slabs, bool add, cudaStream_t s)
+{
+  const int64_t N = b_mn ? B.cols : B.rows;
+  GemmArgs a;
+  a.splits = p.splits;
+  a.slab_rows = (int)p.rows;
+  a.slab_add = add;
+  const CUtensorMap to = tile_map(slabs, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.splits * p.rows, N, p.ld, 32, kBM);
+  gemm<kEpiSlab, T>(a, A, a_mn, B, b_mn, p.bn, nullptr, &to, s);
+}
+template <typename T>
+void add_slabs(const SlabPlan& p, const float* slabs, int64_t M, int N, float alpha, const float* alpha_dev, T* out,
+               cudaStream_t s)
+{
+  const int64_t blocks = std::min<int64_t>(ceil_div(M * (p.ld / 4), 256), (int64_t)sm_count() * 8);
+  add_slabs_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(slabs, p.splits, p.rows * p.ld, M, N, (int)p.ld, alpha, alpha_dev,
+                                                       out);
+  RBQ_LAUNCHED();
+}
+
+// out[M, N] (dense) = alpha * A B^T, written by the product's own epilogue.
+template <typename T>
+void store_gemm(Matrix A, bool a_mn, Matrix B, bool b_mn, float alpha, const float* alpha_dev, T* out, cudaStream_t s)
+{
+  const int64_t M = a_mn ? A.cols : A.rows, N = b_mn ? B.cols : B.rows;
+  GemmArgs a;
+  a.alpha = alpha;
+  a.alpha_dev = alpha_dev;
+  a.out = out;
+  a.ld_out = N;
+  a.io_tma = N % 8 == 0;
+  CUtensorMap to{};
+  if (a.io_tma) to = tile_map(out, map_type<T>(), 2, M, N, N, 64, kBM);
+  gemm<kEpiLinear, T>(a, A, a_mn, B, b_mn, tile_width(M, N), nullptr, a.io_tma ? &to : nullptr, s);
+}
+
+template <typename T>
+void linear_forward(const T* x, const T* w, const T* bias, const T* residual, T* y, int64_t m, int k, int n, int act,
+                    Carver& ws, bool run, cudaStream_t s)
+{
+  const Matrix X = addressable(x, m, k, ws, run, s), W = addressable(w, n, k, ws, run, s);
+  if (!run) return;
+  GemmArgs a;
+  a.bias = bias;
+  a.extra = residual;
+  a.has_extra = residual != nullptr;
+  a.out = y;
+  a.ld_extra = a.ld_out = n;
+  a.io_tma = n % 8 == 0;
+  CUtensorMap tx{}, to{};
+  if (a.io_tma) {
+    to = tile_map(y, map_type<T>(), 2, m, n, n, 64, kBM);
+    tx = residual ? tile_map(residual, map_type<T>(), 2, m, n, n, 64, kBM) : to;
+  }
+  const int bn = tile_width(m, n);
+  const CUtensorMap *px = a.io_tma ? &tx : nullptr, *po = a.io_tma ? &to : nullptr;
+  if (act == RBQ_ACT_GELU)
+    gemm<kEpiLinear, T, RBQ_ACT_GELU>(a, X, false, W, false, bn, px, po, s);
+  else if (act == RBQ_ACT_RELU)
+    gemm<kEpiLinear, T, RBQ_ACT_RELU>(a, X, false, W, false, bn, px, po, s);
+  else
+    gemm<kEpiLinear, T>(a, X, false, W, false, bn, px, po, s);
+}
+
+// dz = g * act'(x w^T + b) recomputes the layer's product: for the encoder's widths (k = 256) that
+// reads and writes less than keeping z, and no rounding of z enters the gradient.  dz is rounded to
+// the operands' 16 bits, as the operand of the two products dx = dz w and dw = dz^T x; the sums of
+// all of them are fp32.
+template <typename T>
+void linear_backward(const T* g, const T* x, const T* w, const T* bias, T* dx, T* dw, T* dbias, int64_t m, int k, int n,
+                     int act, Carver& ws, bool run, cudaStream_t s)
+{
+  const Matrix X = addressable(x, m, k, ws, run, s), W = addressable(w, n, k, ws, run, s);
+  Matrix Z;
+  if (act == RBQ_ACT_NONE) {
+    Z = addressable(g, m, n, ws, run, s);
+  } else {
+    const int64_t ld = round_up(n, 8);
+    T* z = ws.take<T>(m * ld);
+    Z = Matrix{z, m, n, ld};
+    if (run) {
+      GemmArgs a;
+      a.bias = bias;
+      a.extra = g;
+      a.has_extra = 1;
+      a.out = z;
+      a.ld_extra = n;
+      a.ld_out = ld;
+      a.io_tma = n % 8 == 0;
+      CUtensorMap tx{}, to{};
+      if (a.io_tma) {
+        tx = tile_map(g, map_type<T>(), 2, m, n, n, 64, kBM);
+        to = tile_map(z, map_type<T>(), 2, m, n, ld, 64, kBM);
+      }
+      const int bn = tile_width(m, n);
+      const CUtensorMap *px = a.io_tma ? &tx : nullptr, *po = a.io_tma ? &to : nullptr;
+      if (act == RBQ_ACT_GELU)
+        gemm<kEpiActGrad, T, RBQ_ACT_GELU>(a, X, false, W, false, bn, px, po, s);
+      else
+        gemm<kEpiActGrad, T, RBQ_ACT_RELU>(a, X, false, W, false, bn, px, po, s);
+    }
+  }
+  const SlabPlan plan = plan_slabs(n, k, m);
+  float* slabs = ws.take<float>(plan.floats());
+  const int gx = (int)ceil_div(n, kColGroup * 8);
+  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(m, 64), ceil_div(4 * sm_count(), gx)));
+  float* part = ws.take<float>((int64_t)parts * n);
+  if (!run) return;
+  if (dx) store_gemm<T>(Z, false, W, true, 1.0f, nullptr, dx, s);
+  if (dw) {
+    slab_gemm<T>(plan, Z, true, X, true, slabs, false, s);
+    add_slabs<T>(plan, slabs, n, k, 1.0f, nullptr, dw, s);
+  }
+  if (dbias) {
+    column_sums_kernel<T><<<dim3(gx, parts), kColThreads, 0, s>>>(static_cast<const T*>(Z.p), m, n, Z.ld, part);
+    RBQ_LAUNCHED();
+    add_parts_kernel<T><<<(unsigned)ceil_div(n, 32), 256, 0, s>>>(part, parts, n, dbias);
+    RBQ_LAUNCHED();
+  }
+}
+
+template <typename T>
+void loss_forward(const T* q, const T* bank, const int64_t* target, int64_t n, int64_t v, int d, float scale, float* loss,
+                  float* lse, Carver& ws, bool run, cudaStream_t s)
+{
+  const Matrix Q = addressable(q, n, d, ws, run, s), B = addressable(bank, v, d, ws, run, s);
+  const int bn = tile_width(n, v);
+  const int64_t tiles = ceil_div(v, bn);
+  float2* partial = ws.take<float2>(tiles * n);
+  if (!run) return;
+  GemmArgs a;
+  a.c2 = scale * kLog2e;
+  a.target = target;
+  a.partial = partial;
+  gemm<kEpiLse, T>(a, Q, false, B, false, bn, nullptr, nullptr, s);
+  loss_rows_kernel<T><<<(unsigned)ceil_div(n, 32), 1024, 0, s>>>(partial, (int)tiles, n, q, d, bank, d, d, v, target, scale,
+                                                                 loss, lse);
+  RBQ_LAUNCHED();
+}
+
+// The gradient of the logits exists one piece of the bank at a time: 16-bit values [n, piece] small
+// enough to stay in L2 (kPieceBytes) between the product that makes them and the two that read them.
+constexpr int64_t kPieceBytes = 64ll << 20;
+int64_t piece_columns(int64_t n, int64_t v)
+{
+  const int64_t most = std::max<int64_t>(256, kPieceBytes / (2 * n) / 256 * 256);
+  return round_up(ceil_div(v, ceil_div(v, most)), 256);
+}
+
+template <typename T>
+void loss_backward(const float* g, const T* q, const T* bank, const int64_t* target, const float* loss, const float* lse,
+                   int64_t n, int64_t v, int d, float scale, T* dq, T* dbank, Carver& ws, bool run, cudaStream_t s)
+{
+  const Matrix Q = addressable(q, n, d, ws, run, s), B = addressable(bank, v, d, ws, run, s);
+  const int64_t piece = std::min(piece_columns(n, v), round_up(v, 8));
+  float* top = ws.take<float>(2);
+  float4* rows = ws.take<float4>(n);
+  T* prob = ws.take<T>(n * piece);
+  const SlabPlan pq = plan_slabs(n, d, piece), pb = plan_slabs(piece, d, n);
+  float* slabs_q = ws.take<float>(pq.floats());
+  float* slabs_b = ws.take<float>(pb.floats());
+  if (!run) return;
+  grad_top_kernel<<<1, 1024, 0, s>>>(g, target, n, v, scale, top);
+  RBQ_LAUNCHED();
+  grad_rows_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(g, target, loss, lse, n, v, top, rows);
+  RBQ_LAUNCHED();
+  for (int64_t v0 = 0; v0 < v; v0 += piece) {
+    const int64_t cols = std::min(piece, v - v0);
+    const Matrix Bp{static_cast<const T*>(B.p) + v0 * B.ld, cols, d, B.ld};
+    const Matrix P{prob, n, cols, piece};
+    GemmArgs a;
+    a.c2 = scale * kLog2e;
+    a.col0 = v0;
+    a.target = target;
+    a.rows = rows;
+    const CUtensorMap to = tile_map(prob, map_type<T>(), 2, n, cols, piece, 64, kBM);
+    gemm<kEpiProb, T>(a, Q, false, Bp, false, tile_width(n, cols), nullptr, &to, s);
+    if (dq) {
+      SlabPlan p = pq;  // the last, shorter piece keeps the slabs; no split may be empty
+      const int64_t kb = ceil_div(cols, kBK);
+      if (p.splits > kb) p.splits = (int)kb;
+      slab_gemm<T>(p, P, false, Bp, true, slabs_q, v0 > 0, s);
+    }
+    if (dbank) {
+      SlabPlan p = pb;
+      p.rows = round_up(cols, kBM);
+      slab_gemm<T>(p, P, true, Q, true, slabs_b, false, s);
+      add_slabs<T>(p, slabs_b, cols, d, 1.0f, top + 1, dbank + v0 * d, s);
+    }
+  }
+  if (dq) add_slabs<T>(pq, slabs_q, n, d, 1.0f, top + 1, dq, s);
+}
+
+}  // namespace
+
+// ---------------------------------------------------------------------------------------
+// Launchers (arguments checked by the C ABI).  With ws == nullptr they launch nothing and return
+// the workspace they need.
+// ---------------------------------------------------------------------------------------
+int64_t launch_linear(const void* x, const void* w, const void* bias, const void* residual, void* y, int64_t m, int k, int n,
+                      int dtype, int act, void* ws, bool run, cudaStream_t s)
+{
+  Carver c(ws);
+  if (dtype == RBQ_F16)
+    linear_forward<__half>((const __half*)x, (const __half*)w, (const __half*)bias, (const __half*)residual, (__half*)y, m, k,
+                           n, act, c, run, s);
+  else
+    linear_forward<__nv_bfloat16>((const __nv_bfloat16*)x, (const __nv_bfloat16*)w, (const __nv_bfloat16*)bias,
+                                  (const __nv_bfloat16*)residual, (__nv_bfloat16*)y, m, k, n, act, c, run, s);
+  return c.used;
+}
+
+int64_t launch_linear_backward(const void* g, const void* x, const void* w, const void* bias, void* dx, void* dw, void* dbias,
+                               int64_t m, int k, int n, int dtype, int act, void* ws, bool run, cudaStream_t s)
+{
+  Carver c(ws);
+  if (dtype == RBQ_F16)
+    linear_backward<__half>((const __half*)g, (const __half*)x, (const __half*)w, (const __half*)bias, (__half*)dx,
+                            (__half*)dw, (__half*)dbias, m, k, n, act, c, run, s);
+  else
+    linear_backward<__nv_bfloat16>((const __nv_bfloat16*)g, (const __nv_bfloat16*)x, (const __nv_bfloat16*)w,
+                                   (const __nv_bfloat16*)bias, (__nv_bfloat16*)dx, (__nv_bfloat16*)dw,
+                                   (__nv_bfloat16*)dbias, m, k, n, act, c, run, s);
+  return c.used;
+}
+
+int64_t launch_softmax_loss(const void* q, const void* bank, const int64_t* target, int64_t n, int64_t v, int d, float scale,
+                            int dtype, float* loss, float* lse, void* ws, bool run, cudaStream_t s)
+{
+  Carver c(ws);
+  if (dtype == RBQ_F16)
+    loss_forward<__half>((const __half*)q, (const __half*)bank, target, n, v, d, scale, loss, lse, c, run, s);
+  else
+    loss_forward<__nv_bfloat16>((const __nv_bfloat16*)q, (const __nv_bfloat16*)bank, target, n, v, d, scale, loss, lse, c,
+                                run, s);
+  return c.used;
+}
+
+int64_t launch_softmax_loss_backward(const float* g, const void* q, const void* bank, const int64_t* target,
+                                     const float* loss, const float* lse, int64_t n, int64_t v, int d, float scale, int dtype,
+                                     void* dq, void* dbank, void* ws, bool run, cudaStream_t s)
+{
+  Carver c(ws);
+  if (dtype == RBQ_F16)
+    loss_backward<__half>(g, (const __half*)q, (const __half*)bank, target, loss, lse, n, v, d, scale, (__half*)dq,
+                          (__half*)dbank, c, run, s);
+  else
+    loss_backward<__nv_bfloat16>(g, (const __nv_bfloat16*)q, (const __nv_bfloat16*)bank, target, loss, lse, n, v, d, scale,
+                                 (__nv_bfloat16*)dq, (__nv_bfloat16*)dbank, c, run, s);
+  return c.used;
+}
+
+int take_op_error()
+{
+  int code = 0;
+  RBQ_CUDA(cudaMemcpyFromSymbol(&code, g_op_err, sizeof(int)));
+  if (code) {
+    const int zero = 0;
+    RBQ_CUDA(cudaMemcpyToSymbol(g_op_err, &zero, sizeof(int)));
+  }
+  return code;
+}
+
+}  // namespace rbq

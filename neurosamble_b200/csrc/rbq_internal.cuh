@@ -431,4 +431,26 @@ void launch_gen_mixture(float* X, int64_t n, int D, int n_centres, float sigma, 
 void launch_gen_queries(const float* X, int64_t n, int D, float* Q, int64_t nq, float sigma, int normalize,
                         uint64_t seed, uint32_t stream, int64_t* src_rows, cudaStream_t s);
 
+// ---------------------------------------------------------------------------------------
+// Operators of the read encoder (rbq_gemm.cu, rbq_norm.cu).  Arguments are checked by the C ABI; the
+// first four return the bytes of workspace they use and launch only with `run`.
+// ---------------------------------------------------------------------------------------
+int64_t launch_linear(const void* x, const void* w, const void* bias, const void* residual, void* y, int64_t m, int k, int n,
+                      int dtype, int act, void* ws, bool run, cudaStream_t s);
+int64_t launch_linear_backward(const void* g, const void* x, const void* w, const void* bias, void* dx, void* dw, void* dbias,
+                               int64_t m, int k, int n, int dtype, int act, void* ws, bool run, cudaStream_t s);
+int64_t launch_softmax_loss(const void* q, const void* bank, const int64_t* target, int64_t n, int64_t v, int d, float scale,
+                            int dtype, float* loss, float* lse, void* ws, bool run, cudaStream_t s);
+int64_t launch_softmax_loss_backward(const float* g, const void* q, const void* bank, const int64_t* target,
+                                     const float* loss, const float* lse, int64_t n, int64_t v, int d, float scale, int dtype,
+                                     void* dq, void* dbank, void* ws, bool run, cudaStream_t s);
+// Returns and clears the current device's error code of the products above (synchronises).
+int take_op_error();
+void launch_layer_norm(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows, int d,
+                       float eps, int dtype, int param_dtype, cudaStream_t s);
+int64_t layer_norm_workspace(int64_t rows, int d);
+void launch_layer_norm_backward(const void* g, const void* x, const void* w, const float* mean, const float* rstd, void* dx,
+                                void* dw, void* db, float* part, int64_t rows, int d, int dtype, int param_dtype,
+                                cudaStream_t s);
+
 }  // namespace rbq

@@ -1,0 +1,483 @@
+// Layer norm over the last dimension, forward and backward (sm_100a).
+//
+//   xhat = (x - mean) * rstd,  rstd = 1 / sqrt(mean((x - mean)^2) + eps),  y = xhat * w + b
+//   dx = rstd * (gw - mean(gw) - xhat * mean(gw * xhat)),  gw = g * w
+//   dw = sum over rows of g * xhat,  db = sum over rows of g
+//
+// Both passes are bound by HBM: x (and g) are read once, y (or dx) written once.  A row lives in the
+// registers of the threads that share it (a part of a warp, a warp, or a block for wide rows), so the
+// variance is the two-pass one, over differences from the mean.  The backward pass keeps each
+// thread's share of dw and db in registers over all the rows that it sees; a block adds its groups
+// in a fixed order and writes one partial row, and a second kernel adds the blocks' rows in theirs, so
+// the gradients do not depend on timing.  All sums are fp32; the values are rounded once, on output.
+// Rows wider than the register paths hold take loops that read the row once per pass.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include <algorithm>
+#include <atomic>
+#include <initializer_list>
+
+#include "rbq_internal.cuh"
+
+namespace rbq {
+namespace {
+
+constexpr int kNormThreads = 256;
+
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int VEC>
+struct alignas(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) Vec {
+  T e[VEC];
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC])
+{
+  const Vec<T, VEC> x = *reinterpret_cast<const Vec<T, VEC>*>(p);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = to_f(x.e[i]);
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC])
+{
+  Vec<T, VEC> x;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) x.e[i] = from_f<T>(v[i]);
+  *reinterpret_cast<Vec<T, VEC>*>(p) = x;
+}
+
+// Sum over the TPR threads that share a row (TPR = kNormThreads: the block).
+template <int TPR>
+__device__ __forceinline__ float row_sum(float v, float* s_red)
+{
+  if (TPR <= 32) {
+#pragma unroll
+    for (int o = TPR / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  __syncthreads();  // the last sum has been read
+  if ((threadIdx.x & 31) == 0) s_red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  float t = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kNormThreads / 32; ++w) t += s_red[w];
+  return t;
+}
+
+// One row per TPR threads; thread i of a row holds CH pieces of VEC values, piece c at column
+// (c * TPR + i) * VEC.
+template <typename T, typename P, int VEC, int CH, int TPR>
+__global__ void __launch_bounds__(kNormThreads)
+    norm_kernel(const T* __restrict__ x, const P* __restrict__ w, const P* __restrict__ b, T* __restrict__ y,
+                float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int d, float eps)
+{
+  __shared__ float s_red[kNormThreads / 32];
+  constexpr int kRows = kNormThreads / TPR;
+  const int i = threadIdx.x % TPR;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  // whole warps run every round, so that the shuffles see all lanes
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += step) {
+    const int64_t r = r0 + threadIdx.x / TPR;
+    const bool live = r < rows;
+    float v[CH][VEC];
+    float sum = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = (c * TPR + i) * VEC;
+      if (live && col < d) {
+        load_vec<T, VEC>(x + r * d + col, v[c]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[c][e] = 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum += v[c][e];
+    }
+    const float mean = row_sum<TPR>(sum, s_red) / (float)d;
+    float sq = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      if ((c * TPR + i) * VEC < d) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          v[c][e] -= mean;
+          sq = fmaf(v[c][e], v[c][e], sq);
+        }
+      }
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<TPR>(sq, s_red) / (float)d + eps);
+    if (live) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = (c * TPR + i) * VEC;
+        if (col < d) {
+          float wv[VEC], bv[VEC];
+          load_vec<P, VEC>(w + col, wv);
+          load_vec<P, VEC>(b + col, bv);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) v[c][e] = fmaf(v[c][e] * rstd, wv[e], bv[e]);
+          store_vec<T, VEC>(y + r * d + col, v[c]);
+        }
+      }
+      if (i == 0) {
+        mean_out[r] = mean;
+        rstd_out[r] = rstd;
+      }
+    }
+  }
+}
+
+// part[block][2][d]: this block's share of dw and db.
+template <typename T, typename P, int VEC, int CH, int TPR>
+__global__ void __launch_bounds__(kNormThreads)
+    norm_grad_kernel(const T* __restrict__ g, const T* __restrict__ x, const P* __restrict__ w,
+                     const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx,
+                     float* __restrict__ part, int64_t rows, int d)
+{
+  extern __shared__ float s_part[];  // [2][d], rows shared by TPR < kNormThreads threads only
+  __shared__ float s_red[kNormThreads / 32];
+  constexpr int kRows = kNormThreads / TPR;
+  const int i = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  float dw[CH][VEC], db[CH][VEC];
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) dw[c][e] = db[c][e] = 0.0f;
+  for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += step) {
+    const int64_t r = r0 + group;
+    const bool live = r < rows;
+    const float mean = live ? __ldg(mean_in + r) : 0.0f, rstd = live ? __ldg(rstd_in + r) : 0.0f;
+    float xh[CH][VEC], gw[CH][VEC];
+    float a = 0.0f, b = 0.0f;
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = (c * TPR + i) * VEC;
+      if (live && col < d) {
+        load_vec<T, VEC>(x + r * d + col, xh[c]);
+        load_vec<T, VEC>(g + r * d + col, gw[c]);
+        float wv[VEC];
+        load_vec<P, VEC>(w + col, wv);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          xh[c][e] = (xh[c][e] - mean) * rstd;
+          dw[c][e] = fmaf(gw[c][e], xh[c][e], dw[c][e]);
+          db[c][e] += gw[c][e];
+          gw[c][e] *= wv[e];
+          a += gw[c][e];
+          b = fmaf(gw[c][e], xh[c][e], b);
+        }
+      }
+    }
+    if (dx == nullptr) continue;
+    a = row_sum<TPR>(a, s_red) / (float)d;
+    b = row_sum<TPR>(b, s_red) / (float)d;
+    if (live) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = (c * TPR + i) * VEC;
+        if (col < d) {
+          float o[VEC];
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) o[e] = rstd * (gw[c][e] - a - xh[c][e] * b);
+          store_vec<T, VEC>(dx + r * d + col, o);
+        }
+      }
+    }
+  }
+  if (part == nullptr) return;
+  float* out = part + (int64_t)blockIdx.x * 2 * d;
+  if (TPR == kNormThreads) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = (c * TPR + i) * VEC;
+      if (col < d) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          out[col + e] = dw[c][e];
+          out[d + col + e] = db[c][e];
+        }
+      }
+    }
+    return;
+  }
+  for (int k = 0; k < kRows; ++k) {  // the groups in their order
+    if (group == k) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int col = (c * TPR + i) * VEC;
+        if (col < d) {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) {
+            s_part[col + e] = (k ? s_part[col + e] : 0.0f) + dw[c][e];
+            s_part[d + col + e] = (k ? s_part[d + col + e] : 0.0f) + db[c][e];
+          }
+        }
+      }
+    }
+    __syncthreads();
+  }
+  for (int j = threadIdx.x; j < 2 * d; j += kNormThreads) out[j] = s_part[j];
+}
+
+// Rows wider than the register paths: a block per row, the row read once per pass.
+template <typename T, typename P>
+__global__ void __launch_bounds__(kNormThreads)
+    norm_wide_kernel(const T* __restrict__ x, const P* __restrict__ w, const P* __restrict__ b, T* __restrict__ y,
+                     float* __restrict__ mean_out, float* __restrict__ rstd_out, int64_t rows, int d, float eps)
+{
+  __shared__ float s_red[kNormThreads / 32];
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const T* xr = x + r * d;
+    float sum = 0.0f, sq = 0.0f;
+    for (int j = threadIdx.x; j < d; j += kNormThreads) sum += to_f(xr[j]);
+    const float mean = row_sum<kNormThreads>(sum, s_red) / (float)d;
+    for (int j = threadIdx.x; j < d; j += kNormThreads) {
+      const float c = to_f(xr[j]) - mean;
+      sq = fmaf(c, c, sq);
+    }
+    const float rstd = 1.0f / sqrtf(row_sum<kNormThreads>(sq, s_red) / (float)d + eps);
+    for (int j = threadIdx.x; j < d; j += kNormThreads)
+      y[r * d + j] = from_f<T>(fmaf((to_f(xr[j]) - mean) * rstd, to_f(w[j]), to_f(b[j])));
+    if (threadIdx.x == 0) {
+      mean_out[r] = mean;
+      rstd_out[r] = rstd;
+    }
+  }
+}
+template <typename T, typename P>
+__global__ void __launch_bounds__(kNormThreads)
+    norm_wide_grad_kernel(const T* __restrict__ g, const T* __restrict__ x, const P* __restrict__ w,
+                          const float* __restrict__ mean_in, const float* __restrict__ rstd_in, T* __restrict__ dx,
+                          int64_t rows, int d)
+{
+  __shared__ float s_red[kNormThreads / 32];
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const T *xr = x + r * d, *gr = g + r * d;
+    const float mean = mean_in[r], rstd = rstd_in[r];
+    float a = 0.0f, b = 0.0f;
+    for (int j = threadIdx.x; j < d; j += kNormThreads) {
+      const float gw = to_f(gr[j]) * to_f(w[j]);
+      a += gw;
+      b = fmaf(gw, (to_f(xr[j]) - mean) * rstd, b);
+    }
+    a = row_sum<kNormThreads>(a, s_red) / (float)d;
+    b = row_sum<kNormThreads>(b, s_red) / (float)d;
+    for (int j = threadIdx.x; j < d; j += kNormThreads) {
+      const float gw = to_f(gr[j]) * to_f(w[j]);
+      dx[r * d + j] = from_f<T>(rstd * (gw - a - (to_f(xr[j]) - mean) * rstd * b));
+    }
+  }
+}
+// Shares of dw and db of such rows: thread = column, block y = a share of the rows.
+template <typename T>
+__global__ void __launch_bounds__(kNormThreads)
+    norm_wide_sums_kernel(const T* __restrict__ g, const T* __restrict__ x, const float* __restrict__ mean_in,
+                          const float* __restrict__ rstd_in, float* __restrict__ part, int64_t rows, int d)
+{
+  const int64_t c = (int64_t)blockIdx.x * kNormThreads + threadIdx.x;
+  if (c >= d) return;
+  float dw = 0.0f, db = 0.0f;
+  for (int64_t r = rows * blockIdx.y / gridDim.y, e = rows * (blockIdx.y + 1) / gridDim.y; r < e; ++r) {
+    const float gv = to_f(g[r * d + c]);
+    dw = fmaf(gv, (to_f(x[r * d + c]) - __ldg(mean_in + r)) * __ldg(rstd_in + r), dw);
+    db += gv;
+  }
+  part[(int64_t)blockIdx.y * 2 * d + c] = dw;
+  part[(int64_t)blockIdx.y * 2 * d + d + c] = db;
+}
+
+// dw and db from the blocks' shares, in the blocks' order within each of 8 interleaved runs.
+template <typename P>
+__global__ void norm_parts_kernel(const float* __restrict__ part, int parts, int d, P* __restrict__ dw, P* __restrict__ db)
+{
+  __shared__ float s_sum[8][33];
+  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float t = 0.0f;
+  if (c < 2 * (int64_t)d) {
+#pragma unroll 4
+    for (int p = run; p < parts; p += 8) t += part[(int64_t)p * 2 * d + c];
+  }
+  s_sum[run][lane] = t;
+  __syncthreads();
+  if (run == 0 && c < 2 * (int64_t)d) {
+#pragma unroll
+    for (int k = 1; k < 8; ++k) t += s_sum[k][lane];
+    if (c < d) {
+      if (dw != nullptr) dw[c] = from_f<P>(t);
+    } else if (db != nullptr) {
+      db[c - d] = from_f<P>(t);
+    }
+  }
+}
+
+int sms()
+{
+  static std::atomic<int> known[64];
+  int dev = 0, n = 0;
+  RBQ_CUDA(cudaGetDevice(&dev));
+  if (dev < 64 && (n = known[dev].load()) > 0) return n;
+  RBQ_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+  if (dev < 64) known[dev].store(n);
+  return n;
+}
+
+// How a row is shared: vec values per load (16 bytes, or one where the width or an address does not
+// allow that), tpr threads per row, ch loads per thread; tpr = 0: wider than the register paths.
+struct Plan {
+  int vec, tpr, ch;
+};
+Plan plan_of(int d, int esize, bool vector)
+{
+  const int vec = vector ? 16 / esize : 1;
+  const int loads = (d + vec - 1) / vec;
+  if (vector) {
+    if (loads <= 8) return {vec, 8, 1};
+    if (loads <= 32) return {vec, 32, 1};
+    if (loads <= 64) return {vec, 32, 2};
+    if (loads <= 128) return {vec, 32, 4};
+    if (loads <= 4 * kNormThreads) return {vec, kNormThreads, 4};
+  } else {
+    if (loads <= 256) return {vec, 32, 8};
+    if (loads <= 1024) return {vec, 32, 32};
+    if (loads <= 32 * kNormThreads) return {vec, kNormThreads, 32};
+  }
+  return {vec, 0, 0};
+}
+
+int grad_blocks(const Plan& p, int64_t rows)
+{
+  const int64_t per = p.tpr ? kNormThreads / p.tpr : 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, per), (int64_t)sms() * 4));
+}
+
+template <typename T, typename P>
+void run_forward(const T* x, const P* w, const P* b, T* y, float* mean, float* rstd, int64_t rows, int d, float eps,
+                 bool vector, cudaStream_t s)
+{
+  const Plan p = plan_of(d, (int)sizeof(T), vector);
+  constexpr int V = 16 / (int)sizeof(T);
+  const int64_t per = p.tpr ? kNormThreads / p.tpr : 1;
+  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(rows, per), (int64_t)sms() * 32);
+#define RBQ_NORM(VEC, CH, TPR) norm_kernel<T, P, VEC, CH, TPR><<<grid, kNormThreads, 0, s>>>(x, w, b, y, mean, rstd, rows, d, eps)
+  if (p.tpr == 0)
+    norm_wide_kernel<T, P><<<grid, kNormThreads, 0, s>>>(x, w, b, y, mean, rstd, rows, d, eps);
+  else if (p.vec == 1 && p.tpr == 32)
+    p.ch == 8 ? RBQ_NORM(1, 8, 32) : RBQ_NORM(1, 32, 32);
+  else if (p.vec == 1)
+    RBQ_NORM(1, 32, kNormThreads);
+  else if (p.tpr == 8)
+    RBQ_NORM(V, 1, 8);
+  else if (p.tpr == 32)
+    p.ch == 1 ? RBQ_NORM(V, 1, 32) : p.ch == 2 ? RBQ_NORM(V, 2, 32) : RBQ_NORM(V, 4, 32);
+  else
+    RBQ_NORM(V, 4, kNormThreads);
+#undef RBQ_NORM
+  RBQ_LAUNCHED();
+}
+
+template <typename T, typename P>
+void run_backward(const T* g, const T* x, const P* w, const float* mean, const float* rstd, T* dx, P* dw, P* db, float* part,
+                  int64_t rows, int d, bool vector, cudaStream_t s)
+{
+  const Plan p = plan_of(d, (int)sizeof(T), vector);
+  constexpr int V = 16 / (int)sizeof(T);
+  const int blocks = grad_blocks(p, rows);
+  const bool sums = dw != nullptr || db != nullptr;
+  float* out = sums ? part : nullptr;
+  const size_t smem = sums && p.tpr && p.tpr < kNormThreads ? (size_t)2 * d * sizeof(float) : 0;
+#define RBQ_NORM(VEC, CH, TPR) \
+  norm_grad_kernel<T, P, VEC, CH, TPR><<<blocks, kNormThreads, smem, s>>>(g, x, w, mean, rstd, dx, out, rows, d)
+  if (p.tpr == 0) {
+    if (dx != nullptr) {
+      norm_wide_grad_kernel<T, P><<<blocks, kNormThreads, 0, s>>>(g, x, w, mean, rstd, dx, rows, d);
+      RBQ_LAUNCHED();
+    }
+    if (sums) {
+      norm_wide_sums_kernel<T><<<dim3((unsigned)ceil_div(d, kNormThreads), blocks), kNormThreads, 0, s>>>(
+          g, x, mean, rstd, part, rows, d);
+      RBQ_LAUNCHED();
+    }
+  } else {
+    if (p.vec == 1 && p.tpr == 32)
+      p.ch == 8 ? RBQ_NORM(1, 8, 32) : RBQ_NORM(1, 32, 32);
+    else if (p.vec == 1)
+      RBQ_NORM(1, 32, kNormThreads);
+    else if (p.tpr == 8)
+      RBQ_NORM(V, 1, 8);
+    else if (p.tpr == 32)
+      p.ch == 1 ? RBQ_NORM(V, 1, 32) : p.ch == 2 ? RBQ_NORM(V, 2, 32) : RBQ_NORM(V, 4, 32);
+    else
+      RBQ_NORM(V, 4, kNormThreads);
+    RBQ_LAUNCHED();
+  }
+#undef RBQ_NORM
+  if (sums) {
+    norm_parts_kernel<P><<<(unsigned)ceil_div(2 * (int64_t)d, 32), 256, 0, s>>>(part, blocks, d, dw, db);
+    RBQ_LAUNCHED();
+  }
+}
+
+bool aligned16(std::initializer_list<const void*> ps)
+{
+  for (const void* p : ps)
+    if (reinterpret_cast<uintptr_t>(p) & 15u) return false;
+  return true;
+}
+
+}  // namespace
+
+// Parameters are of the rows' type or fp32.  16-byte loads need a width of whole loads (of fp32
+// parameters too: twice as many bytes) and aligned addresses; else one value at a time.
+void launch_layer_norm(const void* x, const void* w, const void* b, void* y, float* mean, float* rstd, int64_t rows, int d,
+                       float eps, int dtype, int param_dtype, cudaStream_t s)
+{
+  const bool vec = d % (dtype == RBQ_F32 ? 4 : 8) == 0 && aligned16({x, w, b, y});
+#define RBQ_RUN(T, P) run_forward<T, P>((const T*)x, (const P*)w, (const P*)b, (T*)y, mean, rstd, rows, d, eps, vec, s)
+  if (dtype == RBQ_F32)
+    RBQ_RUN(float, float);
+  else if (dtype == RBQ_F16)
+    param_dtype == RBQ_F32 ? RBQ_RUN(__half, float) : RBQ_RUN(__half, __half);
+  else
+    param_dtype == RBQ_F32 ? RBQ_RUN(__nv_bfloat16, float) : RBQ_RUN(__nv_bfloat16, __nv_bfloat16);
+#undef RBQ_RUN
+}
+
+int64_t layer_norm_workspace(int64_t rows, int d)
+{
+  // the most blocks any way of sharing a row takes
+  return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)sms() * 4)) * 2 * d * (int64_t)sizeof(float);
+}
+
+void launch_layer_norm_backward(const void* g, const void* x, const void* w, const float* mean, const float* rstd, void* dx,
+                                void* dw, void* db, float* part, int64_t rows, int d, int dtype, int param_dtype,
+                                cudaStream_t s)
+{
+  const bool vec = d % (dtype == RBQ_F32 ? 4 : 8) == 0 && aligned16({g, x, w, dx});
+#define RBQ_RUN(T, P) \
+  run_backward<T, P>((const T*)g, (const T*)x, (const P*)w, mean, rstd, (T*)dx, (P*)dw, (P*)db, part, rows, d, vec, s)
+  if (dtype == RBQ_F32)
+    RBQ_RUN(float, float);
+  else if (dtype == RBQ_F16)
+    param_dtype == RBQ_F32 ? RBQ_RUN(__half, float) : RBQ_RUN(__half, __half);
+  else
+    param_dtype == RBQ_F32 ? RBQ_RUN(__nv_bfloat16, float) : RBQ_RUN(__nv_bfloat16, __nv_bfloat16);
+#undef RBQ_RUN
+}
+
+}  // namespace rbq
