@@ -10,6 +10,7 @@ import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "librbq.so")
+TORCH_LIB_PATH = os.path.join(_HERE, "_lib", "librbq_torch.so")  # PyTorch operators over the C ABI
 
 RBQ_OK = 0
 ERRORS = {1: "invalid argument", 2: "CUDA error", 3: "out of device memory", 4: "I/O error",
@@ -42,7 +43,6 @@ class IndexInfo(ctypes.Structure):
 SHARD_POLICIES = {"round_robin": 0, "balanced": 1}
 KMEANS_KINDS = {"balanced": 0, "lloyd": 1}
 RAW_STORES = {"device": 0, "host": 1}
-ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2}
 
 
 # name -> argtypes (all functions return int status unless listed in _RESTYPES)

@@ -1,4 +1,5 @@
-"""Build librbq.so (the C-ABI CUDA library) in-tree for sm_100a.
+"""Build librbq.so (the C-ABI CUDA library) in-tree for sm_100a, and librbq_torch.so (PyTorch operators
+over it) beside it.
 
 Usage: ``python -m neurosamble_b200.build_ext`` (or ``build()`` from Python).  The shared
 library lands in ``neurosamble_b200/_lib/librbq.so`` so it travels with the source tree.
@@ -15,9 +16,11 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "librbq.so")
+TORCH_LIB = os.path.join(OUT_DIR, "librbq_torch.so")
 
 SOURCES = ["rbq_host_math.cpp", "rbq_build.cu", "rbq_search.cu", "rbq_coarse_tc.cu", "rbq_gemm.cu", "rbq_norm.cu",
            "rbq_capi.cu"]
+TORCH_SOURCE = "rbq_torch.cpp"  # PyTorch operators over the C ABI; a library of its own, so that C users need no torch
 HEADERS = ["rbq_internal.cuh", "rbq_tc.cuh", os.path.join("..", "..", "include", "rbq.h")]
 
 # -fmad=false: no FMA contraction anywhere, so every expression is evaluated as written and
@@ -45,11 +48,26 @@ def _cxx() -> str:
     raise RuntimeError("g++ not found")
 
 
+def build_torch(env: dict) -> None:
+    """Compile the PyTorch operators against the running torch's headers and link them to librbq.so beside them."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    include = os.path.join(root, "include")
+    tmp = TORCH_LIB + ".tmp"
+    subprocess.run([_cxx(), "-std=c++17", "-O2", "-fPIC", "-shared",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + include,
+                    "-I" + os.path.join(include, "torch", "csrc", "api", "include"), "-I/usr/local/cuda/include",
+                    os.path.join(CSRC, TORCH_SOURCE), "-o", tmp, "-L" + os.path.join(root, "lib"), "-L" + OUT_DIR,
+                    "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-lrbq", "-Wl,-rpath,$ORIGIN"],
+                   check=True, env=env)
+    os.replace(tmp, TORCH_LIB)
+
+
 def _stale() -> bool:
-    if not os.path.exists(LIB):
+    if not os.path.exists(LIB) or not os.path.exists(TORCH_LIB):
         return True
-    t = os.path.getmtime(LIB)
-    for f in SOURCES + HEADERS:
+    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_LIB))
+    for f in SOURCES + HEADERS + [TORCH_SOURCE]:
         if os.path.getmtime(os.path.join(CSRC, f)) > t:
             return True
     return False
@@ -86,6 +104,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.replace(tmp, LIB)
     for o in objs:
         os.remove(o)
+    build_torch(env)
     return LIB
 
 

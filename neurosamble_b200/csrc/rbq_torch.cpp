@@ -1,0 +1,537 @@
+// torch.ops.rbq.linear, layer_norm and softmax_loss over the C ABI of librbq.so: definitions, checks
+// of arguments, shapes for meta and fake tensors, and gradients.
+//
+// They are registered from C++ because a training step calls them hundreds of times on small inputs
+// and is then bound by the host: through Python's custom operators a forward and backward pair took the
+// host 230 us, through Python autograd functions 160 us, whatever the sizes.
+//
+// The kernel behind every operator is registered for all devices and refuses what is not on CUDA, so
+// that a host tensor gets the library's message.  Work goes to the current stream of the input's device;
+// nothing synchronises.  Inputs are made dense and moved to a 16-byte boundary where they are not.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/library.h>
+
+#include <array>
+#include <initializer_list>
+#include <memory>
+#include <optional>
+#include <string>
+#include <tuple>
+#include <vector>
+
+#include "../../include/rbq.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using OptTensor = std::optional<Tensor>;
+
+void call(int status)
+{
+  static const char* kNames[] = {"ok", "invalid argument", "CUDA error", "out of device memory", "I/O error",
+                                 "wrong call order", "malformed index file"};
+  TORCH_CHECK(status == RBQ_OK, "rbq error ", status, " (", status >= 0 && status < 7 ? kNames[status] : "?", "): ",
+              rbq_last_error());
+}
+
+std::string type_name(at::ScalarType t)
+{
+  switch (t) {
+    case at::kHalf: return "torch.float16";
+    case at::kBFloat16: return "torch.bfloat16";
+    case at::kFloat: return "torch.float32";
+    case at::kDouble: return "torch.float64";
+    case at::kLong: return "torch.int64";
+    case at::kInt: return "torch.int32";
+    default: return std::string("torch.") + c10::toString(t);
+  }
+}
+
+int type_code(at::ScalarType t) { return t == at::kHalf ? RBQ_F16 : t == at::kBFloat16 ? RBQ_BF16 : RBQ_F32; }
+
+// t of the given type on like's device, dense and on a 16-byte boundary.
+Tensor operand(const Tensor& t, const Tensor& like, at::ScalarType type, const char* name)
+{
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), "rbq: ", name, " must be a CUDA tensor on ", like.device(),
+              ", got ", t.device());
+  TORCH_CHECK(t.scalar_type() == type, "rbq: ", name, " must be ", type_name(type), ", got ", type_name(t.scalar_type()));
+  Tensor d = t.contiguous();
+  return reinterpret_cast<uintptr_t>(d.const_data_ptr()) % 16 == 0 ? d : d.clone();
+}
+
+Tensor first(const Tensor& t, bool f32_too, const char* name)
+{
+  TORCH_CHECK(t.is_cuda(), "rbq: ", name, " must be a CUDA tensor");
+  const auto s = t.scalar_type();
+  TORCH_CHECK(s == at::kHalf || s == at::kBFloat16 || (f32_too && s == at::kFloat), "rbq: ", name,
+              " must be torch.float16 or torch.bfloat16", f32_too ? " or torch.float32" : "", ", got ", type_name(s));
+  return operand(t, t, s, name);
+}
+
+void check_shape(const Tensor& t, at::IntArrayRef want, const char* name)
+{
+  TORCH_CHECK(t.sizes() == want, "rbq: ", name, " must have shape ", want, ", got ", t.sizes());
+}
+
+void* data(const Tensor& t) { return t.defined() ? const_cast<void*>(t.const_data_ptr()) : nullptr; }
+void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
+Tensor scratch(const Tensor& like, int64_t bytes)
+{
+  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+Tensor empty_if(bool need, const Tensor& like) { return need ? at::empty_like(like) : at::empty({0}, like.options()); }
+
+bool wants_grad(std::initializer_list<Tensor> ts)
+{
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor& t : ts)
+    if (t.defined() && t.requires_grad()) return true;
+  return false;
+}
+
+// An output whose own gradient is refused (the backward passes are not differentiable again).
+template <size_t N>
+std::array<Tensor, N> once(std::array<Tensor, N> out, const char* name)
+{
+  if (!at::GradMode::is_enabled()) return out;
+  variable_list in;
+  for (Tensor& t : out)
+    if (t.defined() && t.numel() > 0) {
+      t = t.detach();
+      t.requires_grad_();
+      in.push_back(t);
+    }
+  if (in.empty()) return out;
+  auto fn = std::make_shared<torch::autograd::DelayedError>(
+      std::string("rbq: the gradient of ") + name + " cannot be differentiated again", (int64_t)in.size());
+  variable_list wrapped = (*fn)(std::move(in));
+  size_t i = 0;
+  for (Tensor& t : out)
+    if (t.defined() && t.numel() > 0) t = wrapped[i++];
+  return out;
+}
+
+// ---- linear ------------------------------------------------------------------------------------
+struct LinearArgs {
+  Tensor x, w, bias;
+  int64_t m, k, n;
+  int act, type;
+};
+
+int activation(c10::string_view act)
+{
+  if (act == "none") return RBQ_ACT_NONE;
+  if (act == "relu") return RBQ_ACT_RELU;
+  if (act == "gelu") return RBQ_ACT_GELU;
+  TORCH_CHECK(false, "rbq: act must be one of none, relu, gelu, got '", std::string(act), "'");
+}
+
+LinearArgs linear_args(const Tensor& x, const Tensor& w, const OptTensor& bias, c10::string_view act)
+{
+  LinearArgs a;
+  a.x = first(x, false, "x");
+  a.w = operand(w, a.x, a.x.scalar_type(), "w");
+  TORCH_CHECK(x.dim() >= 1 && w.dim() == 2 && x.size(-1) == w.size(1), "rbq: linear takes x [..., k] and w [n, k], got ",
+              x.sizes(), " and ", w.sizes());
+  a.n = w.size(0);
+  a.k = w.size(1);
+  TORCH_CHECK(a.n >= 1 && a.k >= 1, "rbq: linear needs k >= 1 and n >= 1");
+  TORCH_CHECK(a.n < (1ll << 31) && a.k < (1ll << 31), "rbq: linear: bad sizes");
+  if (bias.has_value() && bias->defined()) {
+    a.bias = operand(*bias, a.x, a.x.scalar_type(), "bias");
+    check_shape(a.bias, {a.n}, "bias");
+  }
+  a.act = activation(act);
+  a.m = a.x.numel() / a.k;
+  a.type = type_code(a.x.scalar_type());
+  return a;
+}
+
+std::vector<int64_t> with_last(const Tensor& x, int64_t n)
+{
+  std::vector<int64_t> s = x.sizes().vec();
+  s.back() = n;
+  return s;
+}
+
+Tensor linear_kernel(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& residual, c10::string_view act)
+{
+  const LinearArgs a = linear_args(x, w, bias, act);
+  const auto out = with_last(a.x, a.n);
+  Tensor r;
+  if (residual.has_value() && residual->defined()) {
+    r = operand(*residual, a.x, a.x.scalar_type(), "residual");
+    check_shape(r, out, "residual");
+  }
+  const c10::cuda::CUDAGuard guard(a.x.device());
+  int64_t bytes = 0;
+  call(rbq_linear_workspace(a.m, a.k, a.n, a.type, a.act, 0, &bytes));
+  Tensor y = at::empty(out, a.x.options()), ws = scratch(a.x, bytes);
+  call(rbq_linear(data(a.x), data(a.w), data(a.bias), data(r), data(y), a.m, a.k, a.n, a.type, a.act, data(ws), bytes,
+                  stream_of(a.x)));
+  return y;
+}
+
+Tensor linear_meta(const Tensor& x, const Tensor& w, const OptTensor&, const OptTensor&, c10::string_view)
+{
+  c10::SymDimVector s(x.sym_sizes().begin(), x.sym_sizes().end());
+  s.back() = w.sym_size(0);
+  return at::empty_symint(s, x.options());
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_backward_kernel(const Tensor& g, const Tensor& x, const Tensor& w,
+                                                          const OptTensor& bias, c10::string_view act, bool need_x,
+                                                          bool need_w, bool need_bias)
+{
+  const LinearArgs a = linear_args(x, w, bias, act);
+  const Tensor gd = operand(g, a.x, a.x.scalar_type(), "g");
+  check_shape(gd, with_last(a.x, a.n), "g");
+  const c10::cuda::CUDAGuard guard(a.x.device());
+  Tensor dx = empty_if(need_x, a.x), dw = empty_if(need_w, a.w), db = at::empty({need_bias ? a.n : 0}, a.x.options());
+  int64_t bytes = 0;
+  call(rbq_linear_workspace(a.m, a.k, a.n, a.type, a.act, 1, &bytes));
+  Tensor ws = scratch(a.x, bytes);
+  call(rbq_linear_backward(data(gd), data(a.x), data(a.w), data(a.bias), need_x ? data(dx) : nullptr,
+                           need_w ? data(dw) : nullptr, need_bias ? data(db) : nullptr, a.m, a.k, a.n, a.type, a.act,
+                           data(ws), bytes, stream_of(a.x)));
+  return {dx, dw, db};
+}
+
+std::tuple<Tensor, Tensor, Tensor> linear_backward_meta(const Tensor&, const Tensor& x, const Tensor& w, const OptTensor&,
+                                                        c10::string_view, bool need_x, bool need_w, bool need_bias)
+{
+  return {empty_if(need_x, x), empty_if(need_w, w),
+          need_bias ? at::empty_symint({w.sym_size(0)}, x.options()) : at::empty({0}, x.options())};
+}
+
+c10::TypedOperatorHandle<decltype(linear_kernel)>& linear_op()
+{
+  static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("rbq::linear", "").typed<decltype(linear_kernel)>();
+  return op;
+}
+
+struct LinearFunction : torch::autograd::Function<LinearFunction> {
+  // Absent optional inputs have no edge: those of bias and residual are numbered without them.
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias,
+                        const OptTensor& residual, const std::string& act)
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({x, w, bias.value_or(Tensor())});
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["residual"] = residual.has_value();
+    return linear_op().call(x, w, bias, residual, act);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads)
+  {
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("rbq::linear_backward", "")
+                         .typed<decltype(linear_backward_kernel)>();
+    const auto saved = ctx->get_saved_variables();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
+    const bool has_bias = saved[2].defined(), nb = has_bias && ctx->needs_input_grad(2);
+    const bool nr = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(has_bias ? 3 : 2);
+    std::array<Tensor, 3> d;
+    if (nx || nw || nb) {
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto [dx, dw, db] = op.call(grads[0], saved[0], saved[1], has_bias ? OptTensor(saved[2]) : OptTensor(),
+                                  ctx->saved_data["act"].toStringRef(), nx, nw, nb);
+      d = {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor()};
+    }
+    d = once(std::move(d), "linear");
+    return {d[0], d[1], d[2], nr ? grads[0] : Tensor(), Tensor()};
+  }
+};
+
+Tensor linear_autograd(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& residual,
+                       c10::string_view act)
+{
+  if (!wants_grad({x, w, bias.value_or(Tensor()), residual.value_or(Tensor())})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return linear_op().call(x, w, bias, residual, act);
+  }
+  return LinearFunction::apply(x, w, bias, residual, std::string(act));
+}
+
+// ---- layer norm --------------------------------------------------------------------------------
+struct NormArgs {
+  Tensor x, w;
+  int64_t rows, d;
+  int type, param_type;
+};
+
+NormArgs norm_args(const Tensor& x, const Tensor& w)
+{
+  NormArgs a;
+  a.x = first(x, true, "x");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "rbq: layer_norm takes x [..., d] with d >= 1, got ", x.sizes());
+  TORCH_CHECK(w.scalar_type() == x.scalar_type() || w.scalar_type() == at::kFloat, "rbq: w must be ",
+              type_name(x.scalar_type()), " or torch.float32, got ", type_name(w.scalar_type()));
+  a.w = operand(w, a.x, w.scalar_type(), "w");
+  a.d = a.x.size(-1);
+  TORCH_CHECK(a.d < (1ll << 31), "rbq: layer norm: bad sizes");
+  check_shape(a.w, {a.d}, "w");
+  a.rows = a.x.numel() / a.d;
+  a.type = type_code(a.x.scalar_type());
+  a.param_type = type_code(a.w.scalar_type());
+  return a;
+}
+
+using Three = std::tuple<Tensor, Tensor, Tensor>;
+
+Three layer_norm_kernel(const Tensor& x, const Tensor& w, const Tensor& b, double eps)
+{
+  const NormArgs a = norm_args(x, w);
+  const Tensor bd = operand(b, a.x, a.w.scalar_type(), "b");
+  check_shape(bd, {a.d}, "b");
+  const c10::cuda::CUDAGuard guard(a.x.device());
+  Tensor y = at::empty_like(a.x);
+  Tensor mean = at::empty(a.x.sizes().slice(0, a.x.dim() - 1), a.x.options().dtype(at::kFloat)), rstd = at::empty_like(mean);
+  call(rbq_layer_norm(data(a.x), data(a.w), data(bd), data(y), (float*)data(mean), (float*)data(rstd), a.rows, a.d, (float)eps,
+                      a.type, a.param_type, stream_of(a.x)));
+  return {y, mean, rstd};
+}
+
+Three layer_norm_meta(const Tensor& x, const Tensor&, const Tensor&, double)
+{
+  c10::SymDimVector s(x.sym_sizes().begin(), x.sym_sizes().end() - 1);
+  Tensor mean = at::empty_symint(s, x.options().dtype(at::kFloat));
+  return {at::empty_like(x), mean, at::empty_like(mean)};
+}
+
+Three layer_norm_backward_kernel(const Tensor& g, const Tensor& x, const Tensor& w, const Tensor& mean, const Tensor& rstd,
+                                 bool need_x, bool need_w, bool need_b)
+{
+  const NormArgs a = norm_args(x, w);
+  const Tensor gd = operand(g, a.x, a.x.scalar_type(), "g");
+  check_shape(gd, a.x.sizes(), "g");
+  const auto rows = a.x.sizes().slice(0, a.x.dim() - 1);
+  const Tensor md = operand(mean, a.x, at::kFloat, "mean"), rd = operand(rstd, a.x, at::kFloat, "rstd");
+  check_shape(md, rows, "mean");
+  check_shape(rd, rows, "rstd");
+  const c10::cuda::CUDAGuard guard(a.x.device());
+  Tensor dx = empty_if(need_x, a.x);
+  Tensor dw = at::empty({need_w ? a.d : 0}, a.w.options()), db = at::empty({need_b ? a.d : 0}, a.w.options());
+  int64_t bytes = 0;
+  if (need_w || need_b) call(rbq_layer_norm_backward_workspace(a.rows, a.d, &bytes));
+  Tensor ws = scratch(a.x, bytes);
+  call(rbq_layer_norm_backward(data(gd), data(a.x), data(a.w), (float*)data(md), (float*)data(rd), need_x ? data(dx) : nullptr,
+                               need_w ? data(dw) : nullptr, need_b ? data(db) : nullptr, a.rows, a.d, a.type, a.param_type,
+                               data(ws), bytes, stream_of(a.x)));
+  return {dx, dw, db};
+}
+
+Three layer_norm_backward_meta(const Tensor&, const Tensor& x, const Tensor& w, const Tensor&, const Tensor&, bool need_x,
+                               bool need_w, bool need_b)
+{
+  return {empty_if(need_x, x), empty_if(need_w, w), empty_if(need_b, w)};
+}
+
+c10::TypedOperatorHandle<decltype(layer_norm_kernel)>& layer_norm_op()
+{
+  static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("rbq::layer_norm", "").typed<decltype(layer_norm_kernel)>();
+  return op;
+}
+
+struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, double eps)
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, mean, rstd] = layer_norm_op().call(x, w, b, eps);
+    ctx->save_for_backward({x, w, mean, rstd});
+    ctx->mark_non_differentiable({mean, rstd});
+    ctx->set_materialize_grads(false);
+    return {y, mean, rstd};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads)
+  {
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("rbq::layer_norm_backward", "")
+                         .typed<decltype(layer_norm_backward_kernel)>();
+    const auto s = ctx->get_saved_variables();
+    const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = ctx->needs_input_grad(2);
+    std::array<Tensor, 3> d;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto [dx, dw, db] = op.call(grads[0], s[0], s[1], s[2], s[3], nx, nw, nb);
+      d = {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor()};
+    }
+    d = once(std::move(d), "layer_norm");
+    return {d[0], d[1], d[2], Tensor()};
+  }
+};
+
+Three layer_norm_autograd(const Tensor& x, const Tensor& w, const Tensor& b, double eps)
+{
+  if (!wants_grad({x, w, b})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return layer_norm_op().call(x, w, b, eps);
+  }
+  auto out = LayerNormFunction::apply(x, w, b, eps);
+  return {out[0], out[1], out[2]};
+}
+
+// ---- softmax loss ------------------------------------------------------------------------------
+struct LossArgs {
+  Tensor q, bank, target;
+  int64_t n, v, d;
+  int type;
+};
+
+LossArgs loss_args(const Tensor& q, const Tensor& bank, const Tensor& target)
+{
+  LossArgs a;
+  a.q = first(q, false, "q");
+  a.bank = operand(bank, a.q, a.q.scalar_type(), "bank");
+  TORCH_CHECK(q.dim() == 2 && bank.dim() == 2 && q.size(1) == bank.size(1) && bank.size(0) >= 1 && q.size(1) >= 1,
+              "rbq: softmax_loss takes q [n, d] and bank [v, d] with v, d >= 1, got ", q.sizes(), " and ", bank.sizes());
+  a.target = operand(target, a.q, at::kLong, "target");
+  a.n = q.size(0);
+  a.v = bank.size(0);
+  a.d = q.size(1);
+  TORCH_CHECK(a.d < (1ll << 31), "rbq: softmax loss: bad sizes");
+  check_shape(a.target, {a.n}, "target");
+  a.type = type_code(a.q.scalar_type());
+  return a;
+}
+
+using Two = std::tuple<Tensor, Tensor>;
+
+Two softmax_loss_kernel(const Tensor& q, const Tensor& bank, const Tensor& target, double scale)
+{
+  const LossArgs a = loss_args(q, bank, target);
+  const c10::cuda::CUDAGuard guard(a.q.device());
+  Tensor loss = at::empty({a.n}, a.q.options().dtype(at::kFloat)), lse = at::empty_like(loss);
+  int64_t bytes = 0;
+  call(rbq_softmax_loss_workspace(a.n, a.v, a.d, a.type, 0, &bytes));
+  Tensor ws = scratch(a.q, bytes);
+  call(rbq_softmax_loss(data(a.q), data(a.bank), (int64_t*)data(a.target), a.n, a.v, a.d, (float)scale, a.type,
+                        (float*)data(loss), (float*)data(lse), data(ws), bytes, stream_of(a.q)));
+  return {loss, lse};
+}
+
+Two softmax_loss_meta(const Tensor& q, const Tensor&, const Tensor&, double)
+{
+  Tensor loss = at::empty_symint({q.sym_size(0)}, q.options().dtype(at::kFloat));
+  return {loss, at::empty_like(loss)};
+}
+
+Two softmax_loss_backward_kernel(const Tensor& g, const Tensor& q, const Tensor& bank, const Tensor& target,
+                                 const Tensor& loss, const Tensor& lse, double scale, bool need_q, bool need_bank)
+{
+  const LossArgs a = loss_args(q, bank, target);
+  const Tensor gd = operand(g, a.q, at::kFloat, "g"), ld = operand(loss, a.q, at::kFloat, "loss"),
+               sd = operand(lse, a.q, at::kFloat, "lse");
+  check_shape(gd, {a.n}, "g");
+  check_shape(ld, {a.n}, "loss");
+  check_shape(sd, {a.n}, "lse");
+  const c10::cuda::CUDAGuard guard(a.q.device());
+  Tensor dq = empty_if(need_q, a.q), dbank = empty_if(need_bank, a.bank);
+  int64_t bytes = 0;
+  call(rbq_softmax_loss_workspace(a.n, a.v, a.d, a.type, 1, &bytes));
+  Tensor ws = scratch(a.q, bytes);
+  call(rbq_softmax_loss_backward((float*)data(gd), data(a.q), data(a.bank), (int64_t*)data(a.target), (float*)data(ld),
+                                 (float*)data(sd), a.n, a.v, a.d, (float)scale, a.type, need_q ? data(dq) : nullptr,
+                                 need_bank ? data(dbank) : nullptr, data(ws), bytes, stream_of(a.q)));
+  return {dq, dbank};
+}
+
+Two softmax_loss_backward_meta(const Tensor&, const Tensor& q, const Tensor& bank, const Tensor&, const Tensor&, const Tensor&,
+                               double, bool need_q, bool need_bank)
+{
+  return {empty_if(need_q, q), empty_if(need_bank, bank)};
+}
+
+c10::TypedOperatorHandle<decltype(softmax_loss_kernel)>& softmax_loss_op()
+{
+  static auto op = c10::Dispatcher::singleton().findSchemaOrThrow("rbq::softmax_loss", "").typed<decltype(softmax_loss_kernel)>();
+  return op;
+}
+
+struct SoftmaxLossFunction : torch::autograd::Function<SoftmaxLossFunction> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& bank, const Tensor& target, double scale)
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [loss, lse] = softmax_loss_op().call(q, bank, target, scale);
+    ctx->save_for_backward({q, bank, target, loss, lse});
+    ctx->saved_data["scale"] = scale;
+    ctx->mark_non_differentiable({lse});
+    ctx->set_materialize_grads(false);
+    return {loss, lse};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads)
+  {
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("rbq::softmax_loss_backward", "")
+                         .typed<decltype(softmax_loss_backward_kernel)>();
+    const auto s = ctx->get_saved_variables();
+    const bool nq = ctx->needs_input_grad(0), nk = ctx->needs_input_grad(1);
+    std::array<Tensor, 2> d;
+    {
+      at::AutoDispatchBelowADInplaceOrView below;
+      auto [dq, dbank] = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(), nq, nk);
+      d = {nq ? dq : Tensor(), nk ? dbank : Tensor()};
+    }
+    d = once(std::move(d), "softmax_loss");
+    return {d[0], d[1], Tensor(), Tensor()};
+  }
+};
+
+Two softmax_loss_autograd(const Tensor& q, const Tensor& bank, const Tensor& target, double scale)
+{
+  if (!wants_grad({q, bank})) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    return softmax_loss_op().call(q, bank, target, scale);
+  }
+  auto out = SoftmaxLossFunction::apply(q, bank, target, scale);
+  return {out[0], out[1]};
+}
+
+TORCH_LIBRARY_FRAGMENT(rbq, m)
+{
+  m.def("linear(Tensor x, Tensor w, Tensor? bias=None, Tensor? residual=None, str act='none') -> Tensor");
+  m.def(
+      "linear_backward(Tensor g, Tensor x, Tensor w, Tensor? bias, str act, bool need_x, bool need_w, bool need_bias) -> "
+      "(Tensor, Tensor, Tensor)");
+  m.def("layer_norm(Tensor x, Tensor w, Tensor b, float eps=1e-5) -> (Tensor, Tensor, Tensor)");
+  m.def(
+      "layer_norm_backward(Tensor g, Tensor x, Tensor w, Tensor mean, Tensor rstd, bool need_x, bool need_w, bool need_b) -> "
+      "(Tensor, Tensor, Tensor)");
+  m.def("softmax_loss(Tensor q, Tensor bank, Tensor target, float scale) -> (Tensor, Tensor)");
+  m.def(
+      "softmax_loss_backward(Tensor g, Tensor q, Tensor bank, Tensor target, Tensor loss, Tensor lse, float scale, "
+      "bool need_q, bool need_bank) -> (Tensor, Tensor)");
+}
+TORCH_LIBRARY_IMPL(rbq, CompositeExplicitAutograd, m)
+{
+  m.impl("linear", linear_kernel);
+  m.impl("linear_backward", linear_backward_kernel);
+  m.impl("layer_norm", layer_norm_kernel);
+  m.impl("layer_norm_backward", layer_norm_backward_kernel);
+  m.impl("softmax_loss", softmax_loss_kernel);
+  m.impl("softmax_loss_backward", softmax_loss_backward_kernel);
+}
+TORCH_LIBRARY_IMPL(rbq, Meta, m)
+{
+  m.impl("linear", linear_meta);
+  m.impl("linear_backward", linear_backward_meta);
+  m.impl("layer_norm", layer_norm_meta);
+  m.impl("layer_norm_backward", layer_norm_backward_meta);
+  m.impl("softmax_loss", softmax_loss_meta);
+  m.impl("softmax_loss_backward", softmax_loss_backward_meta);
+}
+TORCH_LIBRARY_IMPL(rbq, Autograd, m)
+{
+  m.impl("linear", linear_autograd);
+  m.impl("layer_norm", layer_norm_autograd);
+  m.impl("softmax_loss", softmax_loss_autograd);
+}
+
+}  // namespace

@@ -41,6 +41,7 @@ implementation, so output shapes propagate under FakeTensorMode and meta tensors
 from __future__ import annotations
 
 import ctypes
+import os
 from typing import Optional, Tuple
 
 import torch
@@ -238,265 +239,8 @@ def _(dist, ids):
     return dist.new_empty((n, k)), ids.new_empty((n, k))
 
 
-# -- operators of the read encoder ---------------------------------------------------------------
-_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}  # RBQ_F16, RBQ_BF16, RBQ_F32
-_HALVES = (torch.float16, torch.bfloat16)
-
-
-def _operand(t: Tensor, like: Tensor, name: str) -> Tensor:
-    """t, on like's device and of its type, dense and on a 16-byte boundary."""
-    if t.device != like.device or not t.is_cuda:
-        raise RuntimeError(f"rbq: {name} must be a CUDA tensor on {like.device}, got {t.device}")
-    if t.dtype != like.dtype:
-        raise RuntimeError(f"rbq: {name} must be {like.dtype}, got {t.dtype}")
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _first(t: Tensor, types, name: str) -> Tensor:
-    if not t.is_cuda:
-        raise RuntimeError(f"rbq: {name} must be a CUDA tensor")
-    if t.dtype not in types:
-        raise RuntimeError(f"rbq: {name} must be {' or '.join(str(x) for x in types)}, got {t.dtype}")
-    return _operand(t, t, name)
-
-
-def _shape(t: Tensor, want, name: str) -> None:
-    if tuple(t.shape) != tuple(want):
-        raise RuntimeError(f"rbq: {name} must have shape {tuple(want)}, got {tuple(t.shape)}")
-
-
-def _workspace(device: torch.device, query: str, *args) -> Tuple[Optional[Tensor], int]:
-    need = ctypes.c_int64()
-    _lib.call(query, *args, ctypes.byref(need))
-    if need.value == 0:
-        return None, 0
-    return torch.empty(need.value, dtype=torch.uint8, device=device), need.value
-
-
-def _linear_args(x: Tensor, w: Tensor, bias: Optional[Tensor], act: str):
-    x = _first(x, _HALVES, "x")
-    w = _operand(w, x, "w")
-    if x.dim() < 1 or w.dim() != 2 or x.shape[-1] != w.shape[1]:
-        raise RuntimeError(f"rbq: linear takes x [..., k] and w [n, k], got {tuple(x.shape)} and {tuple(w.shape)}")
-    if bias is not None:
-        bias = _operand(bias, x, "bias")
-        _shape(bias, w.shape[:1], "bias")
-    if act not in _lib.ACTIVATIONS:
-        raise RuntimeError(f"rbq: act must be one of {', '.join(_lib.ACTIVATIONS)}, got {act!r}")
-    n, k = w.shape
-    if n < 1 or k < 1:
-        raise RuntimeError("rbq: linear needs k >= 1 and n >= 1")
-    return x, w, bias, x.numel() // k, k, n
-
-
-@custom_op("rbq::linear", mutates_args=())
-def linear(x: Tensor, w: Tensor, bias: Optional[Tensor] = None, residual: Optional[Tensor] = None,
-           act: str = "none") -> Tensor:
-    x, w, bias, m, k, n = _linear_args(x, w, bias, act)
-    out = x.shape[:-1] + (n,)
-    if residual is not None:
-        residual = _operand(residual, x, "residual")
-        _shape(residual, out, "residual")
-    y = torch.empty(out, dtype=x.dtype, device=x.device)
-    with torch.cuda.device(x.device):
-        a = _lib.ACTIVATIONS[act]
-        ws, size = _workspace(x.device, "rbq_linear_workspace", m, k, n, _TYPES[x.dtype], a, 0)
-        _lib.call("rbq_linear", _p(x), _p(w), _p(bias), _p(residual), _p(y), m, k, n, _TYPES[x.dtype], a, _p(ws), size,
-                  _st(x))
-    return y
-
-
-@linear.register_fake
-def _(x, w, bias=None, residual=None, act="none"):
-    return x.new_empty(x.shape[:-1] + (w.shape[0],))
-
-
-@custom_op("rbq::linear_backward", mutates_args=())
-def linear_backward(g: Tensor, x: Tensor, w: Tensor, bias: Optional[Tensor], act: str, need_x: bool, need_w: bool,
-                    need_bias: bool) -> Tuple[Tensor, Tensor, Tensor]:
-    x, w, bias, m, k, n = _linear_args(x, w, bias, act)
-    _shape(g, x.shape[:-1] + (n,), "g")
-    g = _operand(g, x, "g")
-    dx = torch.empty_like(x) if need_x else x.new_empty(0)
-    dw = torch.empty_like(w) if need_w else x.new_empty(0)
-    db = x.new_empty(n if need_bias else 0)
-    with torch.cuda.device(x.device):
-        a = _lib.ACTIVATIONS[act]
-        ws, size = _workspace(x.device, "rbq_linear_workspace", m, k, n, _TYPES[x.dtype], a, 1)
-        _lib.call("rbq_linear_backward", _p(g), _p(x), _p(w), _p(bias), _p(dx if need_x else None),
-                  _p(dw if need_w else None), _p(db if need_bias else None), m, k, n, _TYPES[x.dtype], a, _p(ws), size,
-                  _st(x))
-    return dx, dw, db
-
-
-@linear_backward.register_fake
-def _(g, x, w, bias, act, need_x, need_w, need_bias):
-    return (torch.empty_like(x) if need_x else x.new_empty(0), torch.empty_like(w) if need_w else x.new_empty(0),
-            x.new_empty(w.shape[0] if need_bias else 0))
-
-
-def _linear_context(ctx, inputs, output):
-    x, w, bias, _, ctx.act = inputs
-    ctx.save_for_backward(x, w, bias)
-
-
-def _linear_gradient(ctx, g):
-    x, w, bias = ctx.saved_tensors
-    need = ctx.needs_input_grad + (False,) * 3  # trailing arguments left at their defaults are not listed
-    dx = dw = db = None
-    if need[0] or need[1] or need[2]:
-        dx, dw, db = linear_backward(g, x, w, bias, ctx.act, need[0], need[1], need[2])
-    return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, g if need[3] else None, None)
-
-
-linear.register_autograd(_linear_gradient, setup_context=_linear_context)
-
-
-def _norm_args(x: Tensor, w: Tensor):
-    x = _first(x, tuple(_TYPES), "x")
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise RuntimeError(f"rbq: layer_norm takes x [..., d] with d >= 1, got {tuple(x.shape)}")
-    if w.dtype not in (x.dtype, torch.float32):
-        raise RuntimeError(f"rbq: w must be {x.dtype} or torch.float32, got {w.dtype}")
-    if w.device != x.device:
-        raise RuntimeError(f"rbq: w must be a CUDA tensor on {x.device}, got {w.device}")
-    w = w.contiguous()
-    d = x.shape[-1]
-    _shape(w, (d,), "w")
-    return x, w, x.numel() // d, d
-
-
-@custom_op("rbq::layer_norm", mutates_args=())
-def layer_norm(x: Tensor, w: Tensor, b: Tensor, eps: float = 1e-5) -> Tuple[Tensor, Tensor, Tensor]:
-    x, w, rows, d = _norm_args(x, w)
-    b = _operand(b, w, "b")
-    _shape(b, (d,), "b")
-    y = torch.empty_like(x)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    rstd = torch.empty_like(mean)
-    with torch.cuda.device(x.device):
-        _lib.call("rbq_layer_norm", _p(x), _p(w), _p(b), _p(y), _p(mean), _p(rstd), rows, d, eps, _TYPES[x.dtype],
-                  _TYPES[w.dtype], _st(x))
-    return y, mean, rstd
-
-
-@layer_norm.register_fake
-def _(x, w, b, eps=1e-5):
-    mean = x.new_empty(x.shape[:-1], dtype=torch.float32)
-    return torch.empty_like(x), mean, torch.empty_like(mean)
-
-
-@custom_op("rbq::layer_norm_backward", mutates_args=())
-def layer_norm_backward(g: Tensor, x: Tensor, w: Tensor, mean: Tensor, rstd: Tensor, need_x: bool, need_w: bool,
-                        need_b: bool) -> Tuple[Tensor, Tensor, Tensor]:
-    x, w, rows, d = _norm_args(x, w)
-    _shape(g, x.shape, "g")
-    g = _operand(g, x, "g")
-    for t, name in ((mean, "mean"), (rstd, "rstd")):
-        _shape(t, x.shape[:-1], name)
-    mean, rstd = _cuda(mean, torch.float32, "mean"), _cuda(rstd, torch.float32, "rstd")
-    dx = torch.empty_like(x) if need_x else x.new_empty(0)
-    dw, db = w.new_empty(d if need_w else 0), w.new_empty(d if need_b else 0)
-    with torch.cuda.device(x.device):
-        ws, size = (_workspace(x.device, "rbq_layer_norm_backward_workspace", rows, d) if need_w or need_b
-                    else (None, 0))
-        _lib.call("rbq_layer_norm_backward", _p(g), _p(x), _p(w), _p(mean), _p(rstd), _p(dx if need_x else None),
-                  _p(dw if need_w else None), _p(db if need_b else None), rows, d, _TYPES[x.dtype], _TYPES[w.dtype],
-                  _p(ws), size, _st(x))
-    return dx, dw, db
-
-
-@layer_norm_backward.register_fake
-def _(g, x, w, mean, rstd, need_x, need_w, need_b):
-    d = x.shape[-1]
-    return (torch.empty_like(x) if need_x else x.new_empty(0), w.new_empty(d if need_w else 0),
-            w.new_empty(d if need_b else 0))
-
-
-def _norm_context(ctx, inputs, output):
-    x, w, _, _ = inputs
-    _, mean, rstd = output
-    ctx.mark_non_differentiable(mean, rstd)
-    ctx.save_for_backward(x, w, mean, rstd)
-
-
-def _norm_gradient(ctx, g, _mean, _rstd):
-    x, w, mean, rstd = ctx.saved_tensors
-    need = ctx.needs_input_grad
-    dx, dw, db = layer_norm_backward(g, x, w, mean, rstd, need[0], need[1], need[2])
-    return dx if need[0] else None, dw if need[1] else None, db if need[2] else None, None
-
-
-layer_norm.register_autograd(_norm_gradient, setup_context=_norm_context)
-
-
-def _loss_args(q: Tensor, bank: Tensor, target: Tensor):
-    q = _first(q, _HALVES, "q")
-    bank = _operand(bank, q, "bank")
-    if q.dim() != 2 or bank.dim() != 2 or q.shape[1] != bank.shape[1] or bank.shape[0] < 1 or q.shape[1] < 1:
-        raise RuntimeError(f"rbq: softmax_loss takes q [n, d] and bank [v, d] with v, d >= 1, got {tuple(q.shape)} and "
-                           f"{tuple(bank.shape)}")
-    target = _cuda(target, torch.int64, "target")
-    if target.device != q.device:
-        raise RuntimeError(f"rbq: target must be a CUDA tensor on {q.device}, got {target.device}")
-    _shape(target, q.shape[:1], "target")
-    return q, bank, target
-
-
-@custom_op("rbq::softmax_loss", mutates_args=())
-def softmax_loss(q: Tensor, bank: Tensor, target: Tensor, scale: float) -> Pair:
-    q, bank, target = _loss_args(q, bank, target)
-    (n, d), v = q.shape, bank.shape[0]
-    loss = torch.empty(n, dtype=torch.float32, device=q.device)
-    lse = torch.empty_like(loss)
-    with torch.cuda.device(q.device):
-        ws, size = _workspace(q.device, "rbq_softmax_loss_workspace", n, v, d, _TYPES[q.dtype], 0)
-        _lib.call("rbq_softmax_loss", _p(q), _p(bank), _p(target), n, v, d, scale, _TYPES[q.dtype], _p(loss), _p(lse),
-                  _p(ws), size, _st(q))
-    return loss, lse
-
-
-@softmax_loss.register_fake
-def _(q, bank, target, scale):
-    loss = q.new_empty(q.shape[0], dtype=torch.float32)
-    return loss, torch.empty_like(loss)
-
-
-@custom_op("rbq::softmax_loss_backward", mutates_args=())
-def softmax_loss_backward(g: Tensor, q: Tensor, bank: Tensor, target: Tensor, loss: Tensor, lse: Tensor, scale: float,
-                          need_q: bool, need_bank: bool) -> Pair:
-    q, bank, target = _loss_args(q, bank, target)
-    (n, d), v = q.shape, bank.shape[0]
-    for t, name in ((g, "g"), (loss, "loss"), (lse, "lse")):
-        _shape(t, (n,), name)
-    g, loss, lse = (_cuda(t, torch.float32, name) for t, name in ((g, "g"), (loss, "loss"), (lse, "lse")))
-    dq = torch.empty_like(q) if need_q else q.new_empty(0)
-    dbank = torch.empty_like(bank) if need_bank else q.new_empty(0)
-    with torch.cuda.device(q.device):
-        ws, size = _workspace(q.device, "rbq_softmax_loss_workspace", n, v, d, _TYPES[q.dtype], 1)
-        _lib.call("rbq_softmax_loss_backward", _p(g), _p(q), _p(bank), _p(target), _p(loss), _p(lse), n, v, d, scale,
-                  _TYPES[q.dtype], _p(dq if need_q else None), _p(dbank if need_bank else None), _p(ws), size, _st(q))
-    return dq, dbank
-
-
-@softmax_loss_backward.register_fake
-def _(g, q, bank, target, loss, lse, scale, need_q, need_bank):
-    return (torch.empty_like(q) if need_q else q.new_empty(0), torch.empty_like(bank) if need_bank else q.new_empty(0))
-
-
-def _loss_context(ctx, inputs, output):
-    q, bank, target, ctx.scale = inputs
-    loss, lse = output
-    ctx.mark_non_differentiable(lse)
-    ctx.save_for_backward(q, bank, target, loss, lse)
-
-
-def _loss_gradient(ctx, g, _lse):
-    q, bank, target, loss, lse = ctx.saved_tensors
-    need = ctx.needs_input_grad
-    dq, dbank = softmax_loss_backward(g, q, bank, target, loss, lse, ctx.scale, need[0], need[1])
-    return dq if need[0] else None, dbank if need[1] else None, None, None
-
-
-softmax_loss.register_autograd(_loss_gradient, setup_context=_loss_context)
+# linear, layer_norm, softmax_loss and their backward passes are registered by librbq_torch.so
+# (csrc/rbq_torch.cpp).  Before the libraries are built there is nothing to load: `_lib.lib()` says so
+# at the first call of any other entry point.
+if os.path.exists(_lib.TORCH_LIB_PATH):
+    torch.ops.load_library(_lib.TORCH_LIB_PATH)

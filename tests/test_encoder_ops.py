@@ -72,6 +72,27 @@ def test_host_tensors_are_refused():
         o.layer_norm(x, x[0], x[0])
     with pytest.raises(RuntimeError, match="CUDA tensor"):
         o.softmax_loss(x, x, torch.zeros(3, dtype=torch.int64), 1.0)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        o.linear(x.requires_grad_(), x.detach())
+
+
+@pytest.mark.gpu  # autograd's engine wants the device that the fake tensors name
+def test_fake_tensors_keep_their_shapes_through_a_backward_pass():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    o = ops()
+    with FakeTensorMode():
+        x = torch.empty(6, 16, dtype=F16, device="cuda", requires_grad=True)
+        w = torch.empty(24, 16, dtype=F16, device="cuda", requires_grad=True)
+        y = o.linear(x, w, None, None, "relu")
+        dx, dw = torch.autograd.grad(y, (x, w), torch.empty_like(y))
+        assert y.shape == (6, 24) and dx.shape == (6, 16) and dw.shape == (24, 16) and dw.device.type == "cuda"
+        n = torch.empty(16, device="cuda", requires_grad=True)
+        dx, dn = torch.autograd.grad(o.layer_norm(x, n, n)[0], (x, n), torch.empty_like(x))
+        assert dx.dtype == F16 and dn.dtype == F32 and dn.shape == (16,)
+        t = torch.empty(6, dtype=torch.int64, device="cuda")
+        loss = o.softmax_loss(x, w, t, 2.0)[0]
+        dq, dk = torch.autograd.grad(loss, (x, w), torch.empty_like(loss))
+        assert dq.shape == (6, 16) and dk.shape == (24, 16)
 
 
 P1 = ctypes.c_void_p(16)  # never dereferenced: the checks come first
@@ -146,6 +167,8 @@ def test_wrapper_refusals():
         (lambda: o.layer_norm(x, w[0, :8], w[0, :8]), "w must have shape"),
         (lambda: o.layer_norm(x, w[0].bfloat16(), w[0].bfloat16()), "w must be torch.float16 or torch.float32"),
         (lambda: o.layer_norm(x, w[0], w[0].float()), "b must be torch.float16"),
+        (lambda: o.layer_norm(x, w[0].cpu(), w[0]), "w must be a CUDA tensor"),
+        (lambda: o.softmax_loss(x, w.cpu(), t, 1.0), "bank must be a CUDA tensor"),
         (lambda: o.layer_norm(x, w[0], w[0], -1.0), "eps"),
         (lambda: o.softmax_loss(x, w, t.int(), 1.0), "target must be torch.int64"),
         (lambda: o.softmax_loss(x, w, t[:2], 1.0), "target must have shape"),
@@ -167,6 +190,17 @@ def test_short_workspace_is_refused():
     p = lambda v: ctypes.c_void_p(v.data_ptr())  # noqa: E731
     st = _lib.lib().rbq_softmax_loss(p(x), p(x), p(t), 64, 64, 8, 1.0, 0, p(f), p(f), p(x), 16, None)
     assert st == 1 and "bytes" in _lib.lib().rbq_last_error().decode()
+
+
+@pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    o = ops()
+    x = torch.randn(4, 16, device="cuda").to(F16).requires_grad_()
+    w = torch.randn(8, 16, device="cuda").to(F16).requires_grad_()
+    y = o.linear(x, w, None, None, "gelu")
+    dx, = torch.autograd.grad(y, x, torch.ones_like(y).requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError):
+        dx.float().sum().backward()
 
 
 # -- linear ----------------------------------------------------------------------------------------
