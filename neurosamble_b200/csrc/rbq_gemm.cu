@@ -8,11 +8,17 @@
 // rows contiguous ("MN-major": the same matrices inside a gradient, where the sum runs over the
 // stored rows); the tensor cores read both, so no operand is ever transposed in memory.
 //
-// CTA (320 threads, persistent over output tiles of 128 x BN): warp 8 streams 64-wide k-blocks of A
-// and B by TMA into a ring of shared-memory stages (128-byte swizzle, zero fill past the edges), warp 9
-// issues the MMAs into one of two accumulators (2 x BN of the 512 TMEM columns), and two warpgroups
-// take the finished accumulators in turn, so that the epilogue of one tile runs beside the MMAs of
-// the next.  In an epilogue thread r owns output row r (TMEM lane r).  Output and input tiles of the
+// CTA (320 threads, persistent over output tiles): warp 8 streams 64-wide k-blocks of A and B by TMA into
+// a ring of shared-memory stages (128-byte swizzle, zero fill past the edges), warp 9 issues the MMAs
+// into one of two accumulators (2 x BN of the 512 TMEM columns), and two warpgroups take the
+// finished accumulators in turn, so that the epilogue of one tile runs beside the MMAs of the next.
+// In an epilogue thread r owns output row r (TMEM lane r).
+//
+// Two shapes.  CG = 2, products with enough tiles for every SM pair: two CTAs of a cluster share a
+// 256 x 256 tile (cta_group::2), each holding 128 rows of A and 128 of B per stage, so that a CTA
+// takes 64 operand bytes per MMA clock out of L2; one CTA with a 128 x 256 tile of its own would take
+// 96, and was bound by that.  The leader CTA issues the MMAs for both.  CG = 1, the smaller ones: a CTA
+// takes a 128 x 128 tile.  Output and input tiles of the
 // epilogue pass through 128-byte swizzled staging rows: by TMA where the matrix allows it (rows a
 // multiple of 16 bytes apart), else by coalesced loads and stores of the warp that owns the rows.
 //
@@ -108,12 +114,68 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t saddr, int mn)
          (uint64_t)1 << 46 | (uint64_t)2 << 61;
 }
 
+template <int CG>
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
 {
-  asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(acc));
+  if (CG == 1)
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+  else
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+}
+
+// Arrives on `bar` of this CTA, or of both CTAs of the pair, once the MMAs issued so far are done.
+template <int CG>
+__device__ __forceinline__ void commit(uint32_t bar)
+{
+  if (CG == 1)
+    tc_commit(bar);
+  else
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+// Tile load whose bytes are counted on `bar`, a barrier of the pair's leader.
+template <int CG>
+__device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar)
+{
+  if (CG == 1)
+    tma_load_2d(dst, map, x, y, bar);
+  else
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+// The leader's copy of a shared-memory address, in the cluster's window.
+__device__ __forceinline__ uint32_t leader_addr(uint32_t addr)
+{
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(addr));
+  return r;
+}
+
+template <int CG>
+__device__ __forceinline__ void arrive_leader(uint32_t bar)
+{
+  if (CG == 1)
+    mbar_arrive(bar);
+  else
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+}
+
+__device__ __forceinline__ void cluster_sync()
+{
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
 // Bounded wait that gives up once any role has failed.
@@ -122,7 +184,8 @@ __device__ __forceinline__ bool op_wait(uint32_t bar, uint32_t parity, volatile 
   for (uint32_t it = 0; it < kOpWaitLimit; ++it) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, "
+        "p;\n}"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
         : "memory");
@@ -188,21 +251,110 @@ struct Pack<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 from(float f) { return __float2bfloat16_rn(f); }
 };
 
-// act(z) and act'(z); GELU is z * Phi(z), its slope Phi(z) + z * phi(z).
-template <int ACT>
-__device__ __forceinline__ float act_of(float z)
+// Two fp32 values in a register pair: one instruction for both.
+__device__ __forceinline__ uint64_t pair(float a, float b)
 {
-  if (ACT == RBQ_ACT_RELU) return z > 0.0f ? z : (z != z ? z : 0.0f);
-  if (ACT == RBQ_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678f));
-  return z;
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split(uint64_t v)
+{
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b)
+{
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// GELU z Phi(z) = max(z, 0) - w Phi(-w) and its slope Phi(z) + z phi(z) = [z > 0] - sign(z) (Phi(-w) -
+// w phi(w)), w = |z|.  Both tails are e^{-w^2 / 2} times a smooth function of w, and that is a
+// polynomial here: minimax fits on [0, 6] of the products' absolute error (own fits, weighted by the
+// exponential), good to 8e-7 for the value and 4e-6 for the slope, which is rounded to 16 bits
+// at once.  Past w = 8 the exponential is below 2^-46.  erff and expf in their place made the
+// epilogue five times as long as its tile's memory traffic.
+__device__ __forceinline__ uint64_t gauss2(uint64_t z)  // e^{-z^2 / 2}
+{
+  const float c = -0.72134752f;  // -log2(e) / 2
+  const float2 t = split(mul2(mul2(z, z), pair(c, c)));
+  return pair(ex2(t.x), ex2(t.y));
+}
+template <int N>
+__device__ __forceinline__ uint64_t horner2(const float (&c)[N], uint64_t x)
+{
+  uint64_t r = pair(c[N - 1], c[N - 1]);
+#pragma unroll
+  for (int i = N - 2; i >= 0; --i) r = fma2(r, x, pair(c[i], c[i]));
+  return r;
 }
 template <int ACT>
-__device__ __forceinline__ float act_slope(float z)
+__device__ __forceinline__ float2 act_of(uint64_t z)
 {
-  if (ACT == RBQ_ACT_RELU) return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-  if (ACT == RBQ_ACT_GELU)
-    return fmaf(z * 0.39894228f, __expf(-0.5f * z * z), 0.5f * (1.0f + erff(z * 0.70710678f)));
-  return 1.0f;
+  const float2 v = split(z);
+  if (ACT == RBQ_ACT_RELU) return make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
+  if (ACT == RBQ_ACT_GELU) {
+    // in -w, so that every coefficient is positive
+    const float c[9] = {0.499963641f,  0.398381382f,   0.247026116f,   0.125212014f,  0.050794214f,
+                        0.0154364463f, 0.00319635496f, 0.000392604211f, 2.12489049e-05f};
+    const uint64_t nw = pair(fmaxf(-fabsf(v.x), -8.0f), fmaxf(-fabsf(v.y), -8.0f));
+    return split(fma2(mul2(gauss2(z), nw), horner2(c, nw), pair(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f))));
+  }
+  return v;
+}
+template <int ACT>
+__device__ __forceinline__ float2 act_slope(uint64_t z)
+{
+  const float2 v = split(z);
+  if (ACT == RBQ_ACT_RELU)
+    return make_float2(v.x > 0.0f ? 1.0f : (v.x != v.x ? v.x : 0.0f), v.y > 0.0f ? 1.0f : (v.y != v.y ? v.y : 0.0f));
+  if (ACT == RBQ_ACT_GELU) {
+    const float c[8] = {0.499996036f,  0.797662377f,  0.247959644f,   0.125826955f,
+                        0.0499400385f, 0.013923605f, 0.00231907005f, 0.000168557366f};
+    const uint64_t nw = pair(fmaxf(-fabsf(v.x), -8.0f), fmaxf(-fabsf(v.y), -8.0f));
+    const float2 t = split(mul2(gauss2(z), horner2(c, nw)));
+    return make_float2(v.x > 0.0f ? 1.0f - t.x : t.x, v.y > 0.0f ? 1.0f - t.y : t.y);
+  }
+  return make_float2(1.0f, 1.0f);
+}
+
+// 64 consecutive fp32 accumulator columns of the warp's 32 TMEM lanes.
+__device__ __forceinline__ void tc_ld64(uint32_t taddr, float (&v)[64])
+{
+  uint32_t r[64];
+#define RBQ_R8(i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, "
+      "%39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, "
+      "%62, %63}, [%64];"
+      : RBQ_R8(0), RBQ_R8(8), RBQ_R8(16), RBQ_R8(24), RBQ_R8(32), RBQ_R8(40), RBQ_R8(48), RBQ_R8(56)
+      : "r"(taddr));
+#undef RBQ_R8
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 struct Tile {
@@ -228,13 +380,14 @@ __device__ __forceinline__ int k_begin(const GemmArgs& a, int split)
   return (int)((int64_t)a.kblocks * split / a.splits);
 }
 
-template <int EPI, int BN>
+template <int EPI, int CG>
 struct Shape {
-  static constexpr int kOperands = kBM * 128 + BN * 128;
-  static constexpr bool kStaged = EPI != kEpiLse;  // the loss's forward pass writes no tile
-  static constexpr int kStages = kStaged ? (BN == 256 ? 3 : 5) : (BN == 256 ? 4 : 6);
+  static constexpr int kBN = 128 * CG;                // columns of a tile and of its accumulator
+  static constexpr int kOperands = 2 * kBM * 128;     // a CTA's share of a stage: 128 rows of A, 128 of B
+  static constexpr bool kStaged = EPI != kEpiLse;     // the loss's forward pass writes no tile
+  static constexpr int kStages = !kStaged ? 6 : CG == 2 ? 4 : 5;
   static constexpr int kOutBytes = kStaged ? 4 * kStageOut : 0;  // two buffers per warpgroup
-  static constexpr int kBytes = kStages * kOperands + kOutBytes + 2 * BN * 4 + 1024;
+  static constexpr int kBytes = kStages * kOperands + kOutBytes + 2 * kBN * 4 + 1024;
 };
 
 // The warp's 32 staging rows <-> a matrix whose rows no TMA can address, 64 columns from `col`.
@@ -259,13 +412,14 @@ __device__ __forceinline__ void move_rows(unsigned char* buf, T* mat, int64_t ro
   }
 }
 
-template <int EPI, typename T, int BN, int ACT>
+template <int EPI, typename T, int CG, int ACT>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmO,
                 const __grid_constant__ GemmArgs a)
 {
-  using S = Shape<EPI, BN>;
+  using S = Shape<EPI, CG>;
+  constexpr int BN = S::kBN;
   extern __shared__ unsigned char gemm_smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -276,10 +430,18 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int s_fail;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0;  // in the pair; 0 leads
+  const int first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
   if (warp == kMmaWarp) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
-                 "r"((uint32_t)(2 * BN)));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if (CG == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                   "r"((uint32_t)(2 * BN)));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+                   "r"((uint32_t)(2 * BN)));
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
   }
   if (tid == 0) {
     for (int i = 0; i < S::kStages; ++i) {
@@ -288,7 +450,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&s_done[i]), 1);
-      mbar_init(smem_u32(&s_free[i]), 4);  // one arrival per epilogue warp
+      mbar_init(smem_u32(&s_free[i]), 4 * CG);  // one arrival per epilogue warp of the pair
     }
     for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&s_x[i]), 1);
     s_fail = 0;
@@ -296,6 +458,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (CG == 2) cluster_sync();  // the pair's barriers exist
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s_tmem;
   volatile int* fail = &s_fail;
@@ -307,9 +470,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmB)) : "memory");
       int c = 0;  // k-block, counted over the CTA's whole run: stage c % kStages
       bool ok = true;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x) {
+      for (int t = first_tile; t < total && ok; t += tile_step) {
         const Tile tl = tile_at(a, t);
-        const int m0 = tl.m * kBM, n0 = tl.n * BN;
+        const int m0 = (tl.m * CG + rank) * kBM, n0 = tl.n * BN + rank * 128;  // this CTA's rows of A and of B
         for (int kb = k_begin(a, tl.split), ke = k_begin(a, tl.split + 1); kb < ke; ++kb, ++c) {
           const int st = c % S::kStages;
           if (c >= S::kStages && !op_wait(smem_u32(&s_empty[st]), (uint32_t)((c / S::kStages - 1) & 1), fail)) {
@@ -317,36 +480,44 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = false;
             break;
           }
-          const uint32_t full = smem_u32(&s_full[st]);
+          const uint32_t full = CG == 2 ? leader_addr(smem_u32(&s_full[st])) : smem_u32(&s_full[st]);
           const uint32_t sa = smem_u32(base + st * S::kOperands), sb = sa + kBM * 128;
-          mbar_expect_tx(full, (uint32_t)S::kOperands);
+          if (rank == 0) mbar_expect_tx(smem_u32(&s_full[st]), (uint32_t)(CG * S::kOperands));
           const int k0 = kb * kBK;
           if (a.a_mn) {
 #pragma unroll
-            for (int j = 0; j < kBM / 64; ++j) tma_load_2d(sa + j * kBK * 128, &tmA, m0 + j * 64, k0, full);
+            for (int j = 0; j < 2; ++j) load_tile<CG>(sa + j * kBK * 128, &tmA, m0 + j * 64, k0, full);
           } else {
-            tma_load_2d(sa, &tmA, k0, m0, full);
+            load_tile<CG>(sa, &tmA, k0, m0, full);
           }
           if (a.b_mn) {
 #pragma unroll
-            for (int j = 0; j < BN / 64; ++j) tma_load_2d(sb + j * kBK * 128, &tmB, n0 + j * 64, k0, full);
+            for (int j = 0; j < 2; ++j) load_tile<CG>(sb + j * kBK * 128, &tmB, n0 + j * 64, k0, full);
           } else {
-            tma_load_2d(sb, &tmB, k0, n0, full);
+            load_tile<CG>(sb, &tmB, k0, n0, full);
           }
         }
       }
-      // Copies in flight after a failure land before the CTA's shared memory goes away.
-      if (*fail)
+      // The pair's MMAs arrive on both CTAs' barriers: all have before this one's shared memory goes away.
+      if (ok)
+        for (int i = (c > S::kStages ? c - S::kStages : 0); i < c; ++i)
+          if (!op_wait(smem_u32(&s_empty[i % S::kStages]), (uint32_t)((i / S::kStages) & 1), fail)) {
+            fail_with(fail, 6);
+            break;
+          }
+      // Copies in flight after a failure land before the shared memory goes away (the leader's barriers
+      // count those of both CTAs).
+      if (*fail && rank == 0)
         for (int i = (c > S::kStages ? c - S::kStages : 0); i < c; ++i)
           mbar_wait(smem_u32(&s_full[i % S::kStages]), (uint32_t)((i / S::kStages) & 1));
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       const uint32_t a_step = a.a_mn ? 16 * 128 : 32, b_step = a.b_mn ? 16 * 128 : 32;  // 16 values of k
       int c = 0, i = 0;
       bool ok = true;
-      for (int t = blockIdx.x; t < total && ok; t += gridDim.x, ++i) {
+      for (int t = first_tile; t < total && ok; t += tile_step, ++i) {
         const int acc = i & 1;
         if (i >= 2 && !op_wait(smem_u32(&s_free[acc]), (uint32_t)(((i >> 1) - 1) & 1), fail)) {
           fail_with(fail, 2);
@@ -366,11 +537,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t sa = smem_u32(base + st * S::kOperands), sb = sa + kBM * 128;
 #pragma unroll
           for (int ks = 0; ks < kBK / 16; ++ks)
-            mma_f16(tmem + acc * BN, operand_desc(sa + ks * a_step, a.a_mn), operand_desc(sb + ks * b_step, a.b_mn),
+            mma_f16<CG>(tmem + acc * BN, operand_desc(sa + ks * a_step, a.a_mn), operand_desc(sb + ks * b_step, a.b_mn),
                     a.idesc, (kb > kb0 || ks > 0) ? 1u : 0u);
-          tc_commit(smem_u32(&s_empty[st]));
+          commit<CG>(smem_u32(&s_empty[st]));
         }
-        if (ok) tc_commit(smem_u32(&s_done[acc]));
+        if (ok) commit<CG>(smem_u32(&s_done[acc]));
       }
       // MMAs still running after a failure end before TMEM is freed: the last commit follows them.
       if (*fail && c > 0)
@@ -393,27 +564,27 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Tile tl = tile_at(a, t);
       const uint32_t bar = smem_u32(&s_x[wg * 2 + (cc & 1)]);
       mbar_expect_tx(bar, (uint32_t)kStageOut);
-      tma_load_2d(smem_u32(bufs + (cc & 1) * kStageOut), &tmX, tl.n * BN + s * 64, tl.m * kBM, bar);
+      tma_load_2d(smem_u32(bufs + (cc & 1) * kStageOut), &tmX, tl.n * BN + s * 64, (tl.m * CG + rank) * kBM, bar);
     };
     const bool extra_tma = (EPI == kEpiLinear || EPI == kEpiActGrad) && a.has_extra && a.io_tma;
     int loaded = 0;  // extra tiles asked for (leader)
     if (extra_tma && leader) {
-      const int t = blockIdx.x + wg * gridDim.x;
+      const int t = first_tile + wg * tile_step;
       if (t < total) {
         load_extra(0, t, 0);
         loaded = 1;
       }
     }
 
-    for (int i = wg, t = blockIdx.x + wg * gridDim.x; t < total; i += 2, t += 2 * gridDim.x) {
+    for (int i = wg, t = first_tile + wg * tile_step; t < total; i += 2, t += 2 * tile_step) {
       const Tile tl = tile_at(a, t);
-      const int64_t m0 = (int64_t)tl.m * kBM;
+      const int64_t m0 = (int64_t)(tl.m * CG + rank) * kBM;
       const int n0 = tl.n * BN;
       const int64_t row = m0 + gt;
-      if ((EPI == kEpiLinear || EPI == kEpiActGrad) && a.bias != nullptr) {
+      if (EPI == kEpiLinear || EPI == kEpiActGrad) {
         group_sync(wg);  // the last tile's values have been used
         for (int j = gt; j < BN; j += 128)
-          bias[j] = n0 + j < a.N ? Pack<T>::one(reinterpret_cast<const T*>(a.bias)[n0 + j]) : 0.0f;
+          bias[j] = a.bias != nullptr && n0 + j < a.N ? Pack<T>::one(reinterpret_cast<const T*>(a.bias)[n0 + j]) : 0.0f;
         group_sync(wg);
       }
       if (!dead) {
@@ -430,33 +601,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         float m = -INFINITY, l = 0.0f;
         if (!dead) {
 #pragma unroll 1
-          for (int j = 0; j < BN / 32; ++j) {
-            float v[32];
-            tc_ld32(acc_addr + j * 32, v);
-            const int64_t tj = trow - j * 32;
-            if (__any_sync(0xffffffffu, (uint64_t)tj < 32u)) {
+          for (int j = 0; j < BN / 64; ++j) {
+            float v[64];
+            tc_ld64(acc_addr + j * 64, v);
+            const int64_t tj = trow - j * 64;
+            if (__any_sync(0xffffffffu, (uint64_t)tj < 64u)) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = e == tj ? -INFINITY : v[e];
+              for (int e = 0; e < 64; ++e) v[e] = e == tj ? -INFINITY : v[e];
             }
-            if (n0 + j * 32 + 32 > a.N) {
+            if (n0 + j * 64 + 64 > a.N) {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = n0 + j * 32 + e < a.N ? v[e] : -INFINITY;
+              for (int e = 0; e < 64; ++e) v[e] = n0 + j * 64 + e < a.N ? v[e] : -INFINITY;
             }
-            float top = v[0];
+            float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-            for (int e = 1; e < 32; ++e) top = fmaxf(top, v[e]);
-            const float mn = fmaxf(m, top * a.c2);
+            for (int e = 4; e < 64; ++e) top[e & 3] = fmaxf(top[e & 3], v[e]);
+            const float mn = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.c2);
             const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing but masked logits so far
-            float sum = 0.0f;
+            const uint64_t c2 = pair(a.c2, a.c2), nref = pair(-ref, -ref);
+            uint64_t sum[2] = {0, 0};
 #pragma unroll
-            for (int e = 0; e < 32; ++e) sum += ex2(fmaf(v[e], a.c2, -ref));
-            l = fmaf(l, ex2(m - ref), sum);
+            for (int e = 0; e < 64; e += 2) {
+              const float2 x = split(fma2(pair(v[e], v[e + 1]), c2, nref));
+              sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(ex2(x.x), ex2(x.y)));
+            }
+            const float2 t = split(add2(sum[0], sum[1]));
+            l = fmaf(l, ex2(m - ref), t.x + t.y);
             m = mn;
           }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&s_free[wg]));
+        if (lane == 0) arrive_leader<CG>(smem_u32(&s_free[wg]));
         if (!dead && row < a.M) a.partial[(int64_t)tl.n * a.M + row] = make_float2(m, l);
         continue;
       }
@@ -479,7 +655,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           // ask for the next tile's extra input: its buffer's last store has been read
           if (leader && !dead) {
             int nt = t, ns = s + 1;
-            if (ns == subs) nt = t + 2 * gridDim.x, ns = 0;
+            if (ns == subs) nt = t + 2 * tile_step, ns = 0;
             if (nt < total) {
               asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
               load_extra(c + 1, nt, ns);
@@ -503,73 +679,78 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
         }
         if (!dead) {
-#pragma unroll
-          for (int h = 0; h < kSub / 32; ++h) {
+          if (EPI == kEpiSlab) {
             float v[32];
-            tc_ld32(acc_addr + s * kSub + h * 32, v);
-            if (EPI == kEpiSlab) {
-              float4* at = reinterpret_cast<float4*>(buf + gt * 128);
+            tc_ld32(acc_addr + s * 32, v);
+            float4* at = reinterpret_cast<float4*>(buf + gt * 128);
 #pragma unroll
-              for (int u = 0; u < 8; ++u)
-                at[u ^ (gt & 7)] = make_float4(v[4 * u], v[4 * u + 1], v[4 * u + 2], v[4 * u + 3]);
-              continue;
-            }
+            for (int w = 0; w < 8; ++w)
+              at[w ^ (gt & 7)] = make_float4(v[4 * w], v[4 * w + 1], v[4 * w + 2], v[4 * w + 3]);
+          } else {
+            float v[64];
+            tc_ld64(acc_addr + s * 64, v);
             uint4* at = reinterpret_cast<uint4*>(buf + gt * 128);
             if (EPI == kEpiProb) {
-              const int64_t tj = trow - s * 64 - h * 32;
+              const uint64_t c2 = pair(a.c2, a.c2), nlse = pair(-gr.lse2, -gr.lse2), w = pair(gr.w, gr.w);
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = ex2(fmaf(v[e], a.c2, -gr.lse2)) * gr.w;
-              if (gr.w == 0.0f) {  // a row that takes no part, whatever its logits
-#pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+              for (int e = 0; e < 64; e += 2) {
+                const float2 x = split(fma2(pair(v[e], v[e + 1]), c2, nlse));
+                const float2 y = split(mul2(pair(ex2(x.x), ex2(x.y)), w));
+                v[e] = y.x;
+                v[e + 1] = y.y;
               }
-              if ((uint64_t)tj < 32u) {
+              const int64_t tj = trow - s * 64;
+              if (__any_sync(0xffffffffu, gr.w == 0.0f || (uint64_t)tj < 64u)) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) v[e] = e == tj ? gr.at_target : v[e];
+                for (int e = 0; e < 64; ++e)  // a row that takes no part gives zeros, whatever its logits
+                  v[e] = gr.w == 0.0f ? 0.0f : e == tj ? gr.at_target : v[e];
               }
             }
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const int slot = (h * 4 + u) ^ (gt & 7);
+            for (int w = 0; w < 8; ++w) {
+              const int slot = w ^ (gt & 7);
+              float* o = v + w * 8;
               if (EPI == kEpiLinear || EPI == kEpiActGrad) {
                 uint4 x = make_uint4(0, 0, 0, 0);
                 if (EPI == kEpiActGrad || a.has_extra) x = at[slot];
                 const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+                const uint64_t al = pair(alpha, alpha);
+                const ulonglong2* bp = reinterpret_cast<const ulonglong2*>(bias + s * 64 + w * 8);
+                const ulonglong2 b01 = bp[0], b23 = bp[1];
+                const uint64_t b[4] = {b01.x, b01.y, b23.x, b23.y};
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                  const float2 xe = Pack<T>::get(xs[e]);
-                  float& v0 = v[u * 8 + e * 2];
-                  float& v1 = v[u * 8 + e * 2 + 1];
-                  float b0 = 0.0f, b1 = 0.0f;
-                  if (a.bias != nullptr) {
-                    const float2 b = *reinterpret_cast<const float2*>(bias + s * 64 + h * 32 + u * 8 + e * 2);
-                    b0 = b.x, b1 = b.y;
-                  }
-                  const float z0 = fmaf(v0, alpha, b0), z1 = fmaf(v1, alpha, b1);
+                  const uint64_t z = fma2(pair(o[2 * e], o[2 * e + 1]), al, b[e]);
                   if (EPI == kEpiActGrad) {
-                    v0 = xe.x * act_slope<ACT>(z0);
-                    v1 = xe.y * act_slope<ACT>(z1);
+                    const float2 f = act_slope<ACT>(z), g = Pack<T>::get(xs[e]);
+                    o[2 * e] = g.x * f.x;
+                    o[2 * e + 1] = g.y * f.y;
                   } else {
-                    v0 = act_of<ACT>(z0) + xe.x;
-                    v1 = act_of<ACT>(z1) + xe.y;
+                    const float2 f = act_of<ACT>(z);
+                    o[2 * e] = f.x;
+                    o[2 * e + 1] = f.y;
+                    if (a.has_extra) {
+                      const float2 r = Pack<T>::get(xs[e]);
+                      o[2 * e] += r.x;
+                      o[2 * e + 1] += r.y;
+                    }
                   }
                 }
               }
-              const float* w = v + u * 8;
-              at[slot] = make_uint4(Pack<T>::two(w[0], w[1]), Pack<T>::two(w[2], w[3]), Pack<T>::two(w[4], w[5]),
-                                    Pack<T>::two(w[6], w[7]));
+              at[slot] = make_uint4(Pack<T>::two(o[0], o[1]), Pack<T>::two(o[2], o[3]), Pack<T>::two(o[4], o[5]),
+                                    Pack<T>::two(o[6], o[7]));
             }
           }
         }
         if (s + 1 == subs) {  // the accumulator has been read
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&s_free[wg]));
+          if (lane == 0) arrive_leader<CG>(smem_u32(&s_free[wg]));
         }
         if (EPI == kEpiSlab || a.io_tma) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           group_sync(wg);
-          if (leader && !dead && !*fail) {
+          if (leader && !dead && !*fail && m0 < a.M) {  // a pair's second half may lie past the last row
             const int y = EPI == kEpiSlab ? tl.split * a.slab_rows + (int)m0 : (int)m0;
             if (EPI == kEpiSlab && a.slab_add)
               tma_add_2d(&tmO, smem_u32(buf), col, y);
@@ -594,9 +775,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   }
   __syncthreads();
+  if (CG == 2) cluster_sync();  // the pair is done with each other's barriers and TMEM
   if (warp == kMmaWarp) {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(2 * BN)));
+    if (CG == 1)
+      asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(2 * BN)));
+    else
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((uint32_t)(2 * BN)));
   }
 }
 
@@ -842,27 +1027,37 @@ constexpr CUtensorMapDataType map_type()
   return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
 
-template <int EPI, typename T, int BN, int ACT>
+template <int EPI, typename T, int CG, int ACT>
 void launch_gemm(GemmArgs& a, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tx, const CUtensorMap& to,
                  cudaStream_t s)
 {
-  using S = Shape<EPI, BN>;
+  using S = Shape<EPI, CG>;
   static std::atomic<uint64_t> ready{0};  // devices whose shared-memory limit has been raised
   int dev = 0;
   RBQ_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !(ready.load() >> dev & 1)) {
-    RBQ_CUDA(cudaFuncSetAttribute(gemm_kernel<EPI, T, BN, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
+    RBQ_CUDA(cudaFuncSetAttribute(gemm_kernel<EPI, T, CG, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   const int64_t total = (int64_t)a.tiles_m * a.tiles_n * a.splits;
-  const int grid = (int)std::min<int64_t>(total, sm_count());
-  gemm_kernel<EPI, T, BN, ACT><<<grid, kThreads, S::kBytes, s>>>(ta, tb, tx, to, a);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(total, sm_count() / CG)));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = S::kBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = CG;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  RBQ_CUDA(cudaLaunchKernelEx(&cfg, gemm_kernel<EPI, T, CG, ACT>, ta, tb, tx, to, a));
   RBQ_LAUNCHED();
 }
 
-// One product.  A is [M, K] (or [K, M] with a_mn), B [N, K] (or [K, N] with b_mn).
+// One product.  A is [M, K] (or [K, M] with a_mn), B [N, K] (or [K, N] with b_mn); cg as in the kernel.
 template <int EPI, typename T, int ACT = RBQ_ACT_NONE>
-void gemm(GemmArgs a, Matrix A, bool a_mn, Matrix B, bool b_mn, int bn, const CUtensorMap* tx, const CUtensorMap* to,
+void gemm(GemmArgs a, Matrix A, bool a_mn, Matrix B, bool b_mn, int cg, const CUtensorMap* tx, const CUtensorMap* to,
           cudaStream_t s)
 {
   a.M = a_mn ? A.cols : A.rows;
@@ -870,44 +1065,39 @@ void gemm(GemmArgs a, Matrix A, bool a_mn, Matrix B, bool b_mn, int bn, const CU
   const int64_t K = a_mn ? A.rows : A.cols;
   a.a_mn = a_mn;
   a.b_mn = b_mn;
-  const int64_t tm = ceil_div(a.M, kBM), tn = ceil_div(a.N, bn), kb = ceil_div(K, kBK);
-  RBQ_CHECK(tm * tn * a.splits < (1ll << 31) && kb < (1 << 30) && K < (1ll << 31) && a.M < (1ll << 31) - 128,
-            RBQ_ERR_INVALID, "matrix product: sizes too large");
+  const int64_t tm = ceil_div(a.M, kBM * cg), tn = ceil_div(a.N, 128 * cg), kb = ceil_div(K, kBK);
+  RBQ_CHECK(tm * tn * a.splits < (1ll << 31) && K < (1ll << 31) && a.M < (1ll << 31) - 256, RBQ_ERR_INVALID,
+            "matrix product: sizes too large");
   a.tiles_m = (int)tm;
   a.tiles_n = (int)tn;
   a.kblocks = (int)kb;
   a.m_fast = tm <= tn;  // the operand with fewer tiles stays in L2 while the other streams by once
   const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   a.idesc = (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
-            ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(kBM >> 4) << 24);
-  const CUtensorMap ta = tile_map(A.p, map_type<T>(), 2, A.rows, A.cols, A.ld, 64, a_mn ? kBK : kBM);
-  const CUtensorMap tb = tile_map(B.p, map_type<T>(), 2, B.rows, B.cols, B.ld, 64, b_mn ? kBK : bn);
+            ((uint32_t)(128 * cg >> 3) << 17) | ((uint32_t)(kBM * cg >> 4) << 24);
+  const CUtensorMap ta = tile_map(A.p, map_type<T>(), 2, A.rows, A.cols, A.ld, 64, a_mn ? kBK : 128);
+  const CUtensorMap tb = tile_map(B.p, map_type<T>(), 2, B.rows, B.cols, B.ld, 64, b_mn ? kBK : 128);
   const CUtensorMap& x = tx ? *tx : ta;
   const CUtensorMap& o = to ? *to : ta;
-  if (bn == 256)
-    launch_gemm<EPI, T, 256, ACT>(a, ta, tb, x, o, s);
+  if (cg == 2)
+    launch_gemm<EPI, T, 2, ACT>(a, ta, tb, x, o, s);
   else
-    launch_gemm<EPI, T, 128, ACT>(a, ta, tb, x, o, s);
+    launch_gemm<EPI, T, 1, ACT>(a, ta, tb, x, o, s);
 }
 
-// Tile width: 256 columns feed the tensor cores with the fewest operand bytes; 128 where the product
-// has too few tiles to fill the SMs or no more columns.
-int tile_width(int64_t M, int64_t N, int splits = 1)
-{
-  if (N <= 128) return 128;
-  return ceil_div(M, kBM) * ceil_div(N, 256) * splits >= sm_count() ? 256 : 128;
-}
+// CTAs of a tile: pairs with 256 x 256 tiles where there is one for every SM pair, else single CTAs
+// with 128 x 128 tiles, which spread a small product over four times as many SMs.
+int group_size(int64_t M, int64_t N) { return N > 128 && ceil_div(M, 256) * ceil_div(N, 256) >= sm_count() / 2 ? 2 : 1; }
 
-// Splits along k of a slab product: the smallest estimated time, in units of one k-block's MMAs (about
-// 0.3 us on a tile).  A split costs its share of the k-blocks, about 8 units to fill and drain, and
+// Splits along k of a slab product over `slots` CTAs or pairs: the smallest estimated time, in units
+// of one k-block's MMAs (about 0.3 us on a tile).  A split costs its share of the k-blocks, about 8 units to fill and drain, and
 // 0.15 units a tile for writing its slab and reading it back.
-int plan_splits(int64_t tiles, int64_t kblocks, int most)
+int plan_splits(int64_t tiles, int64_t kblocks, int slots, int most)
 {
-  const int sms = sm_count();
   int best = 1;
   double cost = 1e300;
   for (int s = 1; s <= most && s <= kblocks; ++s) {
-    const double c = (double)ceil_div(tiles * s, sms) * ((double)ceil_div(kblocks, s) + 8.0) + 0.15 * tiles * s;
+    const double c = (double)ceil_div(tiles * s, slots) * ((double)ceil_div(kblocks, s) + 8.0) + 0.15 * tiles * s;
     if (c < cost * 0.999) cost = c, best = s;
   }
   return best;
@@ -948,15 +1138,15 @@ Matrix addressable(const void* p, int64_t rows, int cols, Carver& ws, bool run, 
 // out[M, N] = alpha * A B^T through slabs (or at once where one split is best), dense rows.
 // `slabs` of slab_floats(): null to let the caller count.
 struct SlabPlan {
-  int bn, splits;
+  int cg, splits;
   int64_t rows, ld;  // of a slab
   int64_t floats() const { return (int64_t)splits * rows * ld; }
 };
 SlabPlan plan_slabs(int64_t M, int N, int64_t K)
 {
   SlabPlan p;
-  p.bn = N <= 128 ? 128 : 256;
-  p.splits = plan_splits(ceil_div(M, kBM) * ceil_div(N, p.bn), ceil_div(K, kBK), 64);
+  p.cg = N > 128 && M > 128 ? 2 : 1;
+  p.splits = plan_splits(ceil_div(M, kBM * p.cg) * ceil_div(N, 128 * p.cg), ceil_div(K, kBK), sm_count() / p.cg, 64);
   p.rows = round_up(M, kBM);
   p.ld = round_up(N, 4);
   while (p.splits > 1 && p.splits * p.rows >= (1ll << 31)) --p.splits;
@@ -971,7 +1161,7 @@ void slab_gemm(const SlabPlan& p, Matrix A, bool a_mn, Matrix B, bool b_mn, floa
   a.slab_rows = (int)p.rows;
   a.slab_add = add;
   const CUtensorMap to = tile_map(slabs, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.splits * p.rows, N, p.ld, 32, kBM);
-  gemm<kEpiSlab, T>(a, A, a_mn, B, b_mn, p.bn, nullptr, &to, s);
+  gemm<kEpiSlab, T>(a, A, a_mn, B, b_mn, p.cg, nullptr, &to, s);
 }
 template <typename T>
 void add_slabs(const SlabPlan& p, const float* slabs, int64_t M, int N, float alpha, const float* alpha_dev, T* out,
@@ -996,7 +1186,7 @@ void store_gemm(Matrix A, bool a_mn, Matrix B, bool b_mn, float alpha, const flo
   a.io_tma = N % 8 == 0;
   CUtensorMap to{};
   if (a.io_tma) to = tile_map(out, map_type<T>(), 2, M, N, N, 64, kBM);
-  gemm<kEpiLinear, T>(a, A, a_mn, B, b_mn, tile_width(M, N), nullptr, a.io_tma ? &to : nullptr, s);
+  gemm<kEpiLinear, T>(a, A, a_mn, B, b_mn, group_size(M, N), nullptr, a.io_tma ? &to : nullptr, s);
 }
 
 template <typename T>
@@ -1017,14 +1207,14 @@ void linear_forward(const T* x, const T* w, const T* bias, const T* residual, T*
     to = tile_map(y, map_type<T>(), 2, m, n, n, 64, kBM);
     tx = residual ? tile_map(residual, map_type<T>(), 2, m, n, n, 64, kBM) : to;
   }
-  const int bn = tile_width(m, n);
+  const int cg = group_size(m, n);
   const CUtensorMap *px = a.io_tma ? &tx : nullptr, *po = a.io_tma ? &to : nullptr;
   if (act == RBQ_ACT_GELU)
-    gemm<kEpiLinear, T, RBQ_ACT_GELU>(a, X, false, W, false, bn, px, po, s);
+    gemm<kEpiLinear, T, RBQ_ACT_GELU>(a, X, false, W, false, cg, px, po, s);
   else if (act == RBQ_ACT_RELU)
-    gemm<kEpiLinear, T, RBQ_ACT_RELU>(a, X, false, W, false, bn, px, po, s);
+    gemm<kEpiLinear, T, RBQ_ACT_RELU>(a, X, false, W, false, cg, px, po, s);
   else
-    gemm<kEpiLinear, T>(a, X, false, W, false, bn, px, po, s);
+    gemm<kEpiLinear, T>(a, X, false, W, false, cg, px, po, s);
 }
 
 // dz = g * act'(x w^T + b) recomputes the layer's product: for the encoder's widths (k = 256) that
@@ -1057,12 +1247,12 @@ void linear_backward(const T* g, const T* x, const T* w, const T* bias, T* dx, T
         tx = tile_map(g, map_type<T>(), 2, m, n, n, 64, kBM);
         to = tile_map(z, map_type<T>(), 2, m, n, ld, 64, kBM);
       }
-      const int bn = tile_width(m, n);
+      const int cg = group_size(m, n);
       const CUtensorMap *px = a.io_tma ? &tx : nullptr, *po = a.io_tma ? &to : nullptr;
       if (act == RBQ_ACT_GELU)
-        gemm<kEpiActGrad, T, RBQ_ACT_GELU>(a, X, false, W, false, bn, px, po, s);
+        gemm<kEpiActGrad, T, RBQ_ACT_GELU>(a, X, false, W, false, cg, px, po, s);
       else
-        gemm<kEpiActGrad, T, RBQ_ACT_RELU>(a, X, false, W, false, bn, px, po, s);
+        gemm<kEpiActGrad, T, RBQ_ACT_RELU>(a, X, false, W, false, cg, px, po, s);
     }
   }
   const SlabPlan plan = plan_slabs(n, k, m);
@@ -1089,15 +1279,15 @@ void loss_forward(const T* q, const T* bank, const int64_t* target, int64_t n, i
                   float* lse, Carver& ws, bool run, cudaStream_t s)
 {
   const Matrix Q = addressable(q, n, d, ws, run, s), B = addressable(bank, v, d, ws, run, s);
-  const int bn = tile_width(n, v);
-  const int64_t tiles = ceil_div(v, bn);
+  const int cg = group_size(n, v);
+  const int64_t tiles = ceil_div(v, 128 * cg);
   float2* partial = ws.take<float2>(tiles * n);
   if (!run) return;
   GemmArgs a;
   a.c2 = scale * kLog2e;
   a.target = target;
   a.partial = partial;
-  gemm<kEpiLse, T>(a, Q, false, B, false, bn, nullptr, nullptr, s);
+  gemm<kEpiLse, T>(a, Q, false, B, false, cg, nullptr, nullptr, s);
   loss_rows_kernel<T><<<(unsigned)ceil_div(n, 32), 1024, 0, s>>>(partial, (int)tiles, n, q, d, bank, d, d, v, target, scale,
                                                                  loss, lse);
   RBQ_LAUNCHED();
@@ -1139,7 +1329,7 @@ void loss_backward(const float* g, const T* q, const T* bank, const int64_t* tar
     a.target = target;
     a.rows = rows;
     const CUtensorMap to = tile_map(prob, map_type<T>(), 2, n, cols, piece, 64, kBM);
-    gemm<kEpiProb, T>(a, Q, false, Bp, false, tile_width(n, cols), nullptr, &to, s);
+    gemm<kEpiProb, T>(a, Q, false, Bp, false, group_size(n, cols), nullptr, &to, s);
     if (dq) {
       SlabPlan p = pq;  // the last, shorter piece keeps the slabs; no split may be empty
       const int64_t kb = ceil_div(cols, kBK);
