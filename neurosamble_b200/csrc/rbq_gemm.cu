@@ -11,7 +11,8 @@
 // CTA (320 threads, persistent over output tiles): warp 8 streams 64-wide k-blocks of A and B by TMA into
 // a ring of shared-memory stages (128-byte swizzle, zero fill past the edges), warp 9 issues the MMAs
 // into one of two accumulators (2 x BN of the 512 TMEM columns), and two warpgroups take the
-// finished accumulators in turn, so that the epilogue of one tile runs beside the MMAs of the next.
+// two column halves of the finished one, so that the epilogue of one tile runs beside the MMAs of
+// the next.  (A tile for each warpgroup in turn held both accumulators for as long again.)
 // In an epilogue thread r owns output row r (TMEM lane r).
 //
 // Two shapes.  CG = 2, products with enough tiles for every SM pair: two CTAs of a cluster share a
@@ -83,7 +84,7 @@ struct GemmArgs {
   float c2 = 0.0f;       // scale * log2(e)
   int64_t col0 = 0;
   const int64_t* target = nullptr;   // [M]
-  float2* partial = nullptr;         // [tiles_n, M] (max, sum), base 2
+  float2* partial = nullptr;         // [tiles_n * 2, M] (max, sum) of half a tile's columns, base 2
   const float4* rows = nullptr;      // [M] GradRows
 };
 
@@ -170,7 +171,8 @@ __device__ __forceinline__ void arrive_leader(uint32_t bar)
   if (CG == 1)
     mbar_arrive(bar);
   else
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
+    // what the arrival orders is TMEM reads, and the tcgen05 fence before it has
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_addr(bar)) : "memory");
 }
 
 __device__ __forceinline__ void cluster_sync()
@@ -184,8 +186,7 @@ __device__ __forceinline__ bool op_wait(uint32_t bar, uint32_t parity, volatile 
   for (uint32_t it = 0; it < kOpWaitLimit; ++it) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, "
-        "p;\n}"
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
         : "memory");
@@ -387,7 +388,7 @@ struct Shape {
   static constexpr bool kStaged = EPI != kEpiLse;     // the loss's forward pass writes no tile
   static constexpr int kStages = !kStaged ? 6 : CG == 2 ? 4 : 5;
   static constexpr int kOutBytes = kStaged ? 4 * kStageOut : 0;  // two buffers per warpgroup
-  static constexpr int kBytes = kStages * kOperands + kOutBytes + 2 * kBN * 4 + 1024;
+  static constexpr int kBytes = kStages * kOperands + kOutBytes + kBN * 4 + 1024;
 };
 
 // The warp's 32 staging rows <-> a matrix whose rows no TMA can address, 64 columns from `col`.
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   unsigned char* base = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* staging = base + S::kStages * S::kOperands;
-  float* s_bias = reinterpret_cast<float*>(staging + S::kOutBytes);  // [2][BN]
+  float* s_bias = reinterpret_cast<float*>(staging + S::kOutBytes);  // [BN]
   __shared__ __align__(8) unsigned long long s_full[S::kStages], s_empty[S::kStages], s_done[2], s_free[2], s_x[4];
   __shared__ uint32_t s_tmem;
   __shared__ int s_fail;
@@ -450,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&s_done[i]), 1);
-      mbar_init(smem_u32(&s_free[i]), 4 * CG);  // one arrival per epilogue warp of the pair
+      mbar_init(smem_u32(&s_free[i]), 8 * CG);  // one arrival per epilogue warp of the pair
     }
     for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&s_x[i]), 1);
     s_fail = 0;
@@ -552,43 +553,73 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int wg = warp >> 2, quarter = warp & 3;
     const int gt = tid & 127;  // thread of the warpgroup = accumulator lane = output row
     const bool leader = gt == 0;
-    unsigned char* bufs = staging + wg * 2 * kStageOut;
-    float* bias = s_bias + wg * BN;
-    const uint32_t acc_addr = tmem + wg * BN + ((uint32_t)(quarter * 32) << 16);
+    constexpr int kHalf = BN / 2;                    // columns of the tile that this warpgroup takes
     constexpr int kSub = EPI == kEpiSlab ? 32 : 64;  // columns of one 128-byte staging row
+    unsigned char* bufs = staging + wg * 2 * kStageOut;
+    float* bias = s_bias + wg * kHalf;
     bool dead = false;  // a wait failed: keep the barriers in step, touch nothing
     int c = 0;          // staging tile, counted over the warpgroup's run: buffer c & 1
 
+    auto subs_of = [&](const Tile& tl) {  // staging tiles of the warpgroup's half that hold columns
+      return max(0, min(kHalf / kSub, (a.N - tl.n * BN - wg * kHalf + kSub - 1) / kSub));
+    };
     // The extra input of staging tile c arrives by TMA one tile ahead.
-    auto load_extra = [&](int cc, int t, int s) {
-      const Tile tl = tile_at(a, t);
+    auto load_extra = [&](int cc, const Tile& tl, int s) {
       const uint32_t bar = smem_u32(&s_x[wg * 2 + (cc & 1)]);
       mbar_expect_tx(bar, (uint32_t)kStageOut);
-      tma_load_2d(smem_u32(bufs + (cc & 1) * kStageOut), &tmX, tl.n * BN + s * 64, (tl.m * CG + rank) * kBM, bar);
+      tma_load_2d(smem_u32(bufs + (cc & 1) * kStageOut), &tmX, tl.n * BN + wg * kHalf + s * 64, (tl.m * CG + rank) * kBM,
+                  bar);
     };
     const bool extra_tma = (EPI == kEpiLinear || EPI == kEpiActGrad) && a.has_extra && a.io_tma;
-    int loaded = 0;  // extra tiles asked for (leader)
-    if (extra_tma && leader) {
-      const int t = first_tile + wg * tile_step;
-      if (t < total) {
-        load_extra(0, t, 0);
-        loaded = 1;
+    int loaded = 0;                 // extra tiles asked for (leader)
+    int ask_t = first_tile, ask_s = 0;  // the next one to ask for
+    auto ask_extra = [&]() {
+      for (; ask_t < total; ask_t += tile_step, ask_s = 0) {
+        const Tile tl = tile_at(a, ask_t);
+        if (ask_s < subs_of(tl)) {
+          load_extra(loaded++, tl, ask_s++);
+          return;
+        }
       }
-    }
+    };
+    if (extra_tma && leader) ask_extra();
 
-    for (int i = wg, t = first_tile + wg * tile_step; t < total; i += 2, t += 2 * tile_step) {
+    // What a thread needs of the next tile besides the accumulator is read one tile ahead.
+    float next_bias = 0.0f;
+    int64_t next_target = -1;
+    float4 next_rows = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto read_ahead = [&](int t) {
+      if (t >= total) return;
       const Tile tl = tile_at(a, t);
+      const int64_t row = (int64_t)(tl.m * CG + rank) * kBM + gt;
+      if (EPI == kEpiLinear || EPI == kEpiActGrad) {
+        const int col = tl.n * BN + wg * kHalf + gt;
+        next_bias = a.bias != nullptr && gt < kHalf && col < a.N
+                        ? Pack<T>::one(reinterpret_cast<const T*>(a.bias)[col])
+                        : 0.0f;
+      }
+      if (EPI == kEpiLse || EPI == kEpiProb) next_target = row < a.M ? __ldg(a.target + row) : -1;
+      if (EPI == kEpiProb) next_rows = row < a.M ? __ldg(a.rows + row) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    };
+    read_ahead(first_tile);
+
+    for (int i = 0, t = first_tile; t < total; ++i, t += tile_step) {
+      const Tile tl = tile_at(a, t);
+      const int acc = i & 1;
+      const uint32_t acc_addr = tmem + acc * BN + wg * kHalf + ((uint32_t)(quarter * 32) << 16);
       const int64_t m0 = (int64_t)(tl.m * CG + rank) * kBM;
-      const int n0 = tl.n * BN;
+      const int n0 = tl.n * BN + wg * kHalf;
       const int64_t row = m0 + gt;
+      const int64_t trow = next_target < 0 ? -1 : next_target - a.col0 - n0;
+      const GradRows gr{next_rows.x, next_rows.y, next_rows.z, next_rows.w};
       if (EPI == kEpiLinear || EPI == kEpiActGrad) {
         group_sync(wg);  // the last tile's values have been used
-        for (int j = gt; j < BN; j += 128)
-          bias[j] = a.bias != nullptr && n0 + j < a.N ? Pack<T>::one(reinterpret_cast<const T*>(a.bias)[n0 + j]) : 0.0f;
+        if (gt < kHalf) bias[gt] = next_bias;
         group_sync(wg);
       }
+      read_ahead(t + tile_step);
       if (!dead) {
-        const bool ok = op_wait(smem_u32(&s_done[wg]), (uint32_t)((i >> 1) & 1), fail);
+        const bool ok = op_wait(smem_u32(&s_done[acc]), (uint32_t)((i >> 1) & 1), fail);
         if (!__all_sync(0xffffffffu, ok)) {
           if (lane == 0) fail_with(fail, 4);
           dead = true;
@@ -597,11 +628,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 
       if (EPI == kEpiLse) {
-        const int64_t trow = row < a.M ? __ldg(a.target + row) - a.col0 - n0 : -1;
         float m = -INFINITY, l = 0.0f;
-        if (!dead) {
-#pragma unroll 1
-          for (int j = 0; j < BN / 64; ++j) {
+        if (!dead && n0 < a.N) {
+#pragma unroll
+          for (int j = 0; j < kHalf / 64; ++j) {
             float v[64];
             tc_ld64(acc_addr + j * 64, v);
             const int64_t tj = trow - j * 64;
@@ -625,28 +655,26 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float2 x = split(fma2(pair(v[e], v[e + 1]), c2, nref));
               sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(ex2(x.x), ex2(x.y)));
             }
-            const float2 t = split(add2(sum[0], sum[1]));
-            l = fmaf(l, ex2(m - ref), t.x + t.y);
+            const float2 t2 = split(add2(sum[0], sum[1]));
+            l = fmaf(l, ex2(m - ref), t2.x + t2.y);
             m = mn;
           }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) arrive_leader<CG>(smem_u32(&s_free[wg]));
-        if (!dead && row < a.M) a.partial[(int64_t)tl.n * a.M + row] = make_float2(m, l);
+        if (lane == 0) arrive_leader<CG>(smem_u32(&s_free[acc]));
+        if (!dead && row < a.M) a.partial[(int64_t)(tl.n * 2 + wg) * a.M + row] = make_float2(m, l);
         continue;
       }
 
-      GradRows gr{};
-      int64_t trow = -1;
-      if (EPI == kEpiProb && row < a.M) {
-        const float4 q = __ldg(a.rows + row);
-        gr = GradRows{q.x, q.y, q.z, q.w};
-        trow = __ldg(a.target + row) - a.col0 - n0;
-      }
       float alpha = a.alpha;
       if (a.alpha_dev != nullptr) alpha *= __ldg(a.alpha_dev);
-      const int subs = min(BN / kSub, (a.N - n0 + kSub - 1) / kSub);
+      const int subs = subs_of(tl);
+      if (subs == 0) {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) arrive_leader<CG>(smem_u32(&s_free[acc]));
+      }
 #pragma unroll 1
       for (int s = 0; s < subs; ++s, ++c) {
         unsigned char* buf = bufs + (c & 1) * kStageOut;
@@ -654,13 +682,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (extra_tma) {
           // ask for the next tile's extra input: its buffer's last store has been read
           if (leader && !dead) {
-            int nt = t, ns = s + 1;
-            if (ns == subs) nt = t + 2 * tile_step, ns = 0;
-            if (nt < total) {
-              asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-              load_extra(c + 1, nt, ns);
-              ++loaded;
-            }
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            ask_extra();
           }
           if (!dead) {
             const bool ok = op_wait(smem_u32(&s_x[wg * 2 + (c & 1)]), (uint32_t)((c >> 1) & 1), fail);
@@ -745,7 +768,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (s + 1 == subs) {  // the accumulator has been read
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
-          if (lane == 0) arrive_leader<CG>(smem_u32(&s_free[wg]));
+          if (lane == 0) arrive_leader<CG>(smem_u32(&s_free[acc]));
         }
         if (EPI == kEpiSlab || a.io_tma) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -1280,7 +1303,7 @@ void loss_forward(const T* q, const T* bank, const int64_t* target, int64_t n, i
 {
   const Matrix Q = addressable(q, n, d, ws, run, s), B = addressable(bank, v, d, ws, run, s);
   const int cg = group_size(n, v);
-  const int64_t tiles = ceil_div(v, 128 * cg);
+  const int64_t tiles = 2 * ceil_div(v, 128 * cg);
   float2* partial = ws.take<float2>(tiles * n);
   if (!run) return;
   GemmArgs a;
