@@ -8,12 +8,12 @@
 // rows contiguous ("MN-major": the same matrices inside a gradient, where the sum runs over the
 // stored rows); the tensor cores read both, so no operand is ever transposed in memory.
 //
-// CTA (320 threads, persistent over output tiles): warp 8 streams 64-wide k-blocks of A and B by TMA into
-// a ring of shared-memory stages (128-byte swizzle, zero fill past the edges), warp 9 issues the MMAs
-// into one of two accumulators (2 x BN of the 512 TMEM columns), and two warpgroups take the
-// two column halves of the finished one, so that the epilogue of one tile runs beside the MMAs of
-// the next.  (A tile for each warpgroup in turn held both accumulators for as long again.)
-// In an epilogue thread r owns output row r (TMEM lane r).
+// CTA, persistent over output tiles: one warp streams 64-wide k-blocks of A and B by TMA into a ring
+// of shared-memory stages (128-byte swizzle, zero fill past the edges), one warp issues the MMAs into
+// one of two accumulators (2 x BN of the 512 TMEM columns), and BN / 64 warpgroups take 64 columns each
+// of the finished one; thread r of a group owns row r (TMEM lane r).  The accumulator is free again
+// as soon as its columns are in registers, and the epilogue's arithmetic runs beside the next tiles'
+// MMAs, with four warps per scheduler to hide its latencies.
 //
 // Two shapes.  CG = 2, products with enough tiles for every SM pair: two CTAs of a cluster share a
 // 256 x 256 tile (cta_group::2), each holding 128 rows of A and 128 of B per stage, so that a CTA
@@ -44,8 +44,6 @@ namespace {
 
 constexpr int kBM = 128;       // output rows of a tile (TMEM lanes)
 constexpr int kBK = 64;        // reduction values per stage: one 128-byte row of 16-bit values
-constexpr int kThreads = 320;  // two epilogue warpgroups, the loader warp, the MMA warp
-constexpr int kLoadWarp = 8, kMmaWarp = 9;
 constexpr int kStageOut = kBM * 128;          // one staging buffer: 128 rows of 128 bytes
 constexpr uint32_t kOpWaitLimit = 1u << 22;   // polls; each suspends for up to some microseconds
 constexpr float kLog2e = 1.4426950408889634f;
@@ -65,6 +63,8 @@ struct GemmArgs {
   int64_t M = 0;
   int N = 0;
   int tiles_m = 0, tiles_n = 0, splits = 1, kblocks = 0;
+  int run = 1, units = 0;  // see Walk
+  int len_fast = 0, len_slow = 0, step_fast = 0, step_slow = 0, step_split = 0;
   int m_fast = 0;        // tile order: rows of tiles vary fastest, else columns
   int a_mn = 0, b_mn = 0;  // operand stored with its rows contiguous
   uint32_t idesc = 0;
@@ -84,7 +84,7 @@ struct GemmArgs {
   float c2 = 0.0f;       // scale * log2(e)
   int64_t col0 = 0;
   const int64_t* target = nullptr;   // [M]
-  float2* partial = nullptr;         // [tiles_n * 2, M] (max, sum) of half a tile's columns, base 2
+  float2* partial = nullptr;         // [runs_n * groups, M] (max, sum) of a group's columns, base 2
   const float4* rows = nullptr;      // [M] GradRows
 };
 
@@ -340,42 +340,48 @@ __device__ __forceinline__ float2 act_slope(uint64_t z)
   return make_float2(1.0f, 1.0f);
 }
 
-// 64 consecutive fp32 accumulator columns of the warp's 32 TMEM lanes.
-__device__ __forceinline__ void tc_ld64(uint32_t taddr, float (&v)[64])
-{
-  uint32_t r[64];
-#define RBQ_R8(i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32, %33, %34, %35, %36, %37, %38, "
-      "%39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, "
-      "%62, %63}, [%64];"
-      : RBQ_R8(0), RBQ_R8(8), RBQ_R8(16), RBQ_R8(24), RBQ_R8(32), RBQ_R8(40), RBQ_R8(48), RBQ_R8(56)
-      : "r"(taddr));
-#undef RBQ_R8
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
-}
-
+// A unit of work is a run of `run` tiles next to each other in one row of tiles (one tile but for the
+// loss's forward pass).  Units vary fastest along the shorter side of the product, then along the other,
+// then over the splits.
 struct Tile {
   int m, n, split;
 };
-__device__ __forceinline__ Tile tile_at(const GemmArgs& a, int t)
-{
-  Tile r;
-  const int per = a.tiles_m * a.tiles_n;
-  r.split = t / per;
-  const int i = t - r.split * per;
-  if (a.m_fast) {
-    r.n = i / a.tiles_m;
-    r.m = i - r.n * a.tiles_m;
-  } else {
-    r.m = i / a.tiles_n;
-    r.n = i - r.m * a.tiles_n;
+// Steps through a CTA's (or pair's) tiles in order; every role walks the same sequence.  A step
+// adds the grid's size to the unit's (fast, slow, split) digits: no division, which every thread of
+// the epilogue would pay for at each tile.
+struct Walk {
+  const GemmArgs& a;
+  int fast, slow, split, r;
+  __device__ __forceinline__ Walk(const GemmArgs& args, int first) : a(args), r(0)
+  {
+    const int per = a.len_fast * a.len_slow;
+    split = first / per;
+    slow = (first - split * per) / a.len_fast;
+    fast = first - split * per - slow * a.len_fast;
   }
-  return r;
-}
+  __device__ __forceinline__ bool live() const { return split < a.splits; }
+  __device__ __forceinline__ Tile tile() const
+  {
+    return a.m_fast ? Tile{fast, slow * a.run + r, split} : Tile{slow, fast * a.run + r, split};
+  }
+  __device__ __forceinline__ bool run_ends() const
+  {
+    return r + 1 == a.run || (a.m_fast ? slow : fast) * a.run + r + 1 == a.tiles_n;
+  }
+  __device__ __forceinline__ void next()
+  {
+    if (!run_ends()) {
+      ++r;
+      return;
+    }
+    r = 0;
+    fast += a.step_fast;
+    slow += a.step_slow;
+    split += a.step_split;
+    if (fast >= a.len_fast) fast -= a.len_fast, ++slow;
+    if (slow >= a.len_slow) slow -= a.len_slow, ++split;
+  }
+};
 __device__ __forceinline__ int k_begin(const GemmArgs& a, int split)
 {
   return (int)((int64_t)a.kblocks * split / a.splits);
@@ -383,12 +389,18 @@ __device__ __forceinline__ int k_begin(const GemmArgs& a, int split)
 
 template <int EPI, int CG>
 struct Shape {
-  static constexpr int kBN = 128 * CG;                // columns of a tile and of its accumulator
-  static constexpr int kOperands = 2 * kBM * 128;     // a CTA's share of a stage: 128 rows of A, 128 of B
-  static constexpr bool kStaged = EPI != kEpiLse;     // the loss's forward pass writes no tile
-  static constexpr int kStages = !kStaged ? 6 : CG == 2 ? 4 : 5;
-  static constexpr int kOutBytes = kStaged ? 4 * kStageOut : 0;  // two buffers per warpgroup
-  static constexpr int kBytes = kStages * kOperands + kOutBytes + kBN * 4 + 1024;
+  static constexpr int kBN = 128 * CG;             // columns of a tile and of its accumulator
+  static constexpr int kGroups = kBN / 64;         // epilogue warpgroups
+  static constexpr int kThreads = kGroups * 128 + 64;
+  static constexpr int kLoadWarp = kGroups * 4, kMmaWarp = kLoadWarp + 1;
+  static constexpr int kOperands = 2 * kBM * 128;  // a CTA's share of a stage: 128 rows of A, 128 of B
+  // Staging buffers per group: none in the loss's forward pass, which writes no tile; two where an extra
+  // input streams in for every tile (its load then overlaps the tile before), else one.
+  static constexpr int kBufs = EPI == kEpiLse ? 0 : EPI == kEpiActGrad ? 2 : 1;
+  static constexpr int kOutBytes = kGroups * kBufs * kStageOut;
+  static constexpr int kFit = (226 * 1024 + 512 - 1024 - 2 * kBN * 4 - kOutBytes) / kOperands;  // stages of 227 KB less the barriers
+  static constexpr int kStages = kFit < 6 ? kFit : 6;
+  static constexpr int kBytes = kStages * kOperands + kOutBytes + 2 * kBN * 4 + 1024;
 };
 
 // The warp's 32 staging rows <-> a matrix whose rows no TMA can address, 64 columns from `col`.
@@ -414,25 +426,26 @@ __device__ __forceinline__ void move_rows(unsigned char* buf, T* mat, int64_t ro
 }
 
 template <int EPI, typename T, int CG, int ACT>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                 const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmO,
                 const __grid_constant__ GemmArgs a)
 {
   using S = Shape<EPI, CG>;
-  constexpr int BN = S::kBN;
+  constexpr int BN = S::kBN, kLoadWarp = S::kLoadWarp, kMmaWarp = S::kMmaWarp, kGroups = S::kGroups;
   extern __shared__ unsigned char gemm_smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* staging = base + S::kStages * S::kOperands;
-  float* s_bias = reinterpret_cast<float*>(staging + S::kOutBytes);  // [BN]
-  __shared__ __align__(8) unsigned long long s_full[S::kStages], s_empty[S::kStages], s_done[2], s_free[2], s_x[4];
+  float* s_bias = reinterpret_cast<float*>(staging + S::kOutBytes);  // [2][BN]: this tile's and the next one's
+  __shared__ __align__(8) unsigned long long s_full[S::kStages], s_empty[S::kStages], s_done[2], s_free[2],
+      s_x[kGroups * 2];
   __shared__ uint32_t s_tmem;
   __shared__ int s_fail;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0;  // in the pair; 0 leads
-  const int first_tile = blockIdx.x / CG, tile_step = gridDim.x / CG;
+  const int first_unit = blockIdx.x / CG;
   if (warp == kMmaWarp) {
     if (CG == 1) {
       asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
@@ -451,9 +464,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&s_done[i]), 1);
-      mbar_init(smem_u32(&s_free[i]), 8 * CG);  // one arrival per epilogue warp of the pair
+      mbar_init(smem_u32(&s_free[i]), kGroups * 4 * CG);  // one arrival per epilogue warp of the pair
     }
-    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&s_x[i]), 1);
+    for (int i = 0; i < kGroups * 2; ++i) mbar_init(smem_u32(&s_x[i]), 1);
     s_fail = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -463,26 +476,26 @@ __global__ void __launch_bounds__(kThreads, 1)
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = s_tmem;
   volatile int* fail = &s_fail;
-  const int total = a.tiles_m * a.tiles_n * a.splits;
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmA)) : "memory");
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmB)) : "memory");
-      int c = 0;  // k-block, counted over the CTA's whole run: stage c % kStages
+      int st = 0, done = 0;  // stage of the next k-block; k-blocks asked for (kStages at most are counted)
+      uint32_t lap = 0;      // parity of the ring's laps
       bool ok = true;
-      for (int t = first_tile; t < total && ok; t += tile_step) {
-        const Tile tl = tile_at(a, t);
+      const uint32_t full0 = CG == 2 ? leader_addr(smem_u32(&s_full[0])) : smem_u32(&s_full[0]);
+      for (Walk w(a, first_unit); w.live() && ok; w.next()) {
+        const Tile tl = w.tile();
         const int m0 = (tl.m * CG + rank) * kBM, n0 = tl.n * BN + rank * 128;  // this CTA's rows of A and of B
-        for (int kb = k_begin(a, tl.split), ke = k_begin(a, tl.split + 1); kb < ke; ++kb, ++c) {
-          const int st = c % S::kStages;
-          if (c >= S::kStages && !op_wait(smem_u32(&s_empty[st]), (uint32_t)((c / S::kStages - 1) & 1), fail)) {
+        for (int kb = k_begin(a, tl.split), ke = k_begin(a, tl.split + 1); kb < ke; ++kb) {
+          if (done == S::kStages && !op_wait(smem_u32(&s_empty[st]), lap ^ 1, fail)) {
             fail_with(fail, 1);
             ok = false;
             break;
           }
-          const uint32_t full = CG == 2 ? leader_addr(smem_u32(&s_full[st])) : smem_u32(&s_full[st]);
-          const uint32_t sa = smem_u32(base + st * S::kOperands), sb = sa + kBM * 128;
+          const uint32_t full = full0 + st * 8;
+          const uint32_t sa = smem_u32(base) + st * S::kOperands, sb = sa + kBM * 128;
           if (rank == 0) mbar_expect_tx(smem_u32(&s_full[st]), (uint32_t)(CG * S::kOperands));
           const int k0 = kb * kBK;
           if (a.a_mn) {
@@ -497,90 +510,89 @@ __global__ void __launch_bounds__(kThreads, 1)
           } else {
             load_tile<CG>(sb, &tmB, k0, n0, full);
           }
+          if (done < S::kStages) ++done;
+          if (++st == S::kStages) st = 0, lap ^= 1;
         }
       }
-      // The pair's MMAs arrive on both CTAs' barriers: all have before this one's shared memory goes away.
-      if (ok)
-        for (int i = (c > S::kStages ? c - S::kStages : 0); i < c; ++i)
-          if (!op_wait(smem_u32(&s_empty[i % S::kStages]), (uint32_t)((i / S::kStages) & 1), fail)) {
-            fail_with(fail, 6);
-            break;
-          }
-      // Copies in flight after a failure land before the shared memory goes away (the leader's barriers
-      // count those of both CTAs).
-      if (*fail && rank == 0)
-        for (int i = (c > S::kStages ? c - S::kStages : 0); i < c; ++i)
-          mbar_wait(smem_u32(&s_full[i % S::kStages]), (uint32_t)((i / S::kStages) & 1));
+      // The last lap.  The pair's MMAs arrive on both CTAs' barriers: all have before this one's shared
+      // memory goes away.  After a failure the copies in flight land first (the leader's barriers count
+      // those of both CTAs).
+      for (int i = 0; i < done; ++i) {
+        if (st == 0) st = S::kStages, lap ^= 1;
+        --st;
+        if (!*fail && !op_wait(smem_u32(&s_empty[st]), lap, fail)) fail_with(fail, 6);
+        if (*fail && rank == 0) mbar_wait(smem_u32(&s_full[st]), lap);
+      }
     }
     __syncwarp();
   } else if (warp == kMmaWarp) {
     if (lane == 0 && rank == 0) {
-      const uint32_t a_step = a.a_mn ? 16 * 128 : 32, b_step = a.b_mn ? 16 * 128 : 32;  // 16 values of k
-      int c = 0, i = 0;
-      bool ok = true;
-      for (int t = first_tile; t < total && ok; t += tile_step, ++i) {
+      // One thread issues every MMA: descriptors are one addition each.
+      const uint32_t a_step = (a.a_mn ? 16 * 128 : 32) >> 4, b_step = (a.b_mn ? 16 * 128 : 32) >> 4;  // 16 values of k
+      const uint64_t a_desc = operand_desc(smem_u32(base), a.a_mn), b_desc = operand_desc(smem_u32(base) + kBM * 128, a.b_mn);
+      int st = 0, i = 0;
+      uint32_t lap = 0;
+      bool ok = true, any = false;
+      for (Walk w(a, first_unit); w.live() && ok; w.next(), ++i) {
         const int acc = i & 1;
         if (i >= 2 && !op_wait(smem_u32(&s_free[acc]), (uint32_t)(((i >> 1) - 1) & 1), fail)) {
           fail_with(fail, 2);
           break;
         }
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const int split = t / (a.tiles_m * a.tiles_n);
-        const int kb0 = k_begin(a, split), ke = k_begin(a, split + 1);
-        for (int kb = kb0; kb < ke; ++kb, ++c) {
-          const int st = c % S::kStages;
-          if (!op_wait(smem_u32(&s_full[st]), (uint32_t)((c / S::kStages) & 1), fail)) {
+        const uint32_t d = tmem + acc * BN;
+        uint32_t into = 0;  // the first MMA overwrites the accumulator
+        for (int left = k_begin(a, w.split + 1) - k_begin(a, w.split); left > 0; --left) {
+          if (!op_wait(smem_u32(&s_full[st]), lap, fail)) {
             fail_with(fail, 3);
             ok = false;
             break;
           }
           asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t sa = smem_u32(base + st * S::kOperands), sb = sa + kBM * 128;
+          const uint64_t ad = a_desc + st * (S::kOperands >> 4), bd = b_desc + st * (S::kOperands >> 4);
 #pragma unroll
-          for (int ks = 0; ks < kBK / 16; ++ks)
-            mma_f16<CG>(tmem + acc * BN, operand_desc(sa + ks * a_step, a.a_mn), operand_desc(sb + ks * b_step, a.b_mn),
-                    a.idesc, (kb > kb0 || ks > 0) ? 1u : 0u);
+          for (int ks = 0; ks < kBK / 16; ++ks) {
+            mma_f16<CG>(d, ad + ks * a_step, bd + ks * b_step, a.idesc, into);
+            into = 1;
+          }
           commit<CG>(smem_u32(&s_empty[st]));
+          any = true;
+          if (++st == S::kStages) st = 0, lap ^= 1;
         }
         if (ok) commit<CG>(smem_u32(&s_done[acc]));
       }
       // MMAs still running after a failure end before TMEM is freed: the last commit follows them.
-      if (*fail && c > 0)
-        mbar_wait(smem_u32(&s_empty[(c - 1) % S::kStages]), (uint32_t)(((c - 1) / S::kStages) & 1));
+      if (*fail && any) {
+        if (st == 0) st = S::kStages, lap ^= 1;
+        mbar_wait(smem_u32(&s_empty[st - 1]), lap);
+      }
     }
     __syncwarp();
   } else {
     const int wg = warp >> 2, quarter = warp & 3;
-    const int gt = tid & 127;  // thread of the warpgroup = accumulator lane = output row
+    const int gt = tid & 127;  // thread of the group = accumulator lane = output row
     const bool leader = gt == 0;
-    constexpr int kHalf = BN / 2;                    // columns of the tile that this warpgroup takes
-    constexpr int kSub = EPI == kEpiSlab ? 32 : 64;  // columns of one 128-byte staging row
-    unsigned char* bufs = staging + wg * 2 * kStageOut;
-    float* bias = s_bias + wg * kHalf;
+    constexpr bool kElement = EPI == kEpiLinear || EPI == kEpiActGrad;
+    unsigned char* bufs = staging + wg * S::kBufs * kStageOut;
+    float* bias = s_bias + wg * 64;
     bool dead = false;  // a wait failed: keep the barriers in step, touch nothing
-    int c = 0;          // staging tile, counted over the warpgroup's run: buffer c & 1
+    int c = 0;          // staging tile, counted over the group's run: buffer c % kBufs
+    auto buf_of = [&](int k) { return bufs + (S::kBufs == 2 ? (k & 1) * kStageOut : 0); };
+    auto bar_of = [&](int k) { return smem_u32(&s_x[wg * 2 + (S::kBufs == 2 ? k & 1 : 0)]); };
+    auto parity_of = [&](int k) { return (uint32_t)((S::kBufs == 2 ? k >> 1 : k) & 1); };
 
-    auto subs_of = [&](const Tile& tl) {  // staging tiles of the warpgroup's half that hold columns
-      return max(0, min(kHalf / kSub, (a.N - tl.n * BN - wg * kHalf + kSub - 1) / kSub));
-    };
-    // The extra input of staging tile c arrives by TMA one tile ahead.
-    auto load_extra = [&](int cc, const Tile& tl, int s) {
-      const uint32_t bar = smem_u32(&s_x[wg * 2 + (cc & 1)]);
-      mbar_expect_tx(bar, (uint32_t)kStageOut);
-      tma_load_2d(smem_u32(bufs + (cc & 1) * kStageOut), &tmX, tl.n * BN + wg * kHalf + s * 64, (tl.m * CG + rank) * kBM,
-                  bar);
-    };
-    const bool extra_tma = (EPI == kEpiLinear || EPI == kEpiActGrad) && a.has_extra && a.io_tma;
-    int loaded = 0;                 // extra tiles asked for (leader)
-    int ask_t = first_tile, ask_s = 0;  // the next one to ask for
+    // The extra inputs of the group's tiles arrive by TMA, in order; `ask` is the next tile to ask for.
+    const bool extra_tma = kElement && a.has_extra && a.io_tma;
+    int loaded = 0;
+    Walk ask(a, first_unit);
     auto ask_extra = [&]() {
-      for (; ask_t < total; ask_t += tile_step, ask_s = 0) {
-        const Tile tl = tile_at(a, ask_t);
-        if (ask_s < subs_of(tl)) {
-          load_extra(loaded++, tl, ask_s++);
-          return;
-        }
-      }
+      while (ask.live() && ask.tile().n * BN + wg * 64 >= a.N) ask.next();
+      if (!ask.live()) return;
+      const Tile tl = ask.tile();
+      mbar_expect_tx(bar_of(loaded), (uint32_t)kStageOut);
+      tma_load_2d(smem_u32(buf_of(loaded)), &tmX, tl.n * BN + wg * 64, (tl.m * CG + rank) * kBM, bar_of(loaded));
+      ++loaded;
+      ask.next();
     };
     if (extra_tma && leader) ask_extra();
 
@@ -588,36 +600,40 @@ __global__ void __launch_bounds__(kThreads, 1)
     float next_bias = 0.0f;
     int64_t next_target = -1;
     float4 next_rows = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    auto read_ahead = [&](int t) {
-      if (t >= total) return;
-      const Tile tl = tile_at(a, t);
+    auto read_ahead = [&](const Walk& w) {
+      if (!w.live()) return;
+      const Tile tl = w.tile();
       const int64_t row = (int64_t)(tl.m * CG + rank) * kBM + gt;
-      if (EPI == kEpiLinear || EPI == kEpiActGrad) {
-        const int col = tl.n * BN + wg * kHalf + gt;
-        next_bias = a.bias != nullptr && gt < kHalf && col < a.N
-                        ? Pack<T>::one(reinterpret_cast<const T*>(a.bias)[col])
-                        : 0.0f;
+      if (kElement) {
+        const int col = tl.n * BN + wg * 64 + gt;
+        next_bias = a.bias != nullptr && gt < 64 && col < a.N ? Pack<T>::one(reinterpret_cast<const T*>(a.bias)[col]) : 0.0f;
       }
       if (EPI == kEpiLse || EPI == kEpiProb) next_target = row < a.M ? __ldg(a.target + row) : -1;
       if (EPI == kEpiProb) next_rows = row < a.M ? __ldg(a.rows + row) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     };
-    read_ahead(first_tile);
+    Walk w(a, first_unit);
+    read_ahead(w);
+    if (kElement) {
+      if (gt < 64) bias[gt] = next_bias;
+      group_sync(wg);
+    }
+    float alpha = a.alpha;
+    if (a.alpha_dev != nullptr) alpha *= __ldg(a.alpha_dev);
+    float m = -INFINITY, l = 0.0f;  // of the run of tiles so far (kEpiLse)
 
-    for (int i = 0, t = first_tile; t < total; ++i, t += tile_step) {
-      const Tile tl = tile_at(a, t);
+    for (int i = 0; w.live(); ++i) {
+      const Tile tl = w.tile();
       const int acc = i & 1;
-      const uint32_t acc_addr = tmem + acc * BN + wg * kHalf + ((uint32_t)(quarter * 32) << 16);
+      const uint32_t acc_addr = tmem + acc * BN + wg * 64 + ((uint32_t)(quarter * 32) << 16);
       const int64_t m0 = (int64_t)(tl.m * CG + rank) * kBM;
-      const int n0 = tl.n * BN + wg * kHalf;
+      const int n0 = tl.n * BN + wg * 64;
       const int64_t row = m0 + gt;
-      const int64_t trow = next_target < 0 ? -1 : next_target - a.col0 - n0;
+      const int64_t tj = next_target < 0 ? -1 : next_target - a.col0 - n0;  // the target's column here, if it is one
       const GradRows gr{next_rows.x, next_rows.y, next_rows.z, next_rows.w};
-      if (EPI == kEpiLinear || EPI == kEpiActGrad) {
-        group_sync(wg);  // the last tile's values have been used
-        if (gt < kHalf) bias[gt] = next_bias;
-        group_sync(wg);
-      }
-      read_ahead(t + tile_step);
+      const bool some = n0 < a.N;  // the group's columns lie in the matrix
+      const bool first_of_run = w.r == 0, last_of_run = w.run_ends();
+      w.next();
+      read_ahead(w);
       if (!dead) {
         const bool ok = op_wait(smem_u32(&s_done[acc]), (uint32_t)((i >> 1) & 1), fail);
         if (!__all_sync(0xffffffffu, ok)) {
@@ -626,173 +642,195 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-
-      if (EPI == kEpiLse) {
-        float m = -INFINITY, l = 0.0f;
-        if (!dead && n0 < a.N) {
-#pragma unroll
-          for (int j = 0; j < kHalf / 64; ++j) {
-            float v[64];
-            tc_ld64(acc_addr + j * 64, v);
-            const int64_t tj = trow - j * 64;
-            if (__any_sync(0xffffffffu, (uint64_t)tj < 64u)) {
-#pragma unroll
-              for (int e = 0; e < 64; ++e) v[e] = e == tj ? -INFINITY : v[e];
-            }
-            if (n0 + j * 64 + 64 > a.N) {
-#pragma unroll
-              for (int e = 0; e < 64; ++e) v[e] = n0 + j * 64 + e < a.N ? v[e] : -INFINITY;
-            }
-            float top[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-            for (int e = 4; e < 64; ++e) top[e & 3] = fmaxf(top[e & 3], v[e]);
-            const float mn = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.c2);
-            const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing but masked logits so far
-            const uint64_t c2 = pair(a.c2, a.c2), nref = pair(-ref, -ref);
-            uint64_t sum[2] = {0, 0};
-#pragma unroll
-            for (int e = 0; e < 64; e += 2) {
-              const float2 x = split(fma2(pair(v[e], v[e + 1]), c2, nref));
-              sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(ex2(x.x), ex2(x.y)));
-            }
-            const float2 t2 = split(add2(sum[0], sum[1]));
-            l = fmaf(l, ex2(m - ref), t2.x + t2.y);
-            m = mn;
-          }
-        }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) arrive_leader<CG>(smem_u32(&s_free[acc]));
-        if (!dead && row < a.M) a.partial[(int64_t)(tl.n * 2 + wg) * a.M + row] = make_float2(m, l);
-        continue;
-      }
-
-      float alpha = a.alpha;
-      if (a.alpha_dev != nullptr) alpha *= __ldg(a.alpha_dev);
-      const int subs = subs_of(tl);
-      if (subs == 0) {
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) arrive_leader<CG>(smem_u32(&s_free[acc]));
-      }
-#pragma unroll 1
-      for (int s = 0; s < subs; ++s, ++c) {
-        unsigned char* buf = bufs + (c & 1) * kStageOut;
-        const int col = n0 + s * kSub;
-        if (extra_tma) {
-          // ask for the next tile's extra input: its buffer's last store has been read
-          if (leader && !dead) {
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-            ask_extra();
-          }
-          if (!dead) {
-            const bool ok = op_wait(smem_u32(&s_x[wg * 2 + (c & 1)]), (uint32_t)((c >> 1) & 1), fail);
-            if (!__all_sync(0xffffffffu, ok)) {
-              if (lane == 0) fail_with(fail, 5);
-              dead = true;
-            }
-          }
-        } else if (a.io_tma) {
-          if (leader) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          group_sync(wg);  // the buffer's last store has been read
-        } else if ((EPI == kEpiLinear || EPI == kEpiActGrad) && a.has_extra) {
-          if (!dead)
-            move_rows<T, true>(buf, reinterpret_cast<T*>(const_cast<void*>(a.extra)), m0, a.M, a.ld_extra, col,
-                               a.N, quarter * 32, lane);
-          __syncwarp();
-        }
-        if (!dead) {
-          if (EPI == kEpiSlab) {
-            float v[32];
-            tc_ld32(acc_addr + s * 32, v);
-            float4* at = reinterpret_cast<float4*>(buf + gt * 128);
-#pragma unroll
-            for (int w = 0; w < 8; ++w)
-              at[w ^ (gt & 7)] = make_float4(v[4 * w], v[4 * w + 1], v[4 * w + 2], v[4 * w + 3]);
-          } else {
-            float v[64];
-            tc_ld64(acc_addr + s * 64, v);
-            uint4* at = reinterpret_cast<uint4*>(buf + gt * 128);
-            if (EPI == kEpiProb) {
-              const uint64_t c2 = pair(a.c2, a.c2), nlse = pair(-gr.lse2, -gr.lse2), w = pair(gr.w, gr.w);
-#pragma unroll
-              for (int e = 0; e < 64; e += 2) {
-                const float2 x = split(fma2(pair(v[e], v[e + 1]), c2, nlse));
-                const float2 y = split(mul2(pair(ex2(x.x), ex2(x.y)), w));
-                v[e] = y.x;
-                v[e + 1] = y.y;
-              }
-              const int64_t tj = trow - s * 64;
-              if (__any_sync(0xffffffffu, gr.w == 0.0f || (uint64_t)tj < 64u)) {
-#pragma unroll
-                for (int e = 0; e < 64; ++e)  // a row that takes no part gives zeros, whatever its logits
-                  v[e] = gr.w == 0.0f ? 0.0f : e == tj ? gr.at_target : v[e];
-              }
-            }
-#pragma unroll
-            for (int w = 0; w < 8; ++w) {
-              const int slot = w ^ (gt & 7);
-              float* o = v + w * 8;
-              if (EPI == kEpiLinear || EPI == kEpiActGrad) {
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (EPI == kEpiActGrad || a.has_extra) x = at[slot];
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
-                const uint64_t al = pair(alpha, alpha);
-                const ulonglong2* bp = reinterpret_cast<const ulonglong2*>(bias + s * 64 + w * 8);
-                const ulonglong2 b01 = bp[0], b23 = bp[1];
-                const uint64_t b[4] = {b01.x, b01.y, b23.x, b23.y};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const uint64_t z = fma2(pair(o[2 * e], o[2 * e + 1]), al, b[e]);
-                  if (EPI == kEpiActGrad) {
-                    const float2 f = act_slope<ACT>(z), g = Pack<T>::get(xs[e]);
-                    o[2 * e] = g.x * f.x;
-                    o[2 * e + 1] = g.y * f.y;
-                  } else {
-                    const float2 f = act_of<ACT>(z);
-                    o[2 * e] = f.x;
-                    o[2 * e + 1] = f.y;
-                    if (a.has_extra) {
-                      const float2 r = Pack<T>::get(xs[e]);
-                      o[2 * e] += r.x;
-                      o[2 * e + 1] += r.y;
-                    }
-                  }
-                }
-              }
-              at[slot] = make_uint4(Pack<T>::two(o[0], o[1]), Pack<T>::two(o[2], o[3]), Pack<T>::two(o[4], o[5]),
-                                    Pack<T>::two(o[6], o[7]));
-            }
-          }
-        }
-        if (s + 1 == subs) {  // the accumulator has been read
+      // The share is read 32 columns at a time (64 at once spilled registers), the accumulator free after
+      // the second read.
+      auto read_half = [&](int h, float (&v)[32]) {
+        if (!dead && some) tc_ld32(acc_addr + h * 32, v);
+        if (h == 1) {
           asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
           __syncwarp();
           if (lane == 0) arrive_leader<CG>(smem_u32(&s_free[acc]));
         }
-        if (EPI == kEpiSlab || a.io_tma) {
+      };
+
+      if (EPI == kEpiLse) {
+        if (first_of_run) m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[32];
+          read_half(h, v);
+          if (dead || !some) continue;
+          const int64_t th = tj - h * 32;
+          if (__any_sync(0xffffffffu, (uint64_t)th < 32u)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = e == th ? -INFINITY : v[e];
+          }
+          if (n0 + h * 32 + 32 > a.N) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = n0 + h * 32 + e < a.N ? v[e] : -INFINITY;
+          }
+          float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+          for (int e = 4; e < 32; ++e) top[e & 3] = fmaxf(top[e & 3], v[e]);
+          const float mn = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.c2);
+          const float ref = mn == -INFINITY ? 0.0f : mn;  // nothing but masked logits so far
+          const uint64_t c2 = pair(a.c2, a.c2), nref = pair(-ref, -ref);
+          uint64_t sum[2] = {0, 0};
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 x = split(fma2(pair(v[e], v[e + 1]), c2, nref));
+            sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pair(ex2(x.x), ex2(x.y)));
+          }
+          const float2 t2 = split(add2(sum[0], sum[1]));
+          l = fmaf(l, ex2(m - ref), t2.x + t2.y);
+          m = mn;
+        }
+        if (last_of_run && !dead && row < a.M)
+          a.partial[(int64_t)(tl.n / a.run * kGroups + wg) * a.M + row] = make_float2(m, l);
+        continue;
+      }
+      // The next tile's bias, beside this one's; the group's barriers below publish it.
+      const float* tile_bias = bias + (i & 1) * BN;
+      if (kElement && gt < 64) bias[((i + 1) & 1) * BN + gt] = next_bias;
+      if (!some) {
+        float v[32];
+        read_half(1, v);
+        if (kElement) group_sync(wg);
+        continue;
+      }
+
+      if (EPI == kEpiSlab) {  // 32 columns of fp32 to a staging row, twice
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float v[32];
+          read_half(h, v);
+          if (n0 + h * 32 >= a.N) break;  // only past the first half
+          if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          group_sync(wg);  // the buffer's last store has been read
+          if (!dead) {
+            float4* at = reinterpret_cast<float4*>(bufs + gt * 128);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              at[k ^ (gt & 7)] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
+          }
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           group_sync(wg);
           if (leader && !dead && !*fail && m0 < a.M) {  // a pair's second half may lie past the last row
-            const int y = EPI == kEpiSlab ? tl.split * a.slab_rows + (int)m0 : (int)m0;
-            if (EPI == kEpiSlab && a.slab_add)
-              tma_add_2d(&tmO, smem_u32(buf), col, y);
+            const int y = tl.split * a.slab_rows + (int)m0;
+            if (a.slab_add)
+              tma_add_2d(&tmO, smem_u32(bufs), n0 + h * 32, y);
             else
-              tma_store_2d(&tmO, smem_u32(buf), col, y);
+              tma_store_2d(&tmO, smem_u32(bufs), n0 + h * 32, y);
           }
-        } else {
-          __syncwarp();
-          if (!dead)
-            move_rows<T, false>(buf, reinterpret_cast<T*>(a.out), m0, a.M, a.ld_out, col, a.N, quarter * 32, lane);
-          __syncwarp();
+        }
+        continue;
+      }
+
+      unsigned char* buf = buf_of(c);
+      if (extra_tma) {
+        if (S::kBufs == 2 && leader && !dead) {  // the next tile's, into the buffer whose store has been read
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          ask_extra();
+        }
+        if (!dead) {
+          const bool ok = op_wait(bar_of(c), parity_of(c), fail);
+          if (!__all_sync(0xffffffffu, ok)) {
+            if (lane == 0) fail_with(fail, 5);
+            dead = true;
+          }
+        }
+      } else if (a.io_tma) {
+        if (leader) {
+          if (S::kBufs == 2)
+            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+          else
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        }
+        group_sync(wg);  // the buffer's last store has been read
+      } else if (kElement && a.has_extra) {
+        if (!dead)
+          move_rows<T, true>(buf, reinterpret_cast<T*>(const_cast<void*>(a.extra)), m0, a.M, a.ld_extra, n0, a.N, quarter * 32,
+                             lane);
+        __syncwarp();
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float v[32];
+        read_half(h, v);
+        if (dead) continue;
+        uint4* at = reinterpret_cast<uint4*>(buf + gt * 128);
+        if (EPI == kEpiProb) {
+          const uint64_t c2 = pair(a.c2, a.c2), nlse = pair(-gr.lse2, -gr.lse2), wt = pair(gr.w, gr.w);
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 x = split(fma2(pair(v[e], v[e + 1]), c2, nlse));
+            const float2 y = split(mul2(pair(ex2(x.x), ex2(x.y)), wt));
+            v[e] = y.x;
+            v[e + 1] = y.y;
+          }
+          const int64_t th = tj - h * 32;
+          if (__any_sync(0xffffffffu, gr.w == 0.0f || (uint64_t)th < 32u)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)  // a row that takes no part gives zeros, whatever its logits
+              v[e] = gr.w == 0.0f ? 0.0f : e == th ? gr.at_target : v[e];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int slot = (h * 4 + k) ^ (gt & 7);
+          float* o = v + k * 8;
+          if (kElement) {
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (EPI == kEpiActGrad || a.has_extra) x = at[slot];
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+            const uint64_t al = pair(alpha, alpha);
+            const ulonglong2* bp = reinterpret_cast<const ulonglong2*>(tile_bias + h * 32 + k * 8);
+            const ulonglong2 b01 = bp[0], b23 = bp[1];
+            const uint64_t b[4] = {b01.x, b01.y, b23.x, b23.y};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint64_t z = fma2(pair(o[2 * e], o[2 * e + 1]), al, b[e]);
+              if (EPI == kEpiActGrad) {
+                const float2 f = act_slope<ACT>(z), g = Pack<T>::get(xs[e]);
+                o[2 * e] = g.x * f.x;
+                o[2 * e + 1] = g.y * f.y;
+              } else {
+                const float2 f = act_of<ACT>(z);
+                o[2 * e] = f.x;
+                o[2 * e + 1] = f.y;
+                if (a.has_extra) {
+                  const float2 r = Pack<T>::get(xs[e]);
+                  o[2 * e] += r.x;
+                  o[2 * e + 1] += r.y;
+                }
+              }
+            }
+          }
+          at[slot] = make_uint4(Pack<T>::two(o[0], o[1]), Pack<T>::two(o[2], o[3]), Pack<T>::two(o[4], o[5]),
+                                Pack<T>::two(o[6], o[7]));
         }
       }
+      if (a.io_tma) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        group_sync(wg);
+        if (leader && !dead && !*fail) {
+          if (m0 < a.M) tma_store_2d(&tmO, smem_u32(buf), n0, (int)m0);  // a pair's second half may lie past the last row
+          if (S::kBufs == 1 && extra_tma) {
+            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            ask_extra();
+          }
+        }
+      } else {
+        __syncwarp();
+        if (!dead) move_rows<T, false>(buf, reinterpret_cast<T*>(a.out), m0, a.M, a.ld_out, n0, a.N, quarter * 32, lane);
+        group_sync(wg);
+      }
+      ++c;
     }
     if (leader) {
       // after a failure: extra inputs in flight land before the shared memory goes away
-      if (*fail && loaded > 0)
-        for (int k = (loaded > 2 ? loaded - 2 : 0); k < loaded; ++k)
-          mbar_wait(smem_u32(&s_x[wg * 2 + (k & 1)]), (uint32_t)((k >> 1) & 1));
+      if (S::kBufs > 0 && *fail && loaded > 0)
+        for (int k = (loaded > S::kBufs ? loaded - S::kBufs : 0); k < loaded; ++k) mbar_wait(bar_of(k), parity_of(k));
       asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1062,10 +1100,13 @@ void launch_gemm(GemmArgs& a, const CUtensorMap& ta, const CUtensorMap& tb, cons
     RBQ_CUDA(cudaFuncSetAttribute(gemm_kernel<EPI, T, CG, ACT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kBytes));
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
-  const int64_t total = (int64_t)a.tiles_m * a.tiles_n * a.splits;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(CG * std::min<int64_t>(total, sm_count() / CG)));
-  cfg.blockDim = dim3(kThreads);
+  const int step = std::min(a.units, sm_count() / CG);
+  a.step_fast = step % a.len_fast;
+  a.step_slow = step / a.len_fast % a.len_slow;
+  a.step_split = step / a.len_fast / a.len_slow;
+  cfg.gridDim = dim3((unsigned)(CG * step));
+  cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = s;
   cudaLaunchAttribute attr{};
@@ -1095,6 +1136,10 @@ void gemm(GemmArgs a, Matrix A, bool a_mn, Matrix B, bool b_mn, int cg, const CU
   a.tiles_n = (int)tn;
   a.kblocks = (int)kb;
   a.m_fast = tm <= tn;  // the operand with fewer tiles stays in L2 while the other streams by once
+  const int runs = (int)ceil_div(tn, a.run);
+  a.len_fast = a.m_fast ? (int)tm : runs;
+  a.len_slow = a.m_fast ? runs : (int)tm;
+  a.units = a.len_fast * a.len_slow * a.splits;
   const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   a.idesc = (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
             ((uint32_t)(128 * cg >> 3) << 17) | ((uint32_t)(kBM * cg >> 4) << 24);
@@ -1303,10 +1348,14 @@ void loss_forward(const T* q, const T* bank, const int64_t* target, int64_t n, i
 {
   const Matrix Q = addressable(q, n, d, ws, run, s), B = addressable(bank, v, d, ws, run, s);
   const int cg = group_size(n, v);
-  const int64_t tiles = 2 * ceil_div(v, 128 * cg);
+  // Runs of up to 16 tiles write one partial row each, but leave enough of them to even out over the SMs.
+  const int64_t tiles_m = ceil_div(n, kBM * cg), tiles_n = ceil_div(v, 128 * cg);
+  const int length = (int)std::max<int64_t>(1, std::min<int64_t>(16, tiles_m * tiles_n / (8 * (sm_count() / cg))));
+  const int64_t tiles = 2 * cg * ceil_div(tiles_n, length);
   float2* partial = ws.take<float2>(tiles * n);
   if (!run) return;
   GemmArgs a;
+  a.run = length;
   a.c2 = scale * kLog2e;
   a.target = target;
   a.partial = partial;
