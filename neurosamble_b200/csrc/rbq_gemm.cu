@@ -88,12 +88,12 @@ struct GemmArgs {
   const float4* rows = nullptr;      // [M] GradRows
 };
 
-// What the gradient of a row's logits needs: lse in base 2, the row's weight w = g_i / max|g| times
-// kGradScale (0: the row takes no part) and the value at the target, expm1(-loss) * w.
+// What the gradient of a row's logits needs: lse in base 2, the row's weight w = g_i / max|g| times a
+// scale of at most kGradScale (0: the row takes no part) and the value at the target, expm1(-loss) * w.
 //   d loss_i / d s_ij = p_ij - [j = t_i],   p_ij - 1 = expm1(-loss_i) at the target
 // The gradient of the logits is rounded to the operands' 16 bits, since it is the operand of the two
 // products that follow.  |p - 1| <= 1, so with |w| <= 2^14 nothing overflows in fp16 and
-// probabilities down to 2^-28 keep all 11 bits; the factor max|g| * scale / 2^14 returns in fp32.
+// probabilities down to 2^-27 keep all 11 bits; the factor max|g| * scale / w returns in fp32.
 struct GradRows {
   float lse2, w, at_target, unused;
 };
@@ -252,37 +252,6 @@ struct Pack<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 from(float f) { return __float2bfloat16_rn(f); }
 };
 
-// Two fp32 values in a register pair: one instruction for both.
-__device__ __forceinline__ uint64_t pair(float a, float b)
-{
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ float2 split(uint64_t v)
-{
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
-{
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
-{
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
-{
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
 __device__ __forceinline__ float max_nan(float a, float b)
 {
   float r;
@@ -1003,11 +972,20 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(const float2* __restric
   }
 }
 
-// Largest finite |g| of the rows that take part, and the factor that the gradients return by.
+// Largest |g| of the rows that take part, and the scale of the logits' gradient: kGradScale times one
+// of eight factors in (1/2, 1].  A row's gradient is mostly its target's entry, so its rounding does
+// not average out the way the others' do; rows that have learnt about as much have entries of about
+// one mantissa, and a factor that moves it up towards the next power of two halves the rounding.  The
+// factor is the one with the least squared rounding of the target's entries over the first rows.
+constexpr int kScaleTries = 8;
+constexpr int64_t kScaleRows = 16384;
+template <typename T>
 __global__ void __launch_bounds__(1024) grad_top_kernel(const float* __restrict__ g, const int64_t* __restrict__ target,
-                                                        int64_t n, int64_t v, float scale, float* __restrict__ out)
+                                                        const float* __restrict__ loss, int64_t n, int64_t v, float scale,
+                                                        float* __restrict__ out)
 {
-  __shared__ float s_top[32];
+  __shared__ float s_red[32][kScaleTries];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float top = 0.0f;
   for (int64_t i = threadIdx.x; i < n; i += 1024) {
     const int64_t t = target[i];
@@ -1015,12 +993,39 @@ __global__ void __launch_bounds__(1024) grad_top_kernel(const float* __restrict_
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if ((threadIdx.x & 31) == 0) s_top[threadIdx.x >> 5] = top;
+  if (lane == 0) s_red[warp][0] = top;
+  __syncthreads();
+  for (int w = 0; w < 32; ++w) top = fmaxf(top, s_red[w][0]);
+  __syncthreads();
+  float err[kScaleTries] = {};
+  for (int64_t i = threadIdx.x; i < n && i < kScaleRows; i += 1024) {
+    const int64_t t = target[i];
+    if (t < 0 || t >= v || g[i] == 0.0f) continue;
+    const float at = expm1f(-loss[i]) * (g[i] / top * kGradScale);
+#pragma unroll
+    for (int k = 0; k < kScaleTries; ++k) {
+      const float f = 1.0f - (float)k / (2 * kScaleTries), x = at * f;
+      const float e = (Pack<T>::one(Pack<T>::from(x)) - x) / (f * kGradScale);
+      err[k] = fmaf(e, e, err[k]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kScaleTries; ++k) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) err[k] += __shfl_xor_sync(0xffffffffu, err[k], o);
+    if (lane == 0) s_red[warp][k] = err[k];
+  }
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < 32; ++w) top = fmaxf(top, s_top[w]);
+    float least = INFINITY, factor = 1.0f;
+    for (int k = 0; k < kScaleTries; ++k) {
+      float sum = 0.0f;
+      for (int w = 0; w < 32; ++w) sum += s_red[w][k];
+      if (sum < least) least = sum, factor = 1.0f - (float)k / (2 * kScaleTries);
+    }
     out[0] = top;
-    out[1] = top * scale / kGradScale;
+    out[1] = top * scale / (kGradScale * factor);
+    out[2] = kGradScale * factor;
   }
 }
 __global__ void grad_rows_kernel(const float* __restrict__ g, const int64_t* __restrict__ target,
@@ -1030,9 +1035,8 @@ __global__ void grad_rows_kernel(const float* __restrict__ g, const int64_t* __r
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= n) return;
   const int64_t t = target[i];
-  const float big = top[0];
   float w = 0.0f;
-  if (t >= 0 && t < v && g[i] != 0.0f) w = g[i] / big * kGradScale;
+  if (t >= 0 && t < v && g[i] != 0.0f) w = g[i] / top[0] * top[2];
   rows[i] = make_float4(lse[i] * kLog2e, w, w == 0.0f ? 0.0f : expm1f(-loss[i]) * w, 0.0f);
 }
 
@@ -1365,9 +1369,11 @@ void loss_forward(const T* q, const T* bank, const int64_t* target, int64_t n, i
   RBQ_LAUNCHED();
 }
 
-// The gradient of the logits exists one piece of the bank at a time: 16-bit values [n, piece] small
-// enough to stay in L2 (kPieceBytes) between the product that makes them and the two that read them.
-constexpr int64_t kPieceBytes = 64ll << 20;
+// The gradient of the logits exists one piece of the bank at a time, 16-bit values [n, piece] of at most
+// kPieceBytes.  Pieces that stay in L2 (64 MB) cost more in short kernels than the traffic they save:
+// 8,192 queries x 200,000 rows x 256, the three products of the backward pass: 3.4 ms in pieces of 64 MB,
+// 3.1 of 128, 2.75 of 256, 2.66 of 512, 2.54 of 1,024.
+constexpr int64_t kPieceBytes = 512ll << 20;
 int64_t piece_columns(int64_t n, int64_t v)
 {
   const int64_t most = std::max<int64_t>(256, kPieceBytes / (2 * n) / 256 * 256);
@@ -1380,14 +1386,14 @@ void loss_backward(const float* g, const T* q, const T* bank, const int64_t* tar
 {
   const Matrix Q = addressable(q, n, d, ws, run, s), B = addressable(bank, v, d, ws, run, s);
   const int64_t piece = std::min(piece_columns(n, v), round_up(v, 8));
-  float* top = ws.take<float>(2);
+  float* top = ws.take<float>(3);
   float4* rows = ws.take<float4>(n);
   T* prob = ws.take<T>(n * piece);
   const SlabPlan pq = plan_slabs(n, d, piece), pb = plan_slabs(piece, d, n);
   float* slabs_q = ws.take<float>(pq.floats());
   float* slabs_b = ws.take<float>(pb.floats());
   if (!run) return;
-  grad_top_kernel<<<1, 1024, 0, s>>>(g, target, n, v, scale, top);
+  grad_top_kernel<T><<<1, 1024, 0, s>>>(g, target, loss, n, v, scale, top);
   RBQ_LAUNCHED();
   grad_rows_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(g, target, loss, lse, n, v, top, rows);
   RBQ_LAUNCHED();

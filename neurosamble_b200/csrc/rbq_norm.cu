@@ -50,6 +50,36 @@ __device__ __forceinline__ void load_vec(const T* p, float (&v)[VEC])
   for (int i = 0; i < VEC; ++i) v[i] = to_f(x.e[i]);
 }
 template <typename T, int VEC>
+__device__ __forceinline__ void unpack(const Vec<T, VEC>& x, float (&v)[VEC])
+{
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = to_f(x.e[i]);
+}
+// Keeps x packed: the compiler would unpack loop-invariant values once and hold twice the registers.
+template <typename T, int VEC>
+__device__ __forceinline__ void keep_packed(Vec<T, VEC>& x)
+{
+  static_assert(sizeof(Vec<T, VEC>) % 4 == 0 || VEC == 1, "whole registers");
+  if (sizeof(T) == 2 && VEC % 2 == 0) {
+#pragma unroll
+    for (int k = 0; k < VEC / 2; ++k) asm volatile("" : "+r"(reinterpret_cast<uint32_t*>(&x)[k]));
+  }
+}
+// A thread's pieces of row r of a [rows, d] matrix, as they lie in memory; zeros outside.
+template <typename T, int VEC, int CH, int TPR>
+__device__ __forceinline__ void fetch(const T* p, int64_t r, int64_t rows, int d, int i, Vec<T, VEC> (&x)[CH])
+{
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    const int col = (c * TPR + i) * VEC;
+    if (r < rows && col < d)
+      x[c] = *reinterpret_cast<const Vec<T, VEC>*>(p + r * d + col);
+    else
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) x[c].e[e] = from_f<T>(0.0f);
+  }
+}
+template <typename T, int VEC>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[VEC])
 {
   Vec<T, VEC> x;
@@ -78,8 +108,16 @@ __device__ __forceinline__ float row_sum(float v, float* s_red)
   return t;
 }
 
-// One row per TPR threads; thread i of a row holds CH pieces of VEC values, piece c at column
-// (c * TPR + i) * VEC.
+// sum / d, rounded as a division would: one correction of the product with 1 / d.
+__device__ __forceinline__ float over(float sum, float d, float inv_d)
+{
+  const float q = sum * inv_d;
+  return fmaf(fmaf(-q, d, sum), inv_d, q);
+}
+
+// TPR threads to a row; thread i of a row holds CH pieces of VEC values, piece c at column
+// (c * TPR + i) * VEC.  Few threads with several pieces each need fewer shuffles and scalar steps per row
+// than a warp with one piece each.
 template <typename T, typename P, int VEC, int CH, int TPR>
 __global__ void __launch_bounds__(kNormThreads)
     norm_kernel(const T* __restrict__ x, const P* __restrict__ w, const P* __restrict__ b, T* __restrict__ y,
@@ -87,8 +125,19 @@ __global__ void __launch_bounds__(kNormThreads)
 {
   __shared__ float s_red[kNormThreads / 32];
   constexpr int kRows = kNormThreads / TPR;
+  // The thread's parameters stay in registers, as they lie in memory.  (From shared memory they took
+  // most of the load-store unit's cycles, and as fp32 registers half the warps.)
+  constexpr bool kHold = CH * VEC <= 16;
   const int i = threadIdx.x % TPR;
+  const float fd = (float)d, inv_d = 1.0f / fd;
   const int64_t step = (int64_t)gridDim.x * kRows;
+  Vec<T, VEC> next[CH];  // the thread's next row is on its way while this one is worked on
+  fetch<T, VEC, CH, TPR>(x, (int64_t)blockIdx.x * kRows + threadIdx.x / TPR, rows, d, i, next);
+  Vec<P, VEC> wv[CH], bv[CH];
+  if (kHold) {
+    fetch<P, VEC, CH, TPR>(w, 0, 1, d, i, wv);
+    fetch<P, VEC, CH, TPR>(b, 0, 1, d, i, bv);
+  }
   // whole warps run every round, so that the shuffles see all lanes
   for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += step) {
     const int64_t r = r0 + threadIdx.x / TPR;
@@ -97,17 +146,12 @@ __global__ void __launch_bounds__(kNormThreads)
     float sum = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
-      const int col = (c * TPR + i) * VEC;
-      if (live && col < d) {
-        load_vec<T, VEC>(x + r * d + col, v[c]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[c][e] = 0.0f;
-      }
+      unpack<T, VEC>(next[c], v[c]);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) sum += v[c][e];
     }
-    const float mean = row_sum<TPR>(sum, s_red) / (float)d;
+    fetch<T, VEC, CH, TPR>(x, r + step, rows, d, i, next);
+    const float mean = over(row_sum<TPR>(sum, s_red), fd, inv_d);
     float sq = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -119,17 +163,24 @@ __global__ void __launch_bounds__(kNormThreads)
         }
       }
     }
-    const float rstd = 1.0f / sqrtf(row_sum<TPR>(sq, s_red) / (float)d + eps);
+    const float rstd = rsqrtf(over(row_sum<TPR>(sq, s_red), fd, inv_d) + eps);
     if (live) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const int col = (c * TPR + i) * VEC;
         if (col < d) {
-          float wv[VEC], bv[VEC];
-          load_vec<P, VEC>(w + col, wv);
-          load_vec<P, VEC>(b + col, bv);
+          float wc[VEC], bc[VEC];
+          if (kHold) {
+            keep_packed(wv[c]);
+            keep_packed(bv[c]);
+            unpack<P, VEC>(wv[c], wc);
+            unpack<P, VEC>(bv[c], bc);
+          } else {
+            load_vec<P, VEC>(w + col, wc);
+            load_vec<P, VEC>(b + col, bc);
+          }
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) v[c][e] = fmaf(v[c][e] * rstd, wv[e], bv[e]);
+          for (int e = 0; e < VEC; ++e) v[c][e] = fmaf(v[c][e] * rstd, wc[e], bc[e]);
           store_vec<T, VEC>(y + r * d + col, v[c]);
         }
       }
@@ -151,41 +202,63 @@ __global__ void __launch_bounds__(kNormThreads)
   extern __shared__ float s_part[];  // [2][d], rows shared by TPR < kNormThreads threads only
   __shared__ float s_red[kNormThreads / 32];
   constexpr int kRows = kNormThreads / TPR;
+  constexpr bool kHold = CH * VEC <= 16;
   const int i = threadIdx.x % TPR, group = threadIdx.x / TPR;
+  const float fd = (float)d, inv_d = 1.0f / fd;
   const int64_t step = (int64_t)gridDim.x * kRows;
   float dw[CH][VEC], db[CH][VEC];
 #pragma unroll
   for (int c = 0; c < CH; ++c)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) dw[c][e] = db[c][e] = 0.0f;
+  Vec<T, VEC> next_x[CH], next_g[CH];  // the thread's next row is on its way while this one is worked on
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto fetch_row = [&](int64_t r) {
+    fetch<T, VEC, CH, TPR>(x, r, rows, d, i, next_x);
+    fetch<T, VEC, CH, TPR>(g, r, rows, d, i, next_g);
+    next_mean = r < rows ? __ldg(mean_in + r) : 0.0f;
+    next_rstd = r < rows ? __ldg(rstd_in + r) : 0.0f;
+  };
+  fetch_row((int64_t)blockIdx.x * kRows + group);
+  Vec<P, VEC> wv[CH];
+  if (kHold) fetch<P, VEC, CH, TPR>(w, 0, 1, d, i, wv);
   for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += step) {
     const int64_t r = r0 + group;
     const bool live = r < rows;
-    const float mean = live ? __ldg(mean_in + r) : 0.0f, rstd = live ? __ldg(rstd_in + r) : 0.0f;
+    const float mean = next_mean, rstd = next_rstd;
     float xh[CH][VEC], gw[CH][VEC];
     float a = 0.0f, b = 0.0f;
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
+      unpack<T, VEC>(next_x[c], xh[c]);
+      unpack<T, VEC>(next_g[c], gw[c]);
+    }
+    fetch_row(r + step);
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
       const int col = (c * TPR + i) * VEC;
       if (live && col < d) {
-        load_vec<T, VEC>(x + r * d + col, xh[c]);
-        load_vec<T, VEC>(g + r * d + col, gw[c]);
-        float wv[VEC];
-        load_vec<P, VEC>(w + col, wv);
+        float wc[VEC];
+        if (kHold) {
+          keep_packed(wv[c]);
+          unpack<P, VEC>(wv[c], wc);
+        } else {
+          load_vec<P, VEC>(w + col, wc);
+        }
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
           xh[c][e] = (xh[c][e] - mean) * rstd;
           dw[c][e] = fmaf(gw[c][e], xh[c][e], dw[c][e]);
           db[c][e] += gw[c][e];
-          gw[c][e] *= wv[e];
+          gw[c][e] *= wc[e];
           a += gw[c][e];
           b = fmaf(gw[c][e], xh[c][e], b);
         }
       }
     }
     if (dx == nullptr) continue;
-    a = row_sum<TPR>(a, s_red) / (float)d;
-    b = row_sum<TPR>(b, s_red) / (float)d;
+    a = over(row_sum<TPR>(a, s_red), fd, inv_d);
+    b = over(row_sum<TPR>(b, s_red), fd, inv_d);
     if (live) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
@@ -201,6 +274,18 @@ __global__ void __launch_bounds__(kNormThreads)
   }
   if (part == nullptr) return;
   float* out = part + (int64_t)blockIdx.x * 2 * d;
+  if (TPR < 32) {  // the warp's rows
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+#pragma unroll
+        for (int o = TPR; o < 32; o <<= 1) {
+          dw[c][e] += __shfl_xor_sync(0xffffffffu, dw[c][e], o);
+          db[c][e] += __shfl_xor_sync(0xffffffffu, db[c][e], o);
+        }
+      }
+  }
   if (TPR == kNormThreads) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -215,8 +300,8 @@ __global__ void __launch_bounds__(kNormThreads)
     }
     return;
   }
-  for (int k = 0; k < kRows; ++k) {  // the groups in their order
-    if (group == k) {
+  for (int k = 0; k < kNormThreads / 32; ++k) {  // the warps in their order
+    if ((int)(threadIdx.x >> 5) == k && (threadIdx.x & 31) < TPR) {
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         const int col = (c * TPR + i) * VEC;
@@ -250,7 +335,7 @@ __global__ void __launch_bounds__(kNormThreads)
       const float c = to_f(xr[j]) - mean;
       sq = fmaf(c, c, sq);
     }
-    const float rstd = 1.0f / sqrtf(row_sum<kNormThreads>(sq, s_red) / (float)d + eps);
+    const float rstd = rsqrtf(row_sum<kNormThreads>(sq, s_red) / (float)d + eps);
     for (int j = threadIdx.x; j < d; j += kNormThreads)
       y[r * d + j] = from_f<T>(fmaf((to_f(xr[j]) - mean) * rstd, to_f(w[j]), to_f(b[j])));
     if (threadIdx.x == 0) {
@@ -301,23 +386,24 @@ __global__ void __launch_bounds__(kNormThreads)
   part[(int64_t)blockIdx.y * 2 * d + d + c] = db;
 }
 
-// dw and db from the blocks' shares, in the blocks' order within each of 8 interleaved runs.
+// dw and db from the blocks' shares: 32 interleaved runs of blocks, then the runs in their order.
 template <typename P>
-__global__ void norm_parts_kernel(const float* __restrict__ part, int parts, int d, P* __restrict__ dw, P* __restrict__ db)
+__global__ void __launch_bounds__(1024) norm_parts_kernel(const float* __restrict__ part, int parts, int d, P* __restrict__ dw,
+                                                          P* __restrict__ db)
 {
-  __shared__ float s_sum[8][33];
+  __shared__ float s_sum[32][33];
   const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float t = 0.0f;
   if (c < 2 * (int64_t)d) {
 #pragma unroll 4
-    for (int p = run; p < parts; p += 8) t += part[(int64_t)p * 2 * d + c];
+    for (int p = run; p < parts; p += 32) t += part[(int64_t)p * 2 * d + c];
   }
   s_sum[run][lane] = t;
   __syncthreads();
   if (run == 0 && c < 2 * (int64_t)d) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) t += s_sum[k][lane];
+    for (int k = 1; k < 32; ++k) t += s_sum[k][lane];
     if (c < d) {
       if (dw != nullptr) dw[c] = from_f<P>(t);
     } else if (db != nullptr) {
@@ -342,49 +428,71 @@ int sms()
 struct Plan {
   int vec, tpr, ch;
 };
-Plan plan_of(int d, int esize, bool vector)
+Plan plan_of(int d, int esize, bool vector, bool backward)
 {
   const int vec = vector ? 16 / esize : 1;
   const int loads = (d + vec - 1) / vec;
   if (vector) {
     if (loads <= 8) return {vec, 8, 1};
-    if (loads <= 32) return {vec, 32, 1};
-    if (loads <= 64) return {vec, 32, 2};
+    if (loads <= 16) return {vec, 8, 2};
+    // the backward pass holds five values per column: half the pieces, for as many warps on an SM
+    if (loads <= 32) return backward ? Plan{vec, 32, 1} : Plan{vec, 16, 2};
+    if (loads <= 64) return Plan{vec, 32, 2};
     if (loads <= 128) return {vec, 32, 4};
     if (loads <= 4 * kNormThreads) return {vec, kNormThreads, 4};
   } else {
+    if (loads <= 32) return {vec, 8, 4};
     if (loads <= 256) return {vec, 32, 8};
-    if (loads <= 1024) return {vec, 32, 32};
+    if (loads <= 4 * kNormThreads) return {vec, kNormThreads, 4};
     if (loads <= 32 * kNormThreads) return {vec, kNormThreads, 32};
   }
   return {vec, 0, 0};
 }
 
-int grad_blocks(const Plan& p, int64_t rows)
+// Blocks of a kernel that runs over its rows in rounds: those that an SM holds at once (kMostBlocks at
+// most), so that no block waits for another's end, and no more than there are rows for.
+constexpr int kMostBlocks = 8;
+template <typename T, typename P, int VEC, int CH, int TPR, int PASS>
+struct Kernel;  // names a kernel
+template <typename Name, typename K>
+int blocks_for(K kernel, size_t smem, int64_t rows, int tpr)
 {
-  const int64_t per = p.tpr ? kNormThreads / p.tpr : 1;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, per), (int64_t)sms() * 4));
+  static std::atomic<int> per_sm{0};  // one for every Name
+  int n = per_sm.load();
+  if (n == 0) {
+    RBQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kNormThreads, smem));
+    n = std::max(1, std::min(n, kMostBlocks));
+    per_sm.store(n);
+  }
+  const int64_t per = kNormThreads / tpr;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, per), (int64_t)sms() * n));
 }
 
 template <typename T, typename P>
 void run_forward(const T* x, const P* w, const P* b, T* y, float* mean, float* rstd, int64_t rows, int d, float eps,
                  bool vector, cudaStream_t s)
 {
-  const Plan p = plan_of(d, (int)sizeof(T), vector);
+  const Plan p = plan_of(d, (int)sizeof(T), vector, false);
   constexpr int V = 16 / (int)sizeof(T);
-  const int64_t per = p.tpr ? kNormThreads / p.tpr : 1;
-  const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(rows, per), (int64_t)sms() * 32);
-#define RBQ_NORM(VEC, CH, TPR) norm_kernel<T, P, VEC, CH, TPR><<<grid, kNormThreads, 0, s>>>(x, w, b, y, mean, rstd, rows, d, eps)
+#define RBQ_NORM(VEC, CH, TPR)                                                                                      \
+  norm_kernel<T, P, VEC, CH, TPR>                                                                                   \
+      <<<blocks_for<Kernel<T, P, VEC, CH, TPR, 0>>(norm_kernel<T, P, VEC, CH, TPR>, 0, rows, TPR), kNormThreads, 0, \
+         s>>>(x, w, b, y, mean, rstd, rows, d, eps)
   if (p.tpr == 0)
-    norm_wide_kernel<T, P><<<grid, kNormThreads, 0, s>>>(x, w, b, y, mean, rstd, rows, d, eps);
+    norm_wide_kernel<T, P><<<(unsigned)std::min<int64_t>(rows, (int64_t)sms() * kMostBlocks), kNormThreads, 0, s>>>(
+        x, w, b, y, mean, rstd, rows, d, eps);
+  else if (p.vec == 1 && p.tpr == 8)
+    RBQ_NORM(1, 4, 8);
   else if (p.vec == 1 && p.tpr == 32)
-    p.ch == 8 ? RBQ_NORM(1, 8, 32) : RBQ_NORM(1, 32, 32);
+    RBQ_NORM(1, 8, 32);
   else if (p.vec == 1)
-    RBQ_NORM(1, 32, kNormThreads);
+    p.ch == 4 ? RBQ_NORM(1, 4, kNormThreads) : RBQ_NORM(1, 32, kNormThreads);
   else if (p.tpr == 8)
-    RBQ_NORM(V, 1, 8);
+    p.ch == 1 ? RBQ_NORM(V, 1, 8) : RBQ_NORM(V, 2, 8);
+  else if (p.tpr == 16)
+    RBQ_NORM(V, 2, 16);
   else if (p.tpr == 32)
-    p.ch == 1 ? RBQ_NORM(V, 1, 32) : p.ch == 2 ? RBQ_NORM(V, 2, 32) : RBQ_NORM(V, 4, 32);
+    p.ch == 2 ? RBQ_NORM(V, 2, 32) : RBQ_NORM(V, 4, 32);
   else
     RBQ_NORM(V, 4, kNormThreads);
 #undef RBQ_NORM
@@ -395,14 +503,15 @@ template <typename T, typename P>
 void run_backward(const T* g, const T* x, const P* w, const float* mean, const float* rstd, T* dx, P* dw, P* db, float* part,
                   int64_t rows, int d, bool vector, cudaStream_t s)
 {
-  const Plan p = plan_of(d, (int)sizeof(T), vector);
+  const Plan p = plan_of(d, (int)sizeof(T), vector, true);
   constexpr int V = 16 / (int)sizeof(T);
-  const int blocks = grad_blocks(p, rows);
+  int blocks = (int)std::min<int64_t>(rows, (int64_t)sms() * kMostBlocks);  // of the wide kernels
   const bool sums = dw != nullptr || db != nullptr;
   float* out = sums ? part : nullptr;
   const size_t smem = sums && p.tpr && p.tpr < kNormThreads ? (size_t)2 * d * sizeof(float) : 0;
-#define RBQ_NORM(VEC, CH, TPR) \
-  norm_grad_kernel<T, P, VEC, CH, TPR><<<blocks, kNormThreads, smem, s>>>(g, x, w, mean, rstd, dx, out, rows, d)
+#define RBQ_NORM(VEC, CH, TPR)                                                                                          \
+  (blocks = blocks_for<Kernel<T, P, VEC, CH, TPR, 1>>(norm_grad_kernel<T, P, VEC, CH, TPR>, smem, rows, TPR),            \
+   norm_grad_kernel<T, P, VEC, CH, TPR><<<blocks, kNormThreads, smem, s>>>(g, x, w, mean, rstd, dx, out, rows, d))
   if (p.tpr == 0) {
     if (dx != nullptr) {
       norm_wide_grad_kernel<T, P><<<blocks, kNormThreads, 0, s>>>(g, x, w, mean, rstd, dx, rows, d);
@@ -414,12 +523,14 @@ void run_backward(const T* g, const T* x, const P* w, const float* mean, const f
       RBQ_LAUNCHED();
     }
   } else {
-    if (p.vec == 1 && p.tpr == 32)
-      p.ch == 8 ? RBQ_NORM(1, 8, 32) : RBQ_NORM(1, 32, 32);
+    if (p.vec == 1 && p.tpr == 8)
+      RBQ_NORM(1, 4, 8);
+    else if (p.vec == 1 && p.tpr == 32)
+      RBQ_NORM(1, 8, 32);
     else if (p.vec == 1)
-      RBQ_NORM(1, 32, kNormThreads);
+      p.ch == 4 ? RBQ_NORM(1, 4, kNormThreads) : RBQ_NORM(1, 32, kNormThreads);
     else if (p.tpr == 8)
-      RBQ_NORM(V, 1, 8);
+      p.ch == 1 ? RBQ_NORM(V, 1, 8) : RBQ_NORM(V, 2, 8);
     else if (p.tpr == 32)
       p.ch == 1 ? RBQ_NORM(V, 1, 32) : p.ch == 2 ? RBQ_NORM(V, 2, 32) : RBQ_NORM(V, 4, 32);
     else
@@ -428,7 +539,7 @@ void run_backward(const T* g, const T* x, const P* w, const float* mean, const f
   }
 #undef RBQ_NORM
   if (sums) {
-    norm_parts_kernel<P><<<(unsigned)ceil_div(2 * (int64_t)d, 32), 256, 0, s>>>(part, blocks, d, dw, db);
+    norm_parts_kernel<P><<<(unsigned)ceil_div(2 * (int64_t)d, 32), 1024, 0, s>>>(part, blocks, d, dw, db);
     RBQ_LAUNCHED();
   }
 }
@@ -460,8 +571,7 @@ void launch_layer_norm(const void* x, const void* w, const void* b, void* y, flo
 
 int64_t layer_norm_workspace(int64_t rows, int d)
 {
-  // the most blocks any way of sharing a row takes
-  return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)sms() * 4)) * 2 * d * (int64_t)sizeof(float);
+  return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)sms() * kMostBlocks)) * 2 * d * (int64_t)sizeof(float);
 }
 
 void launch_layer_norm_backward(const void* g, const void* x, const void* w, const float* mean, const float* rstd, void* dx,

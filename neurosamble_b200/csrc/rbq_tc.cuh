@@ -1,5 +1,5 @@
 // PTX wrappers shared by the tensor-core kernels (sm_100a): mbarriers with bounded waits, TMA tile
-// loads, tcgen05 commits and accumulator reads, and the host's tensor-map encoder.
+// loads, tcgen05 commits and accumulator reads, packed fp32 arithmetic, and the host's tensor-map encoder.
 #pragma once
 
 #include <cuda.h>
@@ -91,6 +91,37 @@ static __device__ __forceinline__ bool mbar_wait_or_fail(uint32_t bar, uint32_t 
   return false;
 }
 
+// Two fp32 values in a register pair: one instruction for both.
+static __device__ __forceinline__ uint64_t pair(float a, float b)
+{
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+static __device__ __forceinline__ float2 split(uint64_t v)
+{
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+static __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+static __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b)
+{
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+static __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b)
+{
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no link-time libcuda).
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
