@@ -51,6 +51,12 @@ constexpr float kGradScale = 16384.0f;        // power of two, see GradRows
 
 __device__ int g_op_err;
 
+// Column sums of the gradient kernel's output (the bias's gradient) come from its staging tiles: in a
+// group, thread t adds columns 2 (t % 32) and the next over the 32 rows of warp t / 32, in registers
+// for as long as the CTA stays in one column of tiles.  Tiles run down the columns for that, so a CTA (or
+// pair) visits each column of tiles once at most and writes one row of sums for it:
+//   sums[((cta * CG + rank) * 4 + warp) * N + column]
+// A pass of its own over the output took as long as a third of the gradient kernel.
 enum Epilogue {
   kEpiLinear,  // out = act(alpha * acc + bias) + extra
   kEpiActGrad, // out = extra * act'(acc + bias)
@@ -78,6 +84,7 @@ struct GemmArgs {
   float alpha = 1.0f;
   const float* alpha_dev = nullptr;  // further factor held on the device
   int act = RBQ_ACT_NONE;
+  float* sums = nullptr;  // kEpiActGrad: column sums of out, see ColumnSums
   int slab_rows = 0;     // rows between slabs
   int slab_add = 0;      // add to what the slab holds
   // softmax loss: rows are queries, columns bank rows col0 + n
@@ -582,6 +589,14 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
     };
     Walk w(a, first_unit);
     read_ahead(w);
+    float2 sums = make_float2(0.0f, 0.0f);
+    int sums_n = -1;  // the column of tiles that they belong to
+    auto write_sums = [&]() {
+      const int col = sums_n * BN + wg * 64 + lane * 2;
+      float* at = a.sums + ((int64_t)(first_unit * CG + rank) * 4 + quarter) * a.N + col;
+      if (col < a.N) at[0] = sums.x;
+      if (col + 1 < a.N) at[1] = sums.y;
+    };
     if (kElement) {
       if (gt < 64) bias[gt] = next_bias;
       group_sync(wg);
@@ -779,6 +794,23 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
                                 Pack<T>::two(o[6], o[7]));
         }
       }
+      if (EPI == kEpiActGrad && a.sums != nullptr && tl.n != sums_n) {
+        if (sums_n >= 0 && !dead) write_sums();
+        sums_n = tl.n;
+        sums = make_float2(0.0f, 0.0f);
+      }
+      if (EPI == kEpiActGrad && a.sums != nullptr) {  // before the barrier: a warp reads its own rows only
+        __syncwarp();
+        const int rows = dead ? 0 : (int)min((int64_t)32, a.M - m0 - quarter * 32);
+#pragma unroll 8
+        for (int r = 0; r < rows; ++r) {
+          const int at = quarter * 32 + r;
+          const float2 f = Pack<T>::get(
+              *reinterpret_cast<const uint32_t*>(buf + at * 128 + (((lane >> 2) ^ (at & 7)) << 4) + (lane & 3) * 4));
+          sums.x += f.x;
+          sums.y += f.y;
+        }
+      }
       if (a.io_tma) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         group_sync(wg);
@@ -796,6 +828,7 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
       }
       ++c;
     }
+    if (EPI == kEpiActGrad && a.sums != nullptr && sums_n >= 0 && !dead) write_sums();
     if (leader) {
       // after a failure: extra inputs in flight land before the shared memory goes away
       if (S::kBufs > 0 && *fail && loaded > 0)
@@ -896,19 +929,35 @@ __global__ void __launch_bounds__(kColThreads) column_sums_kernel(const T* __res
     part[(int64_t)blockIdx.y * cols + c] = t;
   }
 }
+// The parts' columns in 32 interleaved runs, then the runs in their order.  Parts are rows of `cols`
+// floats; with tiles > 0 they are the gradient kernel's sums, `each` rows from each of `ctas` CTAs (or
+// pairs) that walked `tiles` tiles of `width` columns down each column, and those of a CTA that no tile
+// of a column fell to are left out.
 template <typename T>
-__global__ void add_parts_kernel(const float* __restrict__ part, int parts, int cols, T* __restrict__ out)
+__global__ void __launch_bounds__(1024) add_parts_kernel(const float* __restrict__ part, int parts, int cols, int tiles, int width,
+                                                         int ctas, int each, T* __restrict__ out)
 {
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
-  __shared__ float s_sum[8][33];
+  const int lane = threadIdx.x & 31, run = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  __shared__ float s_sum[32][33];
   float t = 0.0f;
-  if (c < cols)
-    for (int p = w; p < parts; p += 8) t += part[(int64_t)p * cols + c];
-  s_sum[w][threadIdx.x & 31] = t;
+  if (c < cols) {
+    const int first = tiles > 0 ? (int)((int64_t)(c / width) * tiles % ctas) : 0;  // CTA of the column's first unit
+#pragma unroll 4
+    for (int p = run; p < parts; p += 32) {
+      bool here = true;
+      if (tiles > 0) {
+        const int ahead = p / each - first;  // units to the CTA's first one in this column
+        here = (ahead < 0 ? ahead + ctas : ahead) < tiles;
+      }
+      if (here) t += part[(int64_t)p * cols + c];
+    }
+  }
+  s_sum[run][lane] = t;
   __syncthreads();
-  if (w == 0 && c < cols) {
+  if (run == 0 && c < cols) {
 #pragma unroll
-    for (int i = 1; i < 8; ++i) t += s_sum[i][threadIdx.x];
+    for (int i = 1; i < 32; ++i) t += s_sum[i][lane];
     out[c] = Pack<T>::from(t);
   }
 }
@@ -1139,7 +1188,8 @@ void gemm(GemmArgs a, Matrix A, bool a_mn, Matrix B, bool b_mn, int cg, const CU
   a.tiles_m = (int)tm;
   a.tiles_n = (int)tn;
   a.kblocks = (int)kb;
-  a.m_fast = tm <= tn;  // the operand with fewer tiles stays in L2 while the other streams by once
+  // The operand with fewer tiles stays in L2 while the other streams by once; column sums want columns.
+  a.m_fast = tm <= tn || a.sums != nullptr;
   const int runs = (int)ceil_div(tn, a.run);
   a.len_fast = a.m_fast ? (int)tm : runs;
   a.len_slow = a.m_fast ? runs : (int)tm;
@@ -1299,6 +1349,15 @@ void linear_backward(const T* g, const T* x, const T* w, const T* bias, T* dx, T
 {
   const Matrix X = addressable(x, m, k, ws, run, s), W = addressable(w, n, k, ws, run, s);
   Matrix Z;
+  const int cg = group_size(m, n);
+  // The gradient kernel's sums are 4 rows of n floats per CTA: less than a pass over dz from about 2,048 rows.
+  const bool fused = act != RBQ_ACT_NONE && m >= 2048;
+  const int64_t tiles_m = ceil_div(m, kBM * cg), tiles_n = ceil_div(n, 128 * cg);
+  const int ctas = (int)std::min<int64_t>(tiles_m * tiles_n, sm_count() / cg);
+  const int gx = (int)ceil_div(n, kColGroup * 8);
+  const int parts = fused ? ctas * cg * 4
+                          : (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(m, 64), ceil_div(4 * sm_count(), gx)));
+  float* part = ws.take<float>((int64_t)parts * n);
   if (act == RBQ_ACT_NONE) {
     Z = addressable(g, m, n, ws, run, s);
   } else {
@@ -1314,12 +1373,12 @@ void linear_backward(const T* g, const T* x, const T* w, const T* bias, T* dx, T
       a.ld_extra = n;
       a.ld_out = ld;
       a.io_tma = n % 8 == 0;
+      a.sums = fused && dbias ? part : nullptr;
       CUtensorMap tx{}, to{};
       if (a.io_tma) {
         tx = tile_map(g, map_type<T>(), 2, m, n, n, 64, kBM);
         to = tile_map(z, map_type<T>(), 2, m, n, ld, 64, kBM);
       }
-      const int cg = group_size(m, n);
       const CUtensorMap *px = a.io_tma ? &tx : nullptr, *po = a.io_tma ? &to : nullptr;
       if (act == RBQ_ACT_GELU)
         gemm<kEpiActGrad, T, RBQ_ACT_GELU>(a, X, false, W, false, cg, px, po, s);
@@ -1329,9 +1388,6 @@ void linear_backward(const T* g, const T* x, const T* w, const T* bias, T* dx, T
   }
   const SlabPlan plan = plan_slabs(n, k, m);
   float* slabs = ws.take<float>(plan.floats());
-  const int gx = (int)ceil_div(n, kColGroup * 8);
-  const int parts = (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(m, 64), ceil_div(4 * sm_count(), gx)));
-  float* part = ws.take<float>((int64_t)parts * n);
   if (!run) return;
   if (dx) store_gemm<T>(Z, false, W, true, 1.0f, nullptr, dx, s);
   if (dw) {
@@ -1339,9 +1395,12 @@ void linear_backward(const T* g, const T* x, const T* w, const T* bias, T* dx, T
     add_slabs<T>(plan, slabs, n, k, 1.0f, nullptr, dw, s);
   }
   if (dbias) {
-    column_sums_kernel<T><<<dim3(gx, parts), kColThreads, 0, s>>>(static_cast<const T*>(Z.p), m, n, Z.ld, part);
-    RBQ_LAUNCHED();
-    add_parts_kernel<T><<<(unsigned)ceil_div(n, 32), 256, 0, s>>>(part, parts, n, dbias);
+    if (!fused) {
+      column_sums_kernel<T><<<dim3(gx, parts), kColThreads, 0, s>>>(static_cast<const T*>(Z.p), m, n, Z.ld, part);
+      RBQ_LAUNCHED();
+    }
+    add_parts_kernel<T><<<(unsigned)ceil_div(n, 32), 1024, 0, s>>>(part, parts, n, fused ? (int)tiles_m : 0, 128 * cg, ctas,
+                                                                  4 * cg, dbias);
     RBQ_LAUNCHED();
   }
 }
