@@ -103,7 +103,8 @@ def make_data_reads(cfg, dev, rank=0, world=1):
 
     import bench_reads
     X, _, _ = bench_reads.make_read_embeddings(cfg["n"], cfg["read_len"], cfg["genome_len"], cfg["seed"], dev,
-                                               d=cfg["d"], rank=rank, world=world, log=log)
+                                               d=cfg["d"], rank=rank, world=world, log=log,
+                                               kernels=cfg.get("encoder") == "kernels")
     if world > 1:
         import torch.distributed as tdist
         tdist.all_reduce(X, op=tdist.ReduceOp.SUM)
@@ -364,7 +365,8 @@ def workload(cfg, R, kmeans):
         return {"workload": (f"BASELINE config 3: read-overlap retrieval, {cfg['n']} simulated reads of "
                              f"{cfg['read_len']} bp from a seeded {cfg['genome_len'] // 1_000_000} Mbp genome (50% "
                              "reverse-complemented, 8% errors 4:2:2 sub:ins:del), synthetic 6-mer pore-model signal, "
-                             "2000/1000 windows, seeded random-init signal encoder (d 256) under fp16 autocast, "
+                             "2000/1000 windows, seeded random-init signal encoder (d 256) "
+                             f"{'on the library operators in fp16' if cfg.get('encoder') == 'kernels' else 'under fp16 autocast'}, "
                              "mean-pooled per read, L2-normalised, fp16 -> fp32; the read set queried against itself; "
                              f"IVF-RaBitQ {_codes(cfg)}, {cfg.get('query_bits', 4)}-bit queries; data generated on the "
                              "device"),
@@ -883,6 +885,8 @@ def main():
                     help="code bits per dimension of both arms (1: RaBitQ; 2..9: ExRaBitQ extra bits)")
     ap.add_argument("--scan-kind", type=int, default=0, choices=[0, 1, 2],
                     help="0: the library's choice (the list scan for large batches), 1: the tile scan, 2: the list scan")
+    ap.add_argument("--encoder", default="torch", choices=["torch", "kernels"],
+                    help="config 3's read encoder: torch's layers, or this library's linear and layer-norm operators")
     ap.add_argument("--nlist", type=int, default=0,
                     help="list count override (reduced-size cases of a configuration's shape; mixtures keep "
                          "one centre per list)")
@@ -898,6 +902,8 @@ def main():
     cfg["query_bits"] = args.query_bits
     cfg["bits_per_dim"] = args.bits
     cfg["scan_kind"] = args.scan_kind
+    if cfg.get("generator") == "reads":
+        cfg["encoder"] = args.encoder
     if args.n:
         cfg["n"] = args.n
     if args.nq:

@@ -23,6 +23,10 @@ The steps restate the reference pipeline that produces the vectors its overlap s
   read vector the mean of the read's window embeddings, L2-normalised, stored as fp16 and read
               back as fp32 (one vector per read; the reference indexes every window)
 
+With kernels=True the encoder's layers run on the library's own operators (SignalEncoder.
+forward_kernels), the path of a user who encodes or trains beside the index; the default stays
+torch's layers, which benchmark configuration 3's vectors come from.
+
 Everything runs on one CUDA device with torch; reads are processed in fixed batches, so a
 read's vector does not depend on how many processes share the work.
 """
@@ -111,6 +115,37 @@ class SignalEncoder(nn.Module):
             x = b(x)
         return self.final_norm(x)
 
+    def forward_kernels(self, signal: torch.Tensor, mask_t: torch.Tensor, dtype: torch.dtype = torch.float16):
+        """The same layers in 16 bits on the library's operators (torch.ops.rbq.linear, layer_norm): every
+        projection's bias, activation and residual sum in the product's epilogue.  The convolutional
+        front end and the attention product are torch's.  Differentiable; no dropout (eval only)."""
+        import neurosamble_b200  # noqa: F401  (registers torch.ops.rbq)
+        ops = torch.ops.rbq
+        if self.training:
+            raise RuntimeError("forward_kernels has no dropout: call eval() first")
+
+        def norm(m, h):
+            return ops.layer_norm(h, m.weight, m.bias, m.eps)[0]
+
+        def linear(m, h, residual=None, act="none"):
+            return ops.linear(h, m.weight.to(dtype), m.bias.to(dtype), residual, act)
+
+        with torch.autocast(device_type=signal.device.type, dtype=dtype):
+            x = self.act(self.conv1(signal.unsqueeze(1).float()))
+            x = self.act(self.conv2(x))
+        x = linear(self.proj, x.to(dtype).transpose(1, 2))
+        n, t, d = x.shape
+        if mask_t.shape[1] == t:
+            x = x * mask_t.unsqueeze(-1).to(dtype)
+        for b in self.blocks:
+            a = b.self_attn
+            qkv = ops.linear(norm(b.norm1, x), a.in_proj_weight.to(dtype), a.in_proj_bias.to(dtype))
+            q, k, v = qkv.view(n, t, 3, a.num_heads, d // a.num_heads).permute(2, 0, 3, 1, 4)
+            h = F.scaled_dot_product_attention(q, k, v).transpose(1, 2).reshape(n, t, d)
+            x = linear(a.out_proj, h, residual=x)
+            x = linear(b.linear2, linear(b.linear1, norm(b.norm2, x), act="gelu"), residual=x)
+        return norm(self.final_norm, x)
+
 
 def make_encoder(seed: int, device, d: int = 256, heads: int = 8) -> SignalEncoder:
     torch.manual_seed(seed)
@@ -133,12 +168,17 @@ def prep_windows(sig: torch.Tensor, valid: torch.Tensor):
     return diff / std, mask_t
 
 
-def encode_windows(enc: SignalEncoder, sig: torch.Tensor, valid: torch.Tensor, amp: bool = True) -> torch.Tensor:
-    """[B, WIN] raw windows -> [B, d] L2-normalised window embeddings (AveragePooler)."""
+def encode_windows(enc: SignalEncoder, sig: torch.Tensor, valid: torch.Tensor, amp: bool = True,
+                   kernels: bool = False) -> torch.Tensor:
+    """[B, WIN] raw windows -> [B, d] L2-normalised window embeddings (AveragePooler).  `kernels` runs the
+    encoder's projections and norms on the library's operators instead of torch's (CUDA only)."""
     x, mask_t = prep_windows(sig, valid)
     with torch.no_grad():
-        with torch.autocast(device_type=x.device.type, dtype=torch.float16, enabled=amp and x.is_cuda):
-            h = enc(x, mask_t)
+        if kernels:
+            h = enc.forward_kernels(x, mask_t)
+        else:
+            with torch.autocast(device_type=x.device.type, dtype=torch.float16, enabled=amp and x.is_cuda):
+                h = enc(x, mask_t)
         h = h.float()
         y = (h * mask_t.unsqueeze(-1)).sum(1) / mask_t.sum(-1).unsqueeze(-1)
     return F.normalize(y, dim=-1)
@@ -208,11 +248,11 @@ def read_windows(sig: torch.Tensor, slen: torch.Tensor):
 
 
 def make_read_embeddings(n_reads=200_000, read_len=5000, genome_len=10_000_000, seed=3003, device="cuda",
-                         d=256, read_batch=512, win_batch=2048, rank=0, world=1, log=None):
+                         d=256, read_batch=512, win_batch=2048, rank=0, world=1, log=None, kernels=False):
     """Config 3 database (= query set): [n_reads, d] float32 on `device` (fp16-rounded), plus
     (starts, strands) of every read.  Rank r of `world` encodes read batches b with b % world == r;
     the caller gathers the rows (every read batch has the same composition whatever the
-    world size)."""
+    world size).  `kernels`: see encode_windows."""
     dev = torch.device(device)
     gen = torch.Generator(device=dev)
     gen.manual_seed(seed)
@@ -234,7 +274,7 @@ def make_read_embeddings(n_reads=200_000, read_len=5000, genome_len=10_000_000, 
         w, val, rid = read_windows(sig, slen)
         emb = torch.empty((w.shape[0], d), dtype=torch.float32, device=dev)
         for c in range(0, w.shape[0], win_batch):
-            emb[c:c + win_batch] = encode_windows(enc, w[c:c + win_batch], val[c:c + win_batch])
+            emb[c:c + win_batch] = encode_windows(enc, w[c:c + win_batch], val[c:c + win_batch], kernels=kernels)
         acc = torch.zeros((b - a, d), dtype=torch.float32, device=dev)
         acc.index_add_(0, rid, emb)
         X[a:b] = F.normalize(acc / torch.bincount(rid, minlength=b - a).clamp(min=1)[:, None].float(), dim=-1)

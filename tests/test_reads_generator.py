@@ -73,3 +73,50 @@ def test_simulated_reads_have_the_configured_shape():
     fwd = [r for r in range(64) if not rc[r]]
     agree = np.mean([(codes[r, :20] == genome[starts[r]:starts[r] + 20].long()).float().mean().item() for r in fwd])
     assert agree > 0.7
+
+
+@pytest.mark.gpu
+def test_encoder_on_the_library_operators():
+    """encode_windows(kernels=True) against the fp32 encoder: per block eight results on the path are
+    rounded to 16 bits (two norms, five projections or sums, the attention product) and four around
+    the blocks; each moves the norm of what passes by at most u, one half of fp16's eps."""
+    enc = BR.make_encoder(4242, "cuda")
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    sig = 90 + 20 * torch.randn((37, BR.WIN), generator=gen, device="cuda")
+    val = torch.full((37,), BR.WIN, device="cuda", dtype=torch.long)
+    val[5], val[20], val[36] = 1500, 1000, 1733
+    sig *= torch.arange(BR.WIN, device="cuda")[None, :] < val[:, None]
+    want = BR.encode_windows(enc, sig, val, amp=False)
+    got = BR.encode_windows(enc, sig, val, kernels=True)
+    u = torch.finfo(torch.float16).eps / 2
+    rel = ((got - want).norm(dim=1) / want.norm(dim=1)).max()
+    assert float(rel) <= (8 * 6 + 4) * u
+    again = BR.encode_windows(enc, sig, val, kernels=True)
+    assert torch.equal(got, again)
+
+
+@pytest.mark.gpu
+def test_encoder_on_the_library_operators_trains():
+    """A contrastive step through the encoder: every weight gets a gradient near the fp32 encoder's (twice
+    the roundings of the forward pass: each layer's backward pass rounds as often)."""
+    import torch.nn.functional as F
+    enc = BR.make_encoder(7, "cuda", d=64, heads=2)
+    gen = torch.Generator(device="cuda").manual_seed(2)
+    sig = 90 + 20 * torch.randn((12, BR.WIN), generator=gen, device="cuda")
+    x, mask_t = BR.prep_windows(sig, torch.full((12,), BR.WIN, device="cuda"))
+    bank = F.normalize(torch.randn((100, 64), generator=gen, device="cuda"), dim=1)
+    target = torch.arange(12, device="cuda") * 8
+    names = [n for n, _ in enc.named_parameters() if not n.startswith("conv")]
+    params = [p for n, p in enc.named_parameters() if not n.startswith("conv")]
+
+    def embed(h):
+        return F.normalize(h.float().mean(1), dim=-1)
+
+    e = embed(enc.forward_kernels(x, mask_t)).half()
+    loss = torch.ops.rbq.softmax_loss(e, bank.half(), target, 5.0)[0]
+    got = torch.autograd.grad(1024.0 * loss.mean(), params)
+    logits = 5.0 * embed(enc(x, mask_t)) @ bank.half().float().t()
+    want = torch.autograd.grad(1024.0 * F.cross_entropy(logits, target), params)
+    u = torch.finfo(torch.float16).eps / 2
+    for n, a, b in zip(names, got, want):
+        assert float((a - b).norm()) <= 2 * (8 * 6 + 6) * u * float(b.norm()) + 1e-6, n
