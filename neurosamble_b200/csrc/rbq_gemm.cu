@@ -23,8 +23,9 @@
 // epilogue pass through 128-byte swizzled staging rows: by TMA where the matrix allows it (rows a
 // multiple of 16 bytes apart), else by coalesced loads and stores of the warp that owns the rows.
 //
-// Long sums with few output tiles (weight gradients) are split along k: every split writes its own
-// fp32 slab and a second kernel adds the slabs in their order, so results do not depend on timing.
+// Long sums with few output tiles (weight gradients) are cut along k instead: every CTA takes an equal
+// run of k-blocks through the tiles laid end to end, writes what it has of a tile to an fp32 slab of that
+// tile, and a second kernel adds a tile's slabs in their order, so results do not depend on timing.
 //
 // Every mbarrier wait is bounded: on time-out the kernel records a code in g_op_err, all roles stop
 // touching memory, copies in flight are waited for (bounded), TMEM is freed and the kernel returns.
@@ -60,7 +61,7 @@ __device__ int g_op_err;
 enum Epilogue {
   kEpiLinear,  // out = act(alpha * acc + bias) + extra
   kEpiActGrad, // out = extra * act'(acc + bias)
-  kEpiSlab,    // fp32 slab of a split along k, written or added to
+  kEpiSlab,    // fp32 slab of a part of k, written or added to
   kEpiLse,     // per row and tile: max and sum of exp of the scaled logits, without the target's
   kEpiProb,    // out = gradient of the loss with respect to the logits, scaled
 };
@@ -68,9 +69,10 @@ enum Epilogue {
 struct GemmArgs {
   int64_t M = 0;
   int N = 0;
-  int tiles_m = 0, tiles_n = 0, splits = 1, kblocks = 0;
+  int tiles_m = 0, tiles_n = 0, kblocks = 0;
   int run = 1, units = 0;  // see Walk
-  int len_fast = 0, len_slow = 0, step_fast = 0, step_slow = 0, step_split = 0;
+  int len_fast = 0, len_slow = 0, step_fast = 0, step_slow = 0;
+  int ctas = 0;  // or pairs
   int m_fast = 0;        // tile order: rows of tiles vary fastest, else columns
   int a_mn = 0, b_mn = 0;  // operand stored with its rows contiguous
   uint32_t idesc = 0;
@@ -316,34 +318,34 @@ __device__ __forceinline__ float2 act_slope(uint64_t z)
   return make_float2(1.0f, 1.0f);
 }
 
-// A unit of work is a run of `run` tiles next to each other in one row of tiles (one tile but for the
-// loss's forward pass).  Units vary fastest along the shorter side of the product, then along the other,
-// then over the splits.
 struct Tile {
-  int m, n, split;
+  int m, n;
 };
-// Steps through a CTA's (or pair's) tiles in order; every role walks the same sequence.  A step
-// adds the grid's size to the unit's (fast, slow, split) digits: no division, which every thread of
-// the epilogue would pay for at each tile.
-struct Walk {
+// Steps through a CTA's (or pair's) tiles in order; every role walks the same sequence.  A unit of work is
+// a run of `run` tiles next to each other in one row of tiles (one tile but for the loss's forward pass);
+// units vary fastest along the shorter side of the product.  A step adds the grid's size to the unit's
+// (fast, slow) digits: no division, which every thread of the epilogue would pay for at each tile.
+struct UnitWalk {
   const GemmArgs& a;
-  int fast, slow, split, r;
-  __device__ __forceinline__ Walk(const GemmArgs& args, int first) : a(args), r(0)
+  int fast, slow, r;
+  __device__ __forceinline__ UnitWalk(const GemmArgs& args, int first) : a(args), r(0)
   {
-    const int per = a.len_fast * a.len_slow;
-    split = first / per;
-    slow = (first - split * per) / a.len_fast;
-    fast = first - split * per - slow * a.len_fast;
+    slow = first / a.len_fast;
+    fast = first - slow * a.len_fast;
   }
-  __device__ __forceinline__ bool live() const { return split < a.splits; }
+  __device__ __forceinline__ bool live() const { return slow < a.len_slow; }
   __device__ __forceinline__ Tile tile() const
   {
-    return a.m_fast ? Tile{fast, slow * a.run + r, split} : Tile{slow, fast * a.run + r, split};
+    return a.m_fast ? Tile{fast, slow * a.run + r} : Tile{slow, fast * a.run + r};
   }
+  __device__ __forceinline__ bool run_starts() const { return r == 0; }
   __device__ __forceinline__ bool run_ends() const
   {
     return r + 1 == a.run || (a.m_fast ? slow : fast) * a.run + r + 1 == a.tiles_n;
   }
+  __device__ __forceinline__ int k_begin() const { return 0; }
+  __device__ __forceinline__ int k_end() const { return a.kblocks; }
+  __device__ __forceinline__ int slab() const { return 0; }
   __device__ __forceinline__ void next()
   {
     if (!run_ends()) {
@@ -353,15 +355,44 @@ struct Walk {
     r = 0;
     fast += a.step_fast;
     slow += a.step_slow;
-    split += a.step_split;
     if (fast >= a.len_fast) fast -= a.len_fast, ++slow;
-    if (slow >= a.len_slow) slow -= a.len_slow, ++split;
   }
 };
-__device__ __forceinline__ int k_begin(const GemmArgs& a, int split)
+// The k-blocks of all tiles, column by column, laid end to end: CTA p of P takes [T p / P, T (p + 1) / P) of
+// the T of them.  Its part of a tile is the tile's slab number p - (the first CTA that has a part of it).
+__host__ __device__ __forceinline__ int64_t first_cta(int64_t at, int64_t ctas, int64_t total)
 {
-  return (int)((int64_t)a.kblocks * split / a.splits);
+  return ((at + 1) * ctas - 1) / total;  // the last p with T p / P <= at
 }
+struct RangeWalk {
+  const GemmArgs& a;
+  int64_t at, end;
+  int cta, t, k;  // tile and k-block of `at`
+  __device__ __forceinline__ RangeWalk(const GemmArgs& args, int first) : a(args), cta(first)
+  {
+    const int64_t total = (int64_t)a.tiles_m * a.tiles_n * a.kblocks;
+    at = total * first / a.ctas;
+    end = total * (first + 1) / a.ctas;
+    t = (int)(at / a.kblocks);
+    k = (int)(at - (int64_t)t * a.kblocks);
+  }
+  __device__ __forceinline__ bool live() const { return at < end; }
+  __device__ __forceinline__ Tile tile() const { return Tile{t % a.tiles_m, t / a.tiles_m}; }
+  __device__ __forceinline__ bool run_starts() const { return true; }
+  __device__ __forceinline__ bool run_ends() const { return true; }
+  __device__ __forceinline__ int k_begin() const { return k; }
+  __device__ __forceinline__ int k_end() const { return (int)min((int64_t)a.kblocks, k + end - at); }
+  __device__ __forceinline__ int slab() const
+  {
+    return cta - (int)first_cta((int64_t)t * a.kblocks, a.ctas, (int64_t)a.tiles_m * a.tiles_n * a.kblocks);
+  }
+  __device__ __forceinline__ void next()
+  {
+    at += k_end() - k;
+    ++t;
+    k = 0;
+  }
+};
 
 template <int EPI, int CG>
 struct Shape {
@@ -408,6 +439,7 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
                 const __grid_constant__ GemmArgs a)
 {
   using S = Shape<EPI, CG>;
+  using Walk = typename std::conditional<EPI == kEpiSlab, RangeWalk, UnitWalk>::type;
   constexpr int BN = S::kBN, kLoadWarp = S::kLoadWarp, kMmaWarp = S::kMmaWarp, kGroups = S::kGroups;
   extern __shared__ unsigned char gemm_smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>(
@@ -464,7 +496,7 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
       for (Walk w(a, first_unit); w.live() && ok; w.next()) {
         const Tile tl = w.tile();
         const int m0 = (tl.m * CG + rank) * kBM, n0 = tl.n * BN + rank * 128;  // this CTA's rows of A and of B
-        for (int kb = k_begin(a, tl.split), ke = k_begin(a, tl.split + 1); kb < ke; ++kb) {
+        for (int kb = w.k_begin(), ke = w.k_end(); kb < ke; ++kb) {
           if (done == S::kStages && !op_wait(smem_u32(&s_empty[st]), lap ^ 1, fail)) {
             fail_with(fail, 1);
             ok = false;
@@ -518,7 +550,7 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const uint32_t d = tmem + acc * BN;
         uint32_t into = 0;  // the first MMA overwrites the accumulator
-        for (int left = k_begin(a, w.split + 1) - k_begin(a, w.split); left > 0; --left) {
+        for (int left = w.k_end() - w.k_begin(); left > 0; --left) {
           if (!op_wait(smem_u32(&s_full[st]), lap, fail)) {
             fail_with(fail, 3);
             ok = false;
@@ -615,7 +647,8 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
       const int64_t tj = next_target < 0 ? -1 : next_target - a.col0 - n0;  // the target's column here, if it is one
       const GradRows gr{next_rows.x, next_rows.y, next_rows.z, next_rows.w};
       const bool some = n0 < a.N;  // the group's columns lie in the matrix
-      const bool first_of_run = w.r == 0, last_of_run = w.run_ends();
+      const bool first_of_run = w.run_starts(), last_of_run = w.run_ends();
+      const int slab = w.slab();
       w.next();
       read_ahead(w);
       if (!dead) {
@@ -700,7 +733,7 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           group_sync(wg);
           if (leader && !dead && !*fail && m0 < a.M) {  // a pair's second half may lie past the last row
-            const int y = tl.split * a.slab_rows + (int)m0;
+            const int y = slab * a.slab_rows + (int)m0;
             if (a.slab_add)
               tma_add_2d(&tmO, smem_u32(bufs), n0 + h * 32, y);
             else
@@ -864,9 +897,14 @@ __global__ void pad_rows_kernel(const uint16_t* __restrict__ src, int64_t rows, 
   }
 }
 
-// out[m, n] = alpha * sum over slabs in ascending order; slab rows are ld (multiple of 4) apart.
+// out[m, n] = alpha * sum over the tile's slabs in ascending order; slab rows are ld (multiple of 4) apart.
+// With `ctas` the slabs of a tile are those of the CTAs that had a part of it (RangeWalk), else all of them.
+struct SlabTiles {
+  int slabs, tile, tiles_m, kblocks, ctas;  // tile: rows and columns of one
+  int64_t total;                            // k-blocks of all tiles
+};
 template <typename T>
-__global__ void add_slabs_kernel(const float* __restrict__ slabs, int splits, int64_t slab_stride, int64_t rows, int cols,
+__global__ void add_slabs_kernel(const float* __restrict__ slabs, SlabTiles st, int64_t slab_stride, int64_t rows, int cols,
                                  int ld, float alpha, const float* __restrict__ alpha_dev, T* __restrict__ out)
 {
   if (alpha_dev != nullptr) alpha *= __ldg(alpha_dev);
@@ -875,8 +913,14 @@ __global__ void add_slabs_kernel(const float* __restrict__ slabs, int splits, in
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
     const int64_t r = i / quads;
     const int c = (int)(i - r * quads) * 4;
+    int n = st.slabs;
+    if (st.ctas > 0) {
+      const int64_t at = ((int64_t)(c / st.tile) * st.tiles_m + r / st.tile) * st.kblocks;
+      n = (int)(first_cta(at + st.kblocks - 1, st.ctas, st.total) - first_cta(at, st.ctas, st.total)) + 1;
+    }
     float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int s = 0; s < splits; ++s) {
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
       const float4 v = *reinterpret_cast<const float4*>(slabs + s * slab_stride + r * ld + c);
       sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
@@ -1154,11 +1198,10 @@ void launch_gemm(GemmArgs& a, const CUtensorMap& ta, const CUtensorMap& tb, cons
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   cudaLaunchConfig_t cfg{};
-  const int step = std::min(a.units, sm_count() / CG);
-  a.step_fast = step % a.len_fast;
-  a.step_slow = step / a.len_fast % a.len_slow;
-  a.step_split = step / a.len_fast / a.len_slow;
-  cfg.gridDim = dim3((unsigned)(CG * step));
+  if (EPI != kEpiSlab) a.ctas = std::min(a.units, sm_count() / CG);
+  a.step_fast = a.ctas % a.len_fast;
+  a.step_slow = a.ctas / a.len_fast;
+  cfg.gridDim = dim3((unsigned)(CG * a.ctas));
   cfg.blockDim = dim3(S::kThreads);
   cfg.dynamicSmemBytes = S::kBytes;
   cfg.stream = s;
@@ -1183,7 +1226,7 @@ void gemm(GemmArgs a, Matrix A, bool a_mn, Matrix B, bool b_mn, int cg, const CU
   a.a_mn = a_mn;
   a.b_mn = b_mn;
   const int64_t tm = ceil_div(a.M, kBM * cg), tn = ceil_div(a.N, 128 * cg), kb = ceil_div(K, kBK);
-  RBQ_CHECK(tm * tn * a.splits < (1ll << 31) && K < (1ll << 31) && a.M < (1ll << 31) - 256, RBQ_ERR_INVALID,
+  RBQ_CHECK(tm * tn < (1ll << 31) && K < (1ll << 31) && a.M < (1ll << 31) - 256, RBQ_ERR_INVALID,
             "matrix product: sizes too large");
   a.tiles_m = (int)tm;
   a.tiles_n = (int)tn;
@@ -1193,7 +1236,7 @@ void gemm(GemmArgs a, Matrix A, bool a_mn, Matrix B, bool b_mn, int cg, const CU
   const int runs = (int)ceil_div(tn, a.run);
   a.len_fast = a.m_fast ? (int)tm : runs;
   a.len_slow = a.m_fast ? runs : (int)tm;
-  a.units = a.len_fast * a.len_slow * a.splits;
+  a.units = a.len_fast * a.len_slow;
   const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   a.idesc = (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
             ((uint32_t)(128 * cg >> 3) << 17) | ((uint32_t)(kBM * cg >> 4) << 24);
@@ -1210,20 +1253,6 @@ void gemm(GemmArgs a, Matrix A, bool a_mn, Matrix B, bool b_mn, int cg, const CU
 // CTAs of a tile: pairs with 256 x 256 tiles where there is one for every SM pair, else single CTAs
 // with 128 x 128 tiles, which spread a small product over four times as many SMs.
 int group_size(int64_t M, int64_t N) { return N > 128 && ceil_div(M, 256) * ceil_div(N, 256) >= sm_count() / 2 ? 2 : 1; }
-
-// Splits along k of a slab product over `slots` CTAs or pairs: the smallest estimated time, in units
-// of one k-block's MMAs (about 0.3 us on a tile).  A split costs its share of the k-blocks, about 8 units to fill and drain, and
-// 0.15 units a tile for writing its slab and reading it back.
-int plan_splits(int64_t tiles, int64_t kblocks, int slots, int most)
-{
-  int best = 1;
-  double cost = 1e300;
-  for (int s = 1; s <= most && s <= kblocks; ++s) {
-    const double c = (double)ceil_div(tiles * s, slots) * ((double)ceil_div(kblocks, s) + 8.0) + 0.15 * tiles * s;
-    if (c < cost * 0.999) cost = c, best = s;
-  }
-  return best;
-}
 
 // Carves aligned pieces out of the caller's workspace; with no workspace it only counts.
 struct Carver {
@@ -1257,21 +1286,29 @@ Matrix addressable(const void* p, int64_t rows, int cols, Carver& ws, bool run, 
   return Matrix{copy, rows, cols, ld};
 }
 
-// out[M, N] = alpha * A B^T through slabs (or at once where one split is best), dense rows.
-// `slabs` of slab_floats(): null to let the caller count.
+// How out[M, N] = alpha * A B^T with a long sum is computed: at once, where its tiles fill the SMs to nine
+// tenths or the sum is short, else through slabs.  A CTA takes 8 k-blocks at least, to be worth its
+// prologue and its slab.
 struct SlabPlan {
-  int cg, splits;
-  int64_t rows, ld;  // of a slab
-  int64_t floats() const { return (int64_t)splits * rows * ld; }
+  bool direct;
+  int cg, ctas, slabs, tiles_m, kblocks;
+  int64_t rows, ld, total;  // rows and their distance in a slab; k-blocks of all tiles
+  int64_t floats() const { return direct ? 0 : (int64_t)slabs * rows * ld; }
 };
-SlabPlan plan_slabs(int64_t M, int N, int64_t K)
+SlabPlan plan_slabs(int64_t M, int N, int64_t K, bool must_add)
 {
   SlabPlan p;
   p.cg = N > 128 && M > 128 ? 2 : 1;
-  p.splits = plan_splits(ceil_div(M, kBM * p.cg) * ceil_div(N, 128 * p.cg), ceil_div(K, kBK), sm_count() / p.cg, 64);
+  const int64_t slots = sm_count() / p.cg, tm = ceil_div(M, kBM * p.cg), tiles = tm * ceil_div(N, 128 * p.cg);
+  p.tiles_m = (int)tm;
+  p.kblocks = (int)ceil_div(K, kBK);
+  p.total = tiles * p.kblocks;
+  p.direct = !must_add && (p.kblocks <= 8 || tiles * 10 >= ceil_div(tiles, slots) * slots * 9);
+  p.ctas = (int)std::min(slots, std::max(tiles, p.total / 8));
+  p.slabs = (int)std::min<int64_t>(p.ctas, (p.kblocks - 1) / (p.total / p.ctas) + 2);
   p.rows = round_up(M, kBM);
   p.ld = round_up(N, 4);
-  while (p.splits > 1 && p.splits * p.rows >= (1ll << 31)) --p.splits;
+  RBQ_CHECK(p.direct || p.slabs * p.rows < (1ll << 31), RBQ_ERR_INVALID, "matrix product: sizes too large");
   return p;
 }
 template <typename T>
@@ -1279,36 +1316,36 @@ void slab_gemm(const SlabPlan& p, Matrix A, bool a_mn, Matrix B, bool b_mn, floa
 {
   const int64_t N = b_mn ? B.cols : B.rows;
   GemmArgs a;
-  a.splits = p.splits;
+  a.ctas = p.ctas;
   a.slab_rows = (int)p.rows;
   a.slab_add = add;
-  const CUtensorMap to = tile_map(slabs, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.splits * p.rows, N, p.ld, 32, kBM);
+  const CUtensorMap to = tile_map(slabs, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.slabs * p.rows, N, p.ld, 32, kBM);
   gemm<kEpiSlab, T>(a, A, a_mn, B, b_mn, p.cg, nullptr, &to, s);
 }
+// `all`: every slab holds a sum (of zeros at least), else those of RangeWalk.
 template <typename T>
-void add_slabs(const SlabPlan& p, const float* slabs, int64_t M, int N, float alpha, const float* alpha_dev, T* out,
+void add_slabs(const SlabPlan& p, const float* slabs, bool all, int64_t M, int N, float alpha, const float* alpha_dev, T* out,
                cudaStream_t s)
 {
   const int64_t blocks = std::min<int64_t>(ceil_div(M * (p.ld / 4), 256), (int64_t)sm_count() * 8);
-  add_slabs_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(slabs, p.splits, p.rows * p.ld, M, N, (int)p.ld, alpha, alpha_dev,
-                                                       out);
+  const SlabTiles st{p.slabs, 128 * p.cg, p.tiles_m, p.kblocks, all ? 0 : p.ctas, p.total};
+  add_slabs_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(slabs, st, p.rows * p.ld, M, N, (int)p.ld, alpha, alpha_dev, out);
   RBQ_LAUNCHED();
 }
 
-// out[M, N] (dense) = alpha * A B^T, written by the product's own epilogue.
+// out[M, N] (dense) = alpha_dev * A B^T, written by the product's own epilogue.
 template <typename T>
-void store_gemm(Matrix A, bool a_mn, Matrix B, bool b_mn, float alpha, const float* alpha_dev, T* out, cudaStream_t s)
+void store_gemm(Matrix A, bool a_mn, Matrix B, bool b_mn, int cg, const float* alpha_dev, T* out, cudaStream_t s)
 {
   const int64_t M = a_mn ? A.cols : A.rows, N = b_mn ? B.cols : B.rows;
   GemmArgs a;
-  a.alpha = alpha;
   a.alpha_dev = alpha_dev;
   a.out = out;
   a.ld_out = N;
   a.io_tma = N % 8 == 0;
   CUtensorMap to{};
   if (a.io_tma) to = tile_map(out, map_type<T>(), 2, M, N, N, 64, kBM);
-  gemm<kEpiLinear, T>(a, A, a_mn, B, b_mn, group_size(M, N), nullptr, a.io_tma ? &to : nullptr, s);
+  gemm<kEpiLinear, T>(a, A, a_mn, B, b_mn, cg, nullptr, a.io_tma ? &to : nullptr, s);
 }
 
 template <typename T>
@@ -1386,13 +1423,14 @@ void linear_backward(const T* g, const T* x, const T* w, const T* bias, T* dx, T
         gemm<kEpiActGrad, T, RBQ_ACT_RELU>(a, X, false, W, false, cg, px, po, s);
     }
   }
-  const SlabPlan plan = plan_slabs(n, k, m);
+  const SlabPlan plan = plan_slabs(n, k, m, false);
   float* slabs = ws.take<float>(plan.floats());
   if (!run) return;
-  if (dx) store_gemm<T>(Z, false, W, true, 1.0f, nullptr, dx, s);
-  if (dw) {
+  if (dx) store_gemm<T>(Z, false, W, true, group_size(m, k), nullptr, dx, s);
+  if (dw && plan.direct) store_gemm<T>(Z, true, X, true, plan.cg, nullptr, dw, s);
+  if (dw && !plan.direct) {
     slab_gemm<T>(plan, Z, true, X, true, slabs, false, s);
-    add_slabs<T>(plan, slabs, n, k, 1.0f, nullptr, dw, s);
+    add_slabs<T>(plan, slabs, false, n, k, 1.0f, nullptr, dw, s);
   }
   if (dbias) {
     if (!fused) {
@@ -1435,8 +1473,11 @@ void loss_forward(const T* q, const T* bank, const int64_t* target, int64_t n, i
 constexpr int64_t kPieceBytes = 512ll << 20;
 int64_t piece_columns(int64_t n, int64_t v)
 {
-  const int64_t most = std::max<int64_t>(256, kPieceBytes / (2 * n) / 256 * 256);
-  return round_up(ceil_div(v, ceil_div(v, most)), 256);
+  const int64_t most = std::max<int64_t>(1, kPieceBytes / (2 * n) / 256);  // in tiles of 256 columns
+  // whole rounds of the SM pairs for the bank's gradient, where a piece holds one
+  const int64_t pairs = sm_count() / 2, whole = most >= pairs ? most / pairs * pairs : most;
+  const int64_t tiles = ceil_div(v, 256);
+  return ceil_div(tiles, ceil_div(tiles, whole)) * 256;
 }
 
 template <typename T>
@@ -1448,14 +1489,21 @@ void loss_backward(const float* g, const T* q, const T* bank, const int64_t* tar
   float* top = ws.take<float>(3);
   float4* rows = ws.take<float4>(n);
   T* prob = ws.take<T>(n * piece);
-  const SlabPlan pq = plan_slabs(n, d, piece), pb = plan_slabs(piece, d, n);
+  // The queries' gradient is summed over the pieces, in slabs that start from zero; the last piece may be
+  // shorter than the others.
+  const bool pieces = v > piece;
+  const int64_t whole = std::min(piece, v), last = (v - 1) % piece + 1;
+  SlabPlan pq = plan_slabs(n, d, whole, pieces), pq_last = plan_slabs(n, d, last, pieces);
+  pq.slabs = pq_last.slabs = std::max(pq.slabs, pq_last.slabs);
   float* slabs_q = ws.take<float>(pq.floats());
-  float* slabs_b = ws.take<float>(pb.floats());
+  const SlabPlan pb = plan_slabs(whole, d, n, false), pb_last = plan_slabs(last, d, n, false);
+  float* slabs_b = ws.take<float>(std::max(pb.floats(), pb_last.floats()));
   if (!run) return;
   grad_top_kernel<T><<<1, 1024, 0, s>>>(g, target, loss, n, v, scale, top);
   RBQ_LAUNCHED();
   grad_rows_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(g, target, loss, lse, n, v, top, rows);
   RBQ_LAUNCHED();
+  if (dq && pieces) RBQ_CUDA(cudaMemsetAsync(slabs_q, 0, pq.floats() * sizeof(float), s));
   for (int64_t v0 = 0; v0 < v; v0 += piece) {
     const int64_t cols = std::min(piece, v - v0);
     const Matrix Bp{static_cast<const T*>(B.p) + v0 * B.ld, cols, d, B.ld};
@@ -1467,20 +1515,20 @@ void loss_backward(const float* g, const T* q, const T* bank, const int64_t* tar
     a.rows = rows;
     const CUtensorMap to = tile_map(prob, map_type<T>(), 2, n, cols, piece, 64, kBM);
     gemm<kEpiProb, T>(a, Q, false, Bp, false, group_size(n, cols), nullptr, &to, s);
-    if (dq) {
-      SlabPlan p = pq;  // the last, shorter piece keeps the slabs; no split may be empty
-      const int64_t kb = ceil_div(cols, kBK);
-      if (p.splits > kb) p.splits = (int)kb;
-      slab_gemm<T>(p, P, false, Bp, true, slabs_q, v0 > 0, s);
-    }
+    const bool at_last = v0 + piece >= v;
+    if (dq && pq.direct) store_gemm<T>(P, false, Bp, true, pq.cg, top + 1, dq, s);
+    if (dq && !pq.direct) slab_gemm<T>(at_last ? pq_last : pq, P, false, Bp, true, slabs_q, pieces, s);
     if (dbank) {
-      SlabPlan p = pb;
-      p.rows = round_up(cols, kBM);
-      slab_gemm<T>(p, P, true, Q, true, slabs_b, false, s);
-      add_slabs<T>(p, slabs_b, cols, d, 1.0f, top + 1, dbank + v0 * d, s);
+      const SlabPlan& p = at_last ? pb_last : pb;
+      if (p.direct) {
+        store_gemm<T>(P, true, Q, true, p.cg, top + 1, dbank + v0 * d, s);
+      } else {
+        slab_gemm<T>(p, P, true, Q, true, slabs_b, false, s);
+        add_slabs<T>(p, slabs_b, false, cols, d, 1.0f, top + 1, dbank + v0 * d, s);
+      }
     }
   }
-  if (dq) add_slabs<T>(pq, slabs_q, n, d, 1.0f, top + 1, dq, s);
+  if (dq && !pq.direct) add_slabs<T>(pq, slabs_q, pieces, n, d, 1.0f, top + 1, dq, s);
 }
 
 }  // namespace
