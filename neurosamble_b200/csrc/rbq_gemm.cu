@@ -77,7 +77,7 @@ struct GemmArgs {
   int a_mn = 0, b_mn = 0;  // operand stored with its rows contiguous
   uint32_t idesc = 0;
   // epilogue matrices
-  int io_tma = 1;        // staging moves by TMA; else by the warps from / to the pointers below
+  int extra_tma = 1, out_tma = 1;  // staging moves by TMA; else by the warps from / to the pointers below
   const void* bias = nullptr;   // [N]
   const void* extra = nullptr;  // [M, N]
   void* out = nullptr;          // [M, N]
@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
     auto parity_of = [&](int k) { return (uint32_t)((S::kBufs == 2 ? k >> 1 : k) & 1); };
 
     // The extra inputs of the group's tiles arrive by TMA, in order; `ask` is the next tile to ask for.
-    const bool extra_tma = kElement && a.has_extra && a.io_tma;
+    const bool extra_tma = kElement && a.has_extra && a.extra_tma;
     int loaded = 0;
     Walk ask(a, first_unit);
     auto ask_extra = [&]() {
@@ -756,19 +756,22 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
             dead = true;
           }
         }
-      } else if (a.io_tma) {
-        if (leader) {
-          if (S::kBufs == 2)
-            asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
-          else
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      } else {
+        if (a.out_tma) {
+          if (leader) {
+            if (S::kBufs == 2)
+              asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");
+            else
+              asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+          }
+          group_sync(wg);  // the buffer's last store has been read
         }
-        group_sync(wg);  // the buffer's last store has been read
-      } else if (kElement && a.has_extra) {
-        if (!dead)
-          move_rows<T, true>(buf, reinterpret_cast<T*>(const_cast<void*>(a.extra)), m0, a.M, a.ld_extra, n0, a.N, quarter * 32,
-                             lane);
-        __syncwarp();
+        if (kElement && a.has_extra) {
+          if (!dead)
+            move_rows<T, true>(buf, reinterpret_cast<T*>(const_cast<void*>(a.extra)), m0, a.M, a.ld_extra, n0, a.N,
+                               quarter * 32, lane);
+          __syncwarp();
+        }
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -844,7 +847,7 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
           sums.y += f.y;
         }
       }
-      if (a.io_tma) {
+      if (a.out_tma) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         group_sync(wg);
         if (leader && !dead && !*fail) {
@@ -885,15 +888,20 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
 // Small kernels around the products.
 // ---------------------------------------------------------------------------------------
 
-// Rows of `cols` 16-bit values -> rows `ld` apart (ld a multiple of 8, so that TMA can address them).
+// Rows of `cols` 16-bit values -> rows `ld` apart (ld a multiple of 8, so that TMA can address them).  A thread
+// makes 16 bytes of the copy.
 __global__ void pad_rows_kernel(const uint16_t* __restrict__ src, int64_t rows, int cols, int ld,
                                 uint16_t* __restrict__ dst)
 {
-  const int64_t total = rows * ld;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t r = i / ld;
-    const int c = (int)(i - r * ld);
-    dst[i] = c < cols ? src[r * cols + c] : (uint16_t)0;
+  const int per = ld / 8;
+  for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < rows; r += (int64_t)gridDim.x * blockDim.y) {
+    for (int i = threadIdx.x; i < per; i += blockDim.x) {
+      uint32_t v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = i * 8 + e < cols ? src[r * cols + i * 8 + e] : 0u;
+      *reinterpret_cast<uint4*>(dst + r * ld + i * 8) =
+          make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
+    }
   }
 }
 
@@ -1184,6 +1192,12 @@ constexpr CUtensorMapDataType map_type()
 {
   return std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
+// 64 columns by `box_rows` rows of an operand or output.
+template <typename T>
+CUtensorMap matrix_map(const Matrix& m, int box_rows)
+{
+  return tile_map(m.p, map_type<T>(), 2, m.rows, m.cols, m.ld, 64, box_rows);
+}
 
 template <int EPI, typename T, int CG, int ACT>
 void launch_gemm(GemmArgs& a, const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tx, const CUtensorMap& to,
@@ -1240,8 +1254,7 @@ void gemm(GemmArgs a, Matrix A, bool a_mn, Matrix B, bool b_mn, int cg, const CU
   const uint32_t f = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   a.idesc = (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) |
             ((uint32_t)(128 * cg >> 3) << 17) | ((uint32_t)(kBM * cg >> 4) << 24);
-  const CUtensorMap ta = tile_map(A.p, map_type<T>(), 2, A.rows, A.cols, A.ld, 64, a_mn ? kBK : 128);
-  const CUtensorMap tb = tile_map(B.p, map_type<T>(), 2, B.rows, B.cols, B.ld, 64, b_mn ? kBK : 128);
+  const CUtensorMap ta = matrix_map<T>(A, a_mn ? kBK : 128), tb = matrix_map<T>(B, b_mn ? kBK : 128);
   const CUtensorMap& x = tx ? *tx : ta;
   const CUtensorMap& o = to ? *to : ta;
   if (cg == 2)
@@ -1270,9 +1283,12 @@ struct Carver {
 
 void pad_rows(const void* src, int64_t rows, int cols, int ld, void* dst, cudaStream_t s)
 {
-  const int64_t blocks = std::min<int64_t>(ceil_div(rows * ld, 256), (int64_t)sm_count() * 16);
-  pad_rows_kernel<<<(unsigned)blocks, 256, 0, s>>>(static_cast<const uint16_t*>(src), rows, cols, ld,
-                                                   static_cast<uint16_t*>(dst));
+  int x = 8;  // threads to a row
+  while (x < 256 && x < ld / 8) x *= 2;
+  const dim3 block(x, 256 / x);
+  const int64_t blocks = std::min<int64_t>(ceil_div(rows, block.y), (int64_t)sm_count() * 16);
+  pad_rows_kernel<<<(unsigned)blocks, block, 0, s>>>(static_cast<const uint16_t*>(src), rows, cols, ld,
+                                                     static_cast<uint16_t*>(dst));
   RBQ_LAUNCHED();
 }
 
@@ -1342,10 +1358,10 @@ void store_gemm(Matrix A, bool a_mn, Matrix B, bool b_mn, int cg, const float* a
   a.alpha_dev = alpha_dev;
   a.out = out;
   a.ld_out = N;
-  a.io_tma = N % 8 == 0;
+  a.out_tma = N % 8 == 0;
   CUtensorMap to{};
-  if (a.io_tma) to = tile_map(out, map_type<T>(), 2, M, N, N, 64, kBM);
-  gemm<kEpiLinear, T>(a, A, a_mn, B, b_mn, cg, nullptr, a.io_tma ? &to : nullptr, s);
+  if (a.out_tma) to = matrix_map<T>(Matrix{out, M, N, N}, kBM);
+  gemm<kEpiLinear, T>(a, A, a_mn, B, b_mn, cg, nullptr, a.out_tma ? &to : nullptr, s);
 }
 
 template <typename T>
@@ -1360,14 +1376,14 @@ void linear_forward(const T* x, const T* w, const T* bias, const T* residual, T*
   a.has_extra = residual != nullptr;
   a.out = y;
   a.ld_extra = a.ld_out = n;
-  a.io_tma = n % 8 == 0;
+  a.extra_tma = a.out_tma = n % 8 == 0;
   CUtensorMap tx{}, to{};
-  if (a.io_tma) {
-    to = tile_map(y, map_type<T>(), 2, m, n, n, 64, kBM);
-    tx = residual ? tile_map(residual, map_type<T>(), 2, m, n, n, 64, kBM) : to;
+  if (a.out_tma) {
+    to = matrix_map<T>(Matrix{y, m, n, n}, kBM);
+    tx = residual ? matrix_map<T>(Matrix{residual, m, n, n}, kBM) : to;
   }
   const int cg = group_size(m, n);
-  const CUtensorMap *px = a.io_tma ? &tx : nullptr, *po = a.io_tma ? &to : nullptr;
+  const CUtensorMap *px = a.out_tma ? &tx : nullptr, *po = a.out_tma ? &to : nullptr;
   if (act == RBQ_ACT_GELU)
     gemm<kEpiLinear, T, RBQ_ACT_GELU>(a, X, false, W, false, cg, px, po, s);
   else if (act == RBQ_ACT_RELU)
@@ -1399,24 +1415,18 @@ void linear_backward(const T* g, const T* x, const T* w, const T* bias, T* dx, T
     Z = addressable(g, m, n, ws, run, s);
   } else {
     const int64_t ld = round_up(n, 8);
-    T* z = ws.take<T>(m * ld);
-    Z = Matrix{z, m, n, ld};
+    Z = Matrix{ws.take<T>(m * ld), m, n, ld};
     if (run) {
       GemmArgs a;
       a.bias = bias;
       a.extra = g;
       a.has_extra = 1;
-      a.out = z;
       a.ld_extra = n;
-      a.ld_out = ld;
-      a.io_tma = n % 8 == 0;
+      a.extra_tma = n % 8 == 0;
       a.sums = fused && dbias ? part : nullptr;
-      CUtensorMap tx{}, to{};
-      if (a.io_tma) {
-        tx = tile_map(g, map_type<T>(), 2, m, n, n, 64, kBM);
-        to = tile_map(z, map_type<T>(), 2, m, n, ld, 64, kBM);
-      }
-      const CUtensorMap *px = a.io_tma ? &tx : nullptr, *po = a.io_tma ? &to : nullptr;
+      CUtensorMap tx{};
+      if (a.extra_tma) tx = matrix_map<T>(Matrix{g, m, n, n}, kBM);
+      const CUtensorMap to = matrix_map<T>(Z, kBM), *px = a.extra_tma ? &tx : nullptr, *po = &to;
       if (act == RBQ_ACT_GELU)
         gemm<kEpiActGrad, T, RBQ_ACT_GELU>(a, X, false, W, false, cg, px, po, s);
       else
@@ -1488,7 +1498,8 @@ void loss_backward(const float* g, const T* q, const T* bank, const int64_t* tar
   const int64_t piece = std::min(piece_columns(n, v), round_up(v, 8));
   float* top = ws.take<float>(3);
   float4* rows = ws.take<float4>(n);
-  T* prob = ws.take<T>(n * piece);
+  const int64_t ld = round_up(piece, 8);
+  T* prob = ws.take<T>(n * ld);
   // The queries' gradient is summed over the pieces, in slabs that start from zero; the last piece may be
   // shorter than the others.
   const bool pieces = v > piece;
@@ -1507,13 +1518,13 @@ void loss_backward(const float* g, const T* q, const T* bank, const int64_t* tar
   for (int64_t v0 = 0; v0 < v; v0 += piece) {
     const int64_t cols = std::min(piece, v - v0);
     const Matrix Bp{static_cast<const T*>(B.p) + v0 * B.ld, cols, d, B.ld};
-    const Matrix P{prob, n, cols, piece};
+    const Matrix P{prob, n, cols, ld};
     GemmArgs a;
     a.c2 = scale * kLog2e;
     a.col0 = v0;
     a.target = target;
     a.rows = rows;
-    const CUtensorMap to = tile_map(prob, map_type<T>(), 2, n, cols, piece, 64, kBM);
+    const CUtensorMap to = matrix_map<T>(P, kBM);
     gemm<kEpiProb, T>(a, Q, false, Bp, false, group_size(n, cols), nullptr, &to, s);
     const bool at_last = v0 + piece >= v;
     if (dq && pq.direct) store_gemm<T>(P, false, Bp, true, pq.cg, top + 1, dq, s);
