@@ -405,9 +405,13 @@ struct Shape {
   // input streams in for every tile (its load then overlaps the tile before), else one.
   static constexpr int kBufs = EPI == kEpiLse ? 0 : EPI == kEpiActGrad ? 2 : 1;
   static constexpr int kOutBytes = kGroups * kBufs * kStageOut;
-  static constexpr int kFit = (226 * 1024 + 512 - 1024 - 2 * kBN * 4 - kOutBytes) / kOperands;  // stages of 227 KB less the barriers
+  // Stages, staging, [2][BN] bias values, barriers: as many stages as 227 KB hold, all of it in dynamic
+  // shared memory, which starts on the 1,024 bytes that the swizzle wants when there is no other.
+  static constexpr int kTail = 2 * kBN * 4 + 256;
+  static constexpr int kFit = (227 * 1024 - kTail - kOutBytes) / kOperands;
   static constexpr int kStages = kFit < 6 ? kFit : 6;
-  static constexpr int kBytes = kStages * kOperands + kOutBytes + 2 * kBN * 4 + 1024;
+  static constexpr int kBytes = kStages * kOperands + kOutBytes + kTail;
+  static_assert((2 * kStages + 4 + kGroups * 2) * 8 + 8 <= 256, "barriers");
 };
 
 // The warp's 32 staging rows <-> a matrix whose rows no TMA can address, 64 columns from `col`.
@@ -441,26 +445,29 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
   using S = Shape<EPI, CG>;
   using Walk = typename std::conditional<EPI == kEpiSlab, RangeWalk, UnitWalk>::type;
   constexpr int BN = S::kBN, kLoadWarp = S::kLoadWarp, kMmaWarp = S::kMmaWarp, kGroups = S::kGroups;
-  extern __shared__ unsigned char gemm_smem_raw[];
-  unsigned char* base = reinterpret_cast<unsigned char*>(
-      (reinterpret_cast<uintptr_t>(gemm_smem_raw) + 1023) & ~(uintptr_t)1023);
+  extern __shared__ __align__(1024) unsigned char gemm_smem[];
+  unsigned char* base = gemm_smem;
+  if (smem_u32(base) & 1023u) {  // the swizzle pattern is taken from the address bits
+    if (threadIdx.x == 0) atomicExch(&g_op_err, 7);
+    return;
+  }
   unsigned char* staging = base + S::kStages * S::kOperands;
   float* s_bias = reinterpret_cast<float*>(staging + S::kOutBytes);  // [2][BN]: this tile's and the next one's
-  __shared__ __align__(8) unsigned long long s_full[S::kStages], s_empty[S::kStages], s_done[2], s_free[2],
-      s_x[kGroups * 2];
-  __shared__ uint32_t s_tmem;
-  __shared__ int s_fail;
+  unsigned long long* s_full = reinterpret_cast<unsigned long long*>(s_bias + 2 * BN);
+  unsigned long long *s_empty = s_full + S::kStages, *s_done = s_empty + S::kStages, *s_free = s_done + 2, *s_x = s_free + 2;
+  uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_x + kGroups * 2);
+  int* s_fail = reinterpret_cast<int*>(s_tmem + 1);
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int rank = CG == 2 ? (int)(blockIdx.x & 1) : 0;  // in the pair; 0 leads
   const int first_unit = blockIdx.x / CG;
   if (warp == kMmaWarp) {
     if (CG == 1) {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)),
                    "r"((uint32_t)(2 * BN)));
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     } else {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(s_tmem)),
                    "r"((uint32_t)(2 * BN)));
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     }
@@ -475,15 +482,15 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
       mbar_init(smem_u32(&s_free[i]), kGroups * 4 * CG);  // one arrival per epilogue warp of the pair
     }
     for (int i = 0; i < kGroups * 2; ++i) mbar_init(smem_u32(&s_x[i]), 1);
-    s_fail = 0;
+    *s_fail = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
   if (CG == 2) cluster_sync();  // the pair's barriers exist
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-  const uint32_t tmem = s_tmem;
-  volatile int* fail = &s_fail;
+  const uint32_t tmem = *s_tmem;
+  volatile int* fail = s_fail;
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
