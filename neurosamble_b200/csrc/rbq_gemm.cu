@@ -46,6 +46,8 @@ namespace {
 constexpr int kBM = 128;       // output rows of a tile (TMEM lanes)
 constexpr int kBK = 64;        // reduction values per stage: one 128-byte row of 16-bit values
 constexpr int kStageOut = kBM * 128;          // one staging buffer: 128 rows of 128 bytes
+constexpr int kSlabCols = 16;                 // a slab's: 128 rows of 64 bytes, which leaves room for one more stage
+constexpr int kSlabOut = kBM * kSlabCols * 4;
 constexpr uint32_t kOpWaitLimit = 1u << 22;   // polls; each suspends for up to some microseconds
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGradScale = 16384.0f;        // power of two, see GradRows
@@ -404,12 +406,13 @@ struct Shape {
   // Staging buffers per group: none in the loss's forward pass, which writes no tile; two where an extra
   // input streams in for every tile (its load then overlaps the tile before), else one.
   static constexpr int kBufs = EPI == kEpiLse ? 0 : EPI == kEpiActGrad ? 2 : 1;
-  static constexpr int kOutBytes = kGroups * kBufs * kStageOut;
+  static constexpr int kBufBytes = EPI == kEpiSlab ? kSlabOut : kStageOut;
+  static constexpr int kOutBytes = kGroups * kBufs * kBufBytes;
   // Stages, staging, [2][BN] bias values, barriers: as many stages as 227 KB hold, all of it in dynamic
   // shared memory, which starts on the 1,024 bytes that the swizzle wants when there is no other.
   static constexpr int kTail = 2 * kBN * 4 + 256;
   static constexpr int kFit = (227 * 1024 - kTail - kOutBytes) / kOperands;
-  static constexpr int kStages = kFit < 6 ? kFit : 6;
+  static constexpr int kStages = kFit < 7 ? kFit : 7;
   static constexpr int kBytes = kStages * kOperands + kOutBytes + kTail;
   static_assert((2 * kStages + 4 + kGroups * 2) * 8 + 8 <= 256, "barriers");
 };
@@ -588,7 +591,7 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
     const int gt = tid & 127;  // thread of the group = accumulator lane = output row
     const bool leader = gt == 0;
     constexpr bool kElement = EPI == kEpiLinear || EPI == kEpiActGrad;
-    unsigned char* bufs = staging + wg * S::kBufs * kStageOut;
+    unsigned char* bufs = staging + wg * S::kBufs * S::kBufBytes;
     float* bias = s_bias + wg * 64;
     bool dead = false;  // a wait failed: keep the barriers in step, touch nothing
     int c = 0;          // staging tile, counted over the group's run: buffer c % kBufs
@@ -723,28 +726,35 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
         continue;
       }
 
-      if (EPI == kEpiSlab) {  // 32 columns of fp32 to a staging row, twice
+      if (EPI == kEpiSlab) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           float v[32];
           read_half(h, v);
-          if (n0 + h * 32 >= a.N) break;  // only past the first half
-          if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-          group_sync(wg);  // the buffer's last store has been read
-          if (!dead) {
-            float4* at = reinterpret_cast<float4*>(bufs + gt * 128);
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              at[k ^ (gt & 7)] = make_float4(v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]);
-          }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          group_sync(wg);
-          if (leader && !dead && !*fail && m0 < a.M) {  // a pair's second half may lie past the last row
-            const int y = slab * a.slab_rows + (int)m0;
-            if (a.slab_add)
-              tma_add_2d(&tmO, smem_u32(bufs), n0 + h * 32, y);
-            else
-              tma_store_2d(&tmO, smem_u32(bufs), n0 + h * 32, y);
+          for (int q = 0; q < 32 / kSlabCols; ++q) {
+            const int col = n0 + h * 32 + q * kSlabCols;
+            if (col < a.N) {
+              if (leader) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+              group_sync(wg);  // the buffer's last store has been read
+              if (!dead) {
+                float4* at = reinterpret_cast<float4*>(bufs + gt * kSlabCols * 4);
+#pragma unroll
+                for (int k = 0; k < kSlabCols / 4; ++k) {
+                  const float* e = v + q * kSlabCols + 4 * k;
+                  at[k ^ ((gt >> 1) & 3)] = make_float4(e[0], e[1], e[2], e[3]);  // 64-byte swizzle
+                }
+              }
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              group_sync(wg);
+              if (leader && !dead && !*fail && m0 < a.M) {  // a pair's second half may lie past the last row
+                const int y = slab * a.slab_rows + (int)m0;
+                if (a.slab_add)
+                  tma_add_2d(&tmO, smem_u32(bufs), col, y);
+                else
+                  tma_store_2d(&tmO, smem_u32(bufs), col, y);
+              }
+            }
           }
         }
         continue;
@@ -1171,7 +1181,7 @@ struct Matrix {
 };
 
 CUtensorMap tile_map(const void* p, CUtensorMapDataType type, int esize, int64_t rows, int64_t cols, int64_t ld, int box_cols,
-                     int box_rows)
+                     int box_rows, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B)
 {
   CUtensorMap m;
   // The encoder is a driver call and wants the device's context bound to this host thread, which
@@ -1188,8 +1198,7 @@ CUtensorMap tile_map(const void* p, CUtensorMapDataType type, int esize, int64_t
   const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   const CUresult r = tensor_map_encoder()(&m, type, 2, const_cast<void*>(p), dims, strides, box, estr,
-                                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                          CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   RBQ_CHECK(r == CUDA_SUCCESS, RBQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
   return m;
 }
@@ -1342,7 +1351,8 @@ void slab_gemm(const SlabPlan& p, Matrix A, bool a_mn, Matrix B, bool b_mn, floa
   a.ctas = p.ctas;
   a.slab_rows = (int)p.rows;
   a.slab_add = add;
-  const CUtensorMap to = tile_map(slabs, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.slabs * p.rows, N, p.ld, 32, kBM);
+  const CUtensorMap to = tile_map(slabs, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, p.slabs * p.rows, N, p.ld, kSlabCols, kBM,
+                                  CU_TENSOR_MAP_SWIZZLE_64B);
   gemm<kEpiSlab, T>(a, A, a_mn, B, b_mn, p.cg, nullptr, &to, s);
 }
 // `all`: every slab holds a sum (of zeros at least), else those of RangeWalk.
