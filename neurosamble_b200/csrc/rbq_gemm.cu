@@ -1198,7 +1198,8 @@ CUtensorMap tile_map(const void* p, CUtensorMapDataType type, int esize, int64_t
   const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   const cuuint32_t estr[2] = {1, 1};
   const CUresult r = tensor_map_encoder()(&m, type, 2, const_cast<void*>(p), dims, strides, box, estr,
-                                          CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                                          CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   RBQ_CHECK(r == CUDA_SUCCESS, RBQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (" + std::to_string((int)r) + ")");
   return m;
 }
@@ -1495,16 +1496,16 @@ void loss_forward(const T* q, const T* bank, const int64_t* target, int64_t n, i
 
 // The gradient of the logits exists one piece of the bank at a time, 16-bit values [n, piece] of at most
 // kPieceBytes.  Pieces that stay in L2 (64 MB) cost more in short kernels than the traffic they save:
-// 8,192 queries x 200,000 rows x 256, the three products of the backward pass: 3.4 ms in pieces of 64 MB,
-// 3.1 of 128, 2.75 of 256, 2.66 of 512, 2.54 of 1,024.
-constexpr int64_t kPieceBytes = 512ll << 20;
+// 8,192 queries x 200,000 rows x 256, the three products of the backward pass and the adding: 2.71 ms in
+// pieces of 256 MB, 2.49 of 512, 2.41 of 640, 2.42 of 1,024, 2.46 of 2,048 (3.6 of 64 with an earlier
+// kernel).
+constexpr int64_t kPieceBytes = 640ll << 20;
 int64_t piece_columns(int64_t n, int64_t v)
 {
   const int64_t most = std::max<int64_t>(1, kPieceBytes / (2 * n) / 256);  // in tiles of 256 columns
-  // whole rounds of the SM pairs for the bank's gradient, where a piece holds one
+  // whole rounds of the SM pairs for the bank's gradient, where a piece holds one; the last piece is shorter
   const int64_t pairs = sm_count() / 2, whole = most >= pairs ? most / pairs * pairs : most;
-  const int64_t tiles = ceil_div(v, 256);
-  return ceil_div(tiles, ceil_div(tiles, whole)) * 256;
+  return std::min(whole, ceil_div(v, 256)) * 256;
 }
 
 template <typename T>
