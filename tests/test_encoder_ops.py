@@ -284,6 +284,16 @@ def test_linear_many_rows(m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("m,k,n", [(2048, 24, 4100), (2100, 40, 4104), (5000, 700, 904), (9000, 520, 72), (3000, 1500, 1480)])
+def test_linear_sums_over_uneven_tiles(m, k, n, act):
+    """Weight gradients whose k-blocks the CTAs share unevenly, and bias sums of columns with fewer tiles
+    than there are CTAs."""
+    x, w, b, _, g = linear_inputs(m, k, n, F16, seed=m + k)
+    linear_check(x, w, b, None, act, g * 0.05)
+
+
+@pytest.mark.gpu
 def test_linear_without_bias_and_with_few_gradients():
     x, w, _, _, g = linear_inputs(200, 48, 80, BF16)
     linear_check(x, w, None, None, "gelu", g)
@@ -718,7 +728,7 @@ def test_operators_together_as_an_encoder_block():
     want_e = torch.nn.functional.normalize(y.mean(1), dim=-1)
     want = plain_loss(want_e, rp["bank"], target, 10.0)
     want_grads = torch.autograd.grad(want, ref, g.double())
-    rel = lambda a, b: float((a.double() - b).norm() / b.norm())  # noqa: E731
+    rel = lambda a, b: float((a.detach().double() - b.detach()).norm() / b.detach().norm())  # noqa: E731
     assert rel(e, want_e.detach()) <= 16 * u(dt)
     assert rel(loss, want.detach()) <= 16 * u(dt)
     for name, a, b in zip(["x"] + list(p), grads, want_grads):
@@ -759,6 +769,77 @@ def test_captured_training_step_replays_on_new_inputs():
         torch.cuda.synchronize()
         for out in outs:
             assert all(torch.equal(a, b) for a, b in zip(out, want))
+    check_device()
+
+
+@pytest.mark.gpu
+def test_capture_beside_a_living_eager_graph():
+    """A step is captured while an eager graph of the same leaves waits for its backward pass; both give
+    the gradients of a plain step.  (Autograd ties a leaf to the stream that its living graph was made
+    on, so the capture takes that stream.)"""
+    o, dt = ops(), F16
+    p = block_params(64, 128, 300, dt, seed=5)
+    x = torch.randn(6, 20, 64, device="cuda").to(dt)
+    target = torch.randint(0, 300, (6,), device="cuda")
+    leaves = list(p.values())
+    forward = lambda: encoder_block(o, x, p, lambda *a: o.softmax_loss(*a)[0], target, 10.0)[0]  # noqa: E731
+    backward = lambda loss: torch.autograd.grad(loss, leaves, torch.full_like(loss, 64.0))  # noqa: E731
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(s):
+        want = backward(forward())
+        waiting = forward()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=s):
+            got = backward(forward())
+        graph.replay()
+        late = backward(waiting)
+    torch.cuda.synchronize()
+    for a, b, c in zip(want, got, late):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    check_device()
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Matrices of more than 2^31 values: rows at both ends equal those of small calls, bit for bit."""
+    o = ops()
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    m, k, n = 2_200_011, 16, 1000
+    x = torch.randn((m, k), generator=gen, device="cuda").to(F16)
+    w, b = torch.randn((n, k), generator=gen, device="cuda").to(F16), torch.randn(n, generator=gen, device="cuda").to(F16)
+    y = o.linear(x, w, b, None, "gelu")
+    assert y.numel() > 2 ** 31
+    for a in (0, m - 300):
+        assert torch.equal(y[a:a + 300], o.linear(x[a:a + 300], w, b, None, "gelu"))
+    wn = torch.ones(n, dtype=F16, device="cuda")
+    z, mean, rstd = o.layer_norm(y, wn, wn)
+    for a in (0, m - 300):
+        assert torch.equal(z[a:a + 300], o.layer_norm(y[a:a + 300], wn, wn)[0])
+    dx, _, _ = o.layer_norm_backward(z, y, wn, mean, rstd, True, True, True)
+    part = slice(m - 300, m)
+    assert torch.equal(dx[part], o.layer_norm_backward(z[part], y[part], wn, mean[part], rstd[part], True, False, False)[0])
+    del z, dx
+    gx, _, _ = o.linear_backward(y, x, w, b, "relu", True, True, True)
+    assert torch.equal(gx[part], o.linear_backward(y[part], x[part], w, b, "relu", True, False, False)[0])
+    del gx, y, x
+    torch.cuda.empty_cache()
+    bank = torch.zeros((8_500_003, 256), dtype=BF16, device="cuda")  # all logits 0 but the last row's
+    bank[-1, :8] = 1.0
+    q = torch.zeros((5, 256), dtype=BF16, device="cuda")
+    q[:, 0] = torch.arange(5, device="cuda").to(BF16)
+    target = torch.tensor([8_500_002, 8_500_002, 8_500_002, 0, 8_500_002], device="cuda")
+    loss, lse = o.softmax_loss(q, bank, target, 1.0)
+    want = torch.log(torch.exp(torch.arange(5.0, dtype=torch.float64)) + 8_500_002)
+    assert torch.allclose(lse.double().cpu(), want, rtol=1e-6)
+    assert torch.allclose(loss.double().cpu(), want - torch.tensor([0.0, 1.0, 2.0, 0.0, 4.0], dtype=torch.float64), rtol=1e-6)
+    dq, dbank = o.softmax_loss_backward(torch.ones(5, device="cuda"), q, bank, target, loss, lse, 1.0, True, True)
+    p = torch.exp(torch.arange(5.0, dtype=torch.float64) - want)  # of the last row
+    for d in range(8):
+        assert torch.allclose(dq[[0, 1, 2, 4], d].double().cpu(), (p - 1)[[0, 1, 2, 4]], rtol=2 ** -7)
+    last = ((p - torch.tensor([1.0, 1.0, 1.0, 0.0, 1.0])) * torch.arange(5.0, dtype=torch.float64)).sum()
+    assert abs(float(dbank[-1, 0]) - float(last)) <= 2 ** -7 * abs(float(last))
     check_device()
 
 
