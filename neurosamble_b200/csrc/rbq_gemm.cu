@@ -213,6 +213,13 @@ __device__ __forceinline__ bool op_wait(uint32_t bar, uint32_t parity, volatile 
   return false;
 }
 
+// Bounded wait for copies or MMAs in flight after a failure.
+__device__ __forceinline__ void op_drain(uint32_t bar, uint32_t parity)
+{
+  volatile int never = 0;
+  op_wait(bar, parity, &never);
+}
+
 __device__ __forceinline__ void fail_with(volatile int* fail, int code)
 {
   *fail = 1;
@@ -545,7 +552,7 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
         if (st == 0) st = S::kStages, lap ^= 1;
         --st;
         if (!*fail && !op_wait(smem_u32(&s_empty[st]), lap, fail)) fail_with(fail, 6);
-        if (*fail && rank == 0) mbar_wait(smem_u32(&s_full[st]), lap);
+        if (*fail && rank == 0) op_drain(smem_u32(&s_full[st]), lap);
       }
     }
     __syncwarp();
@@ -588,7 +595,7 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
       // MMAs still running after a failure end before TMEM is freed: the last commit follows them.
       if (*fail && any) {
         if (st == 0) st = S::kStages, lap ^= 1;
-        mbar_wait(smem_u32(&s_empty[st - 1]), lap);
+        op_drain(smem_u32(&s_empty[st - 1]), lap);
       }
     }
     __syncwarp();
@@ -891,7 +898,7 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
     if (leader) {
       // after a failure: extra inputs in flight land before the shared memory goes away
       if (S::kBufs > 0 && *fail && loaded > 0)
-        for (int k = (loaded > S::kBufs ? loaded - S::kBufs : 0); k < loaded; ++k) mbar_wait(bar_of(k), parity_of(k));
+        for (int k = (loaded > S::kBufs ? loaded - S::kBufs : 0); k < loaded; ++k) op_drain(bar_of(k), parity_of(k));
       asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1148,7 +1155,7 @@ __global__ void __launch_bounds__(1024) grad_top_kernel(const float* __restrict_
       if (sum < least) least = sum, factor = 1.0f - (float)k / (2 * kScaleTries);
     }
     out[0] = top;
-    out[1] = top * scale / (kGradScale * factor);
+    out[1] = top * (scale / (kGradScale * factor));
     out[2] = kGradScale * factor;
   }
 }
