@@ -381,7 +381,7 @@ int rbq_merge_result_keys(const uint64_t* keys_dev, int32_t parts, int64_t nq, i
 
 /* y [m, n] = act(x [m, k] w [n, k]^T + bias [n]) + residual [m, n]; bias and residual may be NULL.
  * dtype RBQ_F16 or RBQ_BF16 for every matrix; products are summed in fp32 and y is rounded once.
- * m < 2^31 - 128.  Replaces CustomLinearFn / MyLinear (src/neurosamble/kernels/layers.py:23-75)
+ * m < 2^31 - 256.  Replaces CustomLinearFn / MyLinear (src/neurosamble/kernels/layers.py:23-75)
  * and the encoder's nn.Linear + activation + residual sums (model/signal_encoder.py:51-180). */
 int rbq_linear_workspace(int64_t m, int32_t k, int32_t n, int32_t dtype, int32_t act, int32_t backward, int64_t* bytes);
 int rbq_linear(const void* x_dev, const void* w_dev, const void* bias_dev, const void* residual_dev, void* y_dev, int64_t m,

@@ -2534,7 +2534,7 @@ void check_linear(int64_t m, int32_t k, int32_t n, int32_t dtype, int32_t act)
 {
   check_type(dtype, false);
   RBQ_CHECK(act == RBQ_ACT_NONE || act == RBQ_ACT_RELU || act == RBQ_ACT_GELU, RBQ_ERR_INVALID, "unknown activation");
-  RBQ_CHECK(m >= 0 && m < (1ll << 31) - 128 && k >= 1 && n >= 1 && k <= (1 << 24) && n <= (1 << 24), RBQ_ERR_INVALID,
+  RBQ_CHECK(m >= 0 && m < (1ll << 31) - 256 && k >= 1 && n >= 1 && k <= (1 << 24) && n <= (1 << 24), RBQ_ERR_INVALID,
             "linear: bad sizes");
 }
 void check_norm(int64_t rows, int32_t d)
@@ -2550,7 +2550,7 @@ void check_norm_types(int32_t dtype, int32_t param_dtype)
 void check_loss(int64_t n, int64_t v, int32_t d, int32_t dtype)
 {
   check_type(dtype, false);
-  RBQ_CHECK(n >= 0 && n < (1ll << 31) - 128 && v >= 1 && v < (1ll << 31) - 256 && d >= 1 && d <= (1 << 20),
+  RBQ_CHECK(n >= 0 && n < (1ll << 31) - 256 && v >= 1 && v < (1ll << 31) - 256 && d >= 1 && d <= (1 << 20),
             RBQ_ERR_INVALID, "softmax loss: bad sizes");
 }
 void check_scale(float scale)
