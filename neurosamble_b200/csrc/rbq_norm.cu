@@ -12,8 +12,8 @@
 // the gradients do not depend on timing.  All sums are fp32; the values are rounded once, on output.
 // Rows wider than the register paths hold take loops that read the row once per pass.
 //
-// Measured on one B200: forward 819,200 x 256 fp16 152 us (5.5 TB/s, 0.84 of a plain copy's rate); backward
-// 204,800 x 256 bf16 73 us (4.3 TB/s), its sums' second kernel 4; 5,003 x 771 fp32 9 and 10 us.
+// Measured on one B200: forward 819,200 x 256 fp16 127 us (6.6 TB/s, a plain copy's rate); backward
+// 204,800 x 256 bf16 71 us (4.4 TB/s), its sums' second kernel 4; 5,003 x 771 fp32 9 and 10 us.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -58,6 +58,42 @@ __device__ __forceinline__ void unpack(const Vec<T, VEC>& x, float (&v)[VEC])
 #pragma unroll
   for (int i = 0; i < VEC; ++i) v[i] = to_f(x.e[i]);
 }
+// A thread's own ring of row pieces in shared memory, filled by asynchronous 16-byte copies.  A thread
+// reads only what it copied itself, so waiting for its copies is all the order that is needed; rows
+// outside the matrix are filled with zeros.  The bytes on their way cost no registers.
+template <typename T, int VEC, int CH, int TPR, int DEPTH>
+struct RowRing {
+  uint4 (*slot)[kNormThreads];  // [DEPTH * CH]
+  const T* p;
+  int64_t rows;
+  int d, i;
+  __device__ __forceinline__ void ask(int64_t r, int stage) const
+  {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int col = (c * TPR + i) * VEC;
+      const bool in = r < rows && col < d;
+      const uint32_t dst = (uint32_t)__cvta_generic_to_shared(&slot[stage * CH + c][threadIdx.x]);
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(in ? p + r * d + col : p), "r"(in ? 16 : 0)
+                   : "memory");
+    }
+  }
+  __device__ __forceinline__ void take(int stage, float (&v)[CH][VEC]) const
+  {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const uint4 raw = slot[stage * CH + c][threadIdx.x];
+      unpack<T, VEC>(*reinterpret_cast<const Vec<T, VEC>*>(&raw), v[c]);
+    }
+  }
+};
+__device__ __forceinline__ void ring_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void ring_wait()
+{
+  asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
 // Keeps x packed: the compiler would unpack loop-invariant values once and hold twice the registers.
 template <typename T, int VEC>
 __device__ __forceinline__ void keep_packed(Vec<T, VEC>& x)
@@ -134,8 +170,24 @@ __global__ void __launch_bounds__(kNormThreads)
   const int i = threadIdx.x % TPR;
   const float fd = (float)d, inv_d = 1.0f / fd;
   const int64_t step = (int64_t)gridDim.x * kRows;
-  Vec<T, VEC> next[CH];  // the thread's next row is on its way while this one is worked on
-  fetch<T, VEC, CH, TPR>(x, (int64_t)blockIdx.x * kRows + threadIdx.x / TPR, rows, d, i, next);
+  // Rows on their way while one is worked on: kDepth - 1 in the ring, one in registers where the pieces are not
+  // of 16 bytes or too many.
+  constexpr bool kRing = VEC * sizeof(T) == 16 && CH <= 2;
+  constexpr int kDepth = 4;
+  __shared__ uint4 s_ring[kRing ? kDepth * CH : 1][kRing ? kNormThreads : 1];
+  const RowRing<T, VEC, CH, TPR, kDepth> ring{reinterpret_cast<uint4(*)[kNormThreads]>(s_ring), x, rows, d, i};
+  const int64_t mine = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+  int stage = 0;
+  Vec<T, VEC> next[CH];
+  if (kRing) {
+#pragma unroll
+    for (int k = 0; k < kDepth - 1; ++k) {
+      ring.ask(mine + k * step, k);
+      ring_commit();
+    }
+  } else {
+    fetch<T, VEC, CH, TPR>(x, mine, rows, d, i, next);
+  }
   Vec<P, VEC> wv[CH], bv[CH];
   if (kHold) {
     fetch<P, VEC, CH, TPR>(w, 0, 1, d, i, wv);
@@ -147,13 +199,21 @@ __global__ void __launch_bounds__(kNormThreads)
     const bool live = r < rows;
     float v[CH][VEC];
     float sum = 0.0f;
+    if (kRing) {
+      ring.ask(r + (kDepth - 1) * step, (stage + kDepth - 1) % kDepth);
+      ring_commit();
+      ring_wait<kDepth - 1>();
+      ring.take(stage, v);
+      stage = (stage + 1) % kDepth;
+    } else {
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      unpack<T, VEC>(next[c], v[c]);
+      for (int c = 0; c < CH; ++c) unpack<T, VEC>(next[c], v[c]);
+      fetch<T, VEC, CH, TPR>(x, r + step, rows, d, i, next);
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) sum += v[c][e];
-    }
-    fetch<T, VEC, CH, TPR>(x, r + step, rows, d, i, next);
     const float mean = over(row_sum<TPR>(sum, s_red), fd, inv_d);
     float sq = 0.0f;
 #pragma unroll
@@ -193,10 +253,11 @@ __global__ void __launch_bounds__(kNormThreads)
       }
     }
   }
+  if (kRing) ring_wait<0>();
 }
 
-// part[block][2][d]: this block's share of dw and db.  More warps hide the loads better here than a row
-// fetched ahead, which takes 16 registers: 204,800 rows of 256, 73 against 77 us.
+// part[block][2][d]: this block's share of dw and db.  Rows on their way lie in shared memory: in
+// registers they cost a quarter of the warps (204,800 rows of 256: 71 us, 77 that way, 73 with none ahead).
 template <typename T, typename P, int VEC, int CH, int TPR>
 __global__ void __launch_bounds__(kNormThreads, CH * VEC <= 8 ? 4 : 1)
     norm_grad_kernel(const T* __restrict__ g, const T* __restrict__ x, const P* __restrict__ w,
@@ -217,19 +278,48 @@ __global__ void __launch_bounds__(kNormThreads, CH * VEC <= 8 ? 4 : 1)
     for (int e = 0; e < VEC; ++e) dw[c][e] = db[c][e] = 0.0f;
   Vec<P, VEC> wv[CH];
   if (kHold) fetch<P, VEC, CH, TPR>(w, 0, 1, d, i, wv);
+  constexpr bool kRing = VEC * sizeof(T) == 16 && CH <= 2;
+  constexpr int kDepth = 4 / (CH <= 2 ? CH : 2);
+  __shared__ uint4 s_ring[kRing ? 2 * kDepth * CH : 1][kRing ? kNormThreads : 1];
+  uint4(*ring_slots)[kNormThreads] = reinterpret_cast<uint4(*)[kNormThreads]>(s_ring);
+  const RowRing<T, VEC, CH, TPR, kDepth> ring_x{ring_slots, x, rows, d, i}, ring_g{ring_slots + kDepth * CH, g, rows, d, i};
+  const int64_t mine = (int64_t)blockIdx.x * kRows + group;
+  int stage = 0;
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  if (kRing) {
+#pragma unroll
+    for (int k = 0; k < kDepth - 1; ++k) {
+      ring_x.ask(mine + k * step, k);
+      ring_g.ask(mine + k * step, k);
+      ring_commit();
+    }
+    if (mine < rows) next_mean = __ldg(mean_in + mine), next_rstd = __ldg(rstd_in + mine);
+  }
   for (int64_t r0 = (int64_t)blockIdx.x * kRows; r0 < rows; r0 += step) {
     const int64_t r = r0 + group;
     const bool live = r < rows;
-    const float mean = live ? __ldg(mean_in + r) : 0.0f, rstd = live ? __ldg(rstd_in + r) : 0.0f;
-    Vec<T, VEC> xr[CH], gr[CH];
-    fetch<T, VEC, CH, TPR>(x, r, rows, d, i, xr);
-    fetch<T, VEC, CH, TPR>(g, r, rows, d, i, gr);
-    float xh[CH][VEC], gw[CH][VEC];
+    float mean, rstd, xh[CH][VEC], gw[CH][VEC];
     float a = 0.0f, b = 0.0f;
+    if (kRing) {
+      ring_x.ask(r + (kDepth - 1) * step, (stage + kDepth - 1) % kDepth);
+      ring_g.ask(r + (kDepth - 1) * step, (stage + kDepth - 1) % kDepth);
+      ring_commit();
+      mean = next_mean, rstd = next_rstd;
+      if (r + step < rows) next_mean = __ldg(mean_in + r + step), next_rstd = __ldg(rstd_in + r + step);
+      ring_wait<kDepth - 1>();
+      ring_x.take(stage, xh);
+      ring_g.take(stage, gw);
+      stage = (stage + 1) % kDepth;
+    } else {
+      mean = live ? __ldg(mean_in + r) : 0.0f, rstd = live ? __ldg(rstd_in + r) : 0.0f;
+      Vec<T, VEC> xr[CH], gr[CH];
+      fetch<T, VEC, CH, TPR>(x, r, rows, d, i, xr);
+      fetch<T, VEC, CH, TPR>(g, r, rows, d, i, gr);
 #pragma unroll
-    for (int c = 0; c < CH; ++c) {
-      unpack<T, VEC>(xr[c], xh[c]);
-      unpack<T, VEC>(gr[c], gw[c]);
+      for (int c = 0; c < CH; ++c) {
+        unpack<T, VEC>(xr[c], xh[c]);
+        unpack<T, VEC>(gr[c], gw[c]);
+      }
     }
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
@@ -269,6 +359,7 @@ __global__ void __launch_bounds__(kNormThreads, CH * VEC <= 8 ? 4 : 1)
       }
     }
   }
+  if (kRing) ring_wait<0>();
   if (part == nullptr) return;
   float* out = part + (int64_t)blockIdx.x * 2 * d;
   if (TPR < 32) {  // the warp's rows
@@ -447,22 +538,26 @@ Plan plan_of(int d, int esize, bool vector, bool backward)
 }
 
 // Blocks of a kernel that runs over its rows in rounds: those that an SM holds at once (kMostBlocks at
-// most), so that no block waits for another's end, and no more than there are rows for.
-constexpr int kMostBlocks = 8;
+// most), and no more than there are rows for.  With `rounds` there are as many times that many as leave
+// each block about so many rounds: SMs get through memory traffic at different rates, and blocks that start
+// as others end even that out (forward pass, 819,200 x 256: 159 us in one wave, 127 in 16).  The backward
+// pass writes sums for every block and gains nothing (71 us, 72 in two waves).
+constexpr int kMostBlocks = 8, kRounds = 6;
 template <typename T, typename P, int VEC, int CH, int TPR, int PASS>
 struct Kernel;  // names a kernel
 template <typename Name, typename K>
-int blocks_for(K kernel, size_t smem, int64_t rows, int tpr)
+int blocks_for(K kernel, size_t smem, int64_t rows, int tpr, int rounds)
 {
-  static std::atomic<int> per_sm{0};  // one for every Name
+  static std::atomic<int> per_sm{0};  // one for every Name; smem is that of its widest rows
   int n = per_sm.load();
   if (n == 0) {
     RBQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kNormThreads, smem));
     n = std::max(1, std::min(n, kMostBlocks));
     per_sm.store(n);
   }
-  const int64_t per = kNormThreads / tpr;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(rows, per), (int64_t)sms() * n));
+  const int64_t work = ceil_div(rows, kNormThreads / tpr), wave = (int64_t)sms() * n;
+  const int64_t waves = rounds > 0 ? std::max<int64_t>(1, std::min<int64_t>(64, work / (wave * rounds))) : 1;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(work, wave * waves));
 }
 
 template <typename T, typename P>
@@ -473,7 +568,7 @@ void run_forward(const T* x, const P* w, const P* b, T* y, float* mean, float* r
   constexpr int V = 16 / (int)sizeof(T);
 #define RBQ_NORM(VEC, CH, TPR)                                                                                      \
   norm_kernel<T, P, VEC, CH, TPR>                                                                                   \
-      <<<blocks_for<Kernel<T, P, VEC, CH, TPR, 0>>(norm_kernel<T, P, VEC, CH, TPR>, 0, rows, TPR), kNormThreads, 0, \
+      <<<blocks_for<Kernel<T, P, VEC, CH, TPR, 0>>(norm_kernel<T, P, VEC, CH, TPR>, 0, rows, TPR, kRounds), kNormThreads, 0, \
          s>>>(x, w, b, y, mean, rstd, rows, d, eps)
   if (p.tpr == 0)
     norm_wide_kernel<T, P><<<(unsigned)std::min<int64_t>(rows, (int64_t)sms() * kMostBlocks), kNormThreads, 0, s>>>(
@@ -507,7 +602,8 @@ void run_backward(const T* g, const T* x, const P* w, const float* mean, const f
   float* out = sums ? part : nullptr;
   const size_t smem = sums && p.tpr && p.tpr < kNormThreads ? (size_t)2 * d * sizeof(float) : 0;
 #define RBQ_NORM(VEC, CH, TPR)                                                                                          \
-  (blocks = blocks_for<Kernel<T, P, VEC, CH, TPR, 1>>(norm_grad_kernel<T, P, VEC, CH, TPR>, smem, rows, TPR),            \
+  (blocks = blocks_for<Kernel<T, P, VEC, CH, TPR, 1>>(norm_grad_kernel<T, P, VEC, CH, TPR>,                              \
+                                                    TPR < kNormThreads ? 2 * sizeof(float) * CH * TPR * VEC : 0, rows, TPR, 0), \
    norm_grad_kernel<T, P, VEC, CH, TPR><<<blocks, kNormThreads, smem, s>>>(g, x, w, mean, rstd, dx, out, rows, d))
   if (p.tpr == 0) {
     if (dx != nullptr) {
