@@ -431,6 +431,14 @@ def test_layer_norm(rows, d, dt, pdt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt,pdt", [(F16, F32), (BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("d", [1000, 1023, 1025, 1953, 2048, 2049, 4095, 4096, 4104, 8192, 8200])
+def test_layer_norm_wide_rows_in_rounds(d, dt, pdt):
+    """Rows held by a whole block, of every number of loads per thread, and blocks that take several."""
+    norm_check(*norm_inputs(2999, d, dt, pdt, seed=d))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("d", [1, 2, 8])
 def test_layer_norm_rows_without_spread(d):
     """Equal values: variance 0, y = b, and a gradient of the size of 1 / sqrt(eps)."""
