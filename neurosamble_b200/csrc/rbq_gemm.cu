@@ -430,24 +430,40 @@ struct Shape {
   static_assert((2 * kStages + 4 + kGroups * 2) * 8 + 8 <= 256, "barriers");
 };
 
-// The warp's 32 staging rows <-> a matrix whose rows no TMA can address, 64 columns from `col`.
-template <typename T, bool LOAD>
-__device__ __forceinline__ void move_rows(unsigned char* buf, T* mat, int64_t row0, int64_t M, int64_t ld, int col, int N,
+// The warp's 32 staging rows <-> a matrix of 16-bit values whose rows no TMA can address, 64 columns from
+// `col`: a lane has columns lane and lane + 32, so that an access covers 64 bytes in a row.  BATCH rows are on
+// their way at a time: 200,000 x 300 -> 333 with a residual takes 278 us, row by row in pairs of columns 499.
+// Eight rows of loads gain 20 us there but cost the other products their registers (aligned GELU training 143
+// -> 151).  4-byte accesses, rows that start between them shifted over the lanes, were slower (495).
+template <bool LOAD, int BATCH>
+__device__ __forceinline__ void move_rows(unsigned char* buf, void* mat, int64_t row0, int64_t M, int64_t ld, int col, int N,
                                           int warp_row, int lane)
 {
-#pragma unroll 4
-  for (int r = 0; r < 32; ++r) {
-    const int row = warp_row + r;
-    if (row0 + row >= M) break;
-    T* at = reinterpret_cast<T*>(buf + row * 128 + (((lane >> 2) ^ (row & 7)) << 4) + (lane & 3) * 4);
-    T* g = mat + (row0 + row) * ld + col + lane * 2;
-    const int left = N - col - lane * 2;
-    if (LOAD) {
-      at[0] = left > 0 ? g[0] : T(0.0f);
-      at[1] = left > 1 ? g[1] : T(0.0f);
-    } else {
-      if (left > 0) g[0] = at[0];
-      if (left > 1) g[1] = at[1];
+  const bool in0 = col + lane < N, in1 = col + lane + 32 < N;
+  uint16_t* g = reinterpret_cast<uint16_t*>(mat) + (row0 + warp_row) * ld + col + lane;
+#pragma unroll 1
+  for (int r0 = 0; r0 < 32; r0 += BATCH, g += BATCH * ld) {
+    const int row = warp_row + r0, rows = (int)min((int64_t)BATCH, M - row0 - row);
+    auto at = [&](int r, int half) {
+      return reinterpret_cast<uint16_t*>(buf + (row + r) * 128 + (((lane >> 3) + half * 4) ^ ((row + r) & 7)) * 16 +
+                                         (lane & 7) * 2);
+    };
+    uint16_t v[BATCH], w[BATCH];
+#pragma unroll
+    for (int r = 0; r < BATCH; ++r) {
+      const bool in = r < rows;
+      v[r] = LOAD ? (in && in0 ? g[r * ld] : 0) : *at(r, 0);
+      w[r] = LOAD ? (in && in1 ? g[r * ld + 32] : 0) : *at(r, 1);
+    }
+#pragma unroll
+    for (int r = 0; r < BATCH; ++r) {
+      if (LOAD) {
+        *at(r, 0) = v[r];
+        *at(r, 1) = w[r];
+      } else if (r < rows) {
+        if (in0) g[r * ld] = v[r];
+        if (in1) g[r * ld + 32] = w[r];
+      }
     }
   }
 }
@@ -798,8 +814,8 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
         }
         if (kElement && a.has_extra) {
           if (!dead)
-            move_rows<T, true>(buf, reinterpret_cast<T*>(const_cast<void*>(a.extra)), m0, a.M, a.ld_extra, n0, a.N,
-                               quarter * 32, lane);
+            move_rows<true, 4>(buf, const_cast<void*>(a.extra), m0, a.M, a.ld_extra, n0, a.N, quarter * 32,
+                               lane);
           __syncwarp();
         }
       }
@@ -889,7 +905,7 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
         }
       } else {
         __syncwarp();
-        if (!dead) move_rows<T, false>(buf, reinterpret_cast<T*>(a.out), m0, a.M, a.ld_out, n0, a.N, quarter * 32, lane);
+        if (!dead) move_rows<false, 8>(buf, a.out, m0, a.M, a.ld_out, n0, a.N, quarter * 32, lane);
         group_sync(wg);
       }
       ++c;
