@@ -897,7 +897,12 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         group_sync(wg);
         if (leader && !dead && !*fail) {
-          if (m0 < a.M) tma_store_2d(&tmO, smem_u32(buf), n0, (int)m0);  // a pair's second half may lie past the last row
+          // A pair's second half may lie past the last row: an empty group then, since the waits above count
+          // one group per tile and would else take this tile's for that of the tile before.
+          if (m0 < a.M)
+            tma_store_2d(&tmO, smem_u32(buf), n0, (int)m0);
+          else
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           if (S::kBufs == 1 && extra_tma) {
             asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
             ask_extra();
