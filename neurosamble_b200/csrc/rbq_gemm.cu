@@ -1124,11 +1124,12 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(const float2* __restric
   }
 }
 
-// Largest |g| of the rows that take part, and the scale of the logits' gradient: kGradScale times one
+// Largest finite |g| of the rows that take part (1 if all are 0), and the scale of the logits' gradient: kGradScale times one
 // of eight factors in (1/2, 1].  A row's gradient is mostly its target's entry, so its rounding does
 // not average out the way the others' do; rows that have learnt about as much have entries of about
 // one mantissa, and a factor that moves it up towards the next power of two halves the rounding.  The
-// factor is the one with the least squared rounding of the target's entries over the first rows.
+// factor is the one with the least squared rounding of the target's entries over the first rows.  A row whose g
+// is infinite or NaN has a weight that is: its own gradient and the bank's are lost, the other rows' are not.
 constexpr int kScaleTries = 8;
 constexpr int64_t kScaleRows = 16384;
 template <typename T>
@@ -1141,18 +1142,19 @@ __global__ void __launch_bounds__(1024) grad_top_kernel(const float* __restrict_
   float top = 0.0f;
   for (int64_t i = threadIdx.x; i < n; i += 1024) {
     const int64_t t = target[i];
-    if (t >= 0 && t < v) top = fmaxf(top, fabsf(g[i]));
+    if (t >= 0 && t < v && isfinite(g[i])) top = fmaxf(top, fabsf(g[i]));
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   if (lane == 0) s_red[warp][0] = top;
   __syncthreads();
   for (int w = 0; w < 32; ++w) top = fmaxf(top, s_red[w][0]);
+  if (top == 0.0f) top = 1.0f;
   __syncthreads();
   float err[kScaleTries] = {};
   for (int64_t i = threadIdx.x; i < n && i < kScaleRows; i += 1024) {
     const int64_t t = target[i];
-    if (t < 0 || t >= v || g[i] == 0.0f) continue;
+    if (t < 0 || t >= v || g[i] == 0.0f || !isfinite(g[i])) continue;
     const float at = expm1f(-loss[i]) * (g[i] / top * kGradScale);
 #pragma unroll
     for (int k = 0; k < kScaleTries; ++k) {

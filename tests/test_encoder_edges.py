@@ -3,7 +3,7 @@ bits and the tolerances are those of that file."""
 import pytest
 import torch
 
-from test_encoder_ops import BF16, F16, check_device, linear_check, linear_inputs, ops
+from test_encoder_ops import BF16, F16, check_device, linear_check, linear_inputs, loss_inputs, ops
 
 
 @pytest.mark.gpu
@@ -18,4 +18,34 @@ def test_gradient_of_odd_widths_whose_last_tile_is_half_empty(m, k, n, act):
     first = ops().linear_backward(g, x, w, b, act, True, True, True)
     for _ in range(20):
         assert all(torch.equal(p, q) for p, q in zip(first, ops().linear_backward(g, x, w, b, act, True, True, True)))
+    check_device()
+
+
+def loss_gradients(q, bank, target, g, scale=3.0):
+    leaves = [q.detach().clone().requires_grad_(), bank.detach().clone().requires_grad_()]
+    return torch.autograd.grad(ops().softmax_loss(*leaves, target, scale)[0], leaves, g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_softmax_loss_weight_that_is_not_finite(bad, dt):
+    """An infinite or NaN weight spoils its own row of dq and the bank's gradient, where the definition has
+    sums of infinities, and leaves the bits of every other row's dq."""
+    q, bank, target, g = loss_inputs(300, 500, 64, dt, ignored=0.1, seed=2)
+    target[7] = 30
+    g[7] = 0.0
+    want, _ = loss_gradients(q, bank, target, g)
+    g[7] = bad
+    dq, dbank = loss_gradients(q, bank, target, g)
+    keep = torch.arange(300, device="cuda") != 7
+    assert torch.equal(dq[keep], want[keep]) and want.isfinite().all()
+    assert dq[7].isnan().all() and not dbank.isfinite().any()
+    g.zero_()
+    g[7] = bad  # no finite weight but zeros
+    dq, _ = loss_gradients(q, bank, target, g)
+    assert not dq[keep].any() and dq[7].isnan().all()
+    target[7] = -1  # and one of a row that takes no part
+    dq, dbank = loss_gradients(q, bank, target, g)
+    assert not dq.any() and not dbank.any()
     check_device()
