@@ -940,16 +940,17 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
 // ---------------------------------------------------------------------------------------
 
 // Rows of `cols` 16-bit values -> rows `ld` apart (ld a multiple of 8, so that TMA can address them).  A thread
-// makes 16 bytes of the copy.
+// makes 16 bytes of the copy.  With `weights` (GradRows) a row of weight 0 is zeros in the copy, whatever it holds.
 __global__ void pad_rows_kernel(const uint16_t* __restrict__ src, int64_t rows, int cols, int ld,
-                                uint16_t* __restrict__ dst)
+                                uint16_t* __restrict__ dst, const float4* __restrict__ weights)
 {
   const int per = ld / 8;
   for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < rows; r += (int64_t)gridDim.x * blockDim.y) {
+    const bool kept = weights == nullptr || weights[r].y != 0.0f;
     for (int i = threadIdx.x; i < per; i += blockDim.x) {
       uint32_t v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = i * 8 + e < cols ? src[r * cols + i * 8 + e] : 0u;
+      for (int e = 0; e < 8; ++e) v[e] = kept && i * 8 + e < cols ? src[r * cols + i * 8 + e] : 0u;
       *reinterpret_cast<uint4*>(dst + r * ld + i * 8) =
           make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
     }
@@ -1334,14 +1335,14 @@ struct Carver {
   }
 };
 
-void pad_rows(const void* src, int64_t rows, int cols, int ld, void* dst, cudaStream_t s)
+void pad_rows(const void* src, int64_t rows, int cols, int ld, void* dst, const float4* weights, cudaStream_t s)
 {
   int x = 8;  // threads to a row
   while (x < 256 && x < ld / 8) x *= 2;
   const dim3 block(x, 256 / x);
   const int64_t blocks = std::min<int64_t>(ceil_div(rows, block.y), (int64_t)sm_count() * 16);
   pad_rows_kernel<<<(unsigned)blocks, block, 0, s>>>(static_cast<const uint16_t*>(src), rows, cols, ld,
-                                                     static_cast<uint16_t*>(dst));
+                                                     static_cast<uint16_t*>(dst), weights);
   RBQ_LAUNCHED();
 }
 
@@ -1351,7 +1352,7 @@ Matrix addressable(const void* p, int64_t rows, int cols, Carver& ws, bool run, 
   if (cols % 8 == 0) return Matrix{p, rows, cols, cols};
   const int ld = (int)round_up(cols, 8);
   uint16_t* copy = ws.take<uint16_t>(rows * ld);
-  if (run) pad_rows(p, rows, cols, ld, copy, s);
+  if (run) pad_rows(p, rows, cols, ld, copy, nullptr, s);
   return Matrix{copy, rows, cols, ld};
 }
 
@@ -1548,7 +1549,12 @@ template <typename T>
 void loss_backward(const float* g, const T* q, const T* bank, const int64_t* target, const float* loss, const float* lse,
                    int64_t n, int64_t v, int d, float scale, T* dq, T* dbank, Carver& ws, bool run, cudaStream_t s)
 {
-  const Matrix Q = addressable(q, n, d, ws, run, s), B = addressable(bank, v, d, ws, run, s);
+  // q with zeros in the rows that take no part: they meet zeros of the logits' gradient in the bank's sums, and
+  // zero times an infinity or NaN that such a row may hold (a batch's padding) would spoil every row of dbank.  It is
+  // the padded copy too where the width wants one.
+  const int ldq = (int)round_up(d, 8);
+  uint16_t* kept = ws.take<uint16_t>(n * ldq);
+  const Matrix Q{kept, n, d, ldq}, B = addressable(bank, v, d, ws, run, s);
   const int64_t piece = std::min(piece_columns(n, v), round_up(v, 8));
   float* top = ws.take<float>(3);
   float4* rows = ws.take<float4>(n);
@@ -1568,6 +1574,7 @@ void loss_backward(const float* g, const T* q, const T* bank, const int64_t* tar
   RBQ_LAUNCHED();
   grad_rows_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(g, target, loss, lse, n, v, top, rows);
   RBQ_LAUNCHED();
+  pad_rows(q, n, d, ldq, kept, rows, s);
   if (dq && pieces) RBQ_CUDA(cudaMemsetAsync(slabs_q, 0, pq.floats() * sizeof(float), s));
   for (int64_t v0 = 0; v0 < v; v0 += piece) {
     const int64_t cols = std::min(piece, v - v0);

@@ -49,3 +49,19 @@ def test_softmax_loss_weight_that_is_not_finite(bad, dt):
     dq, dbank = loss_gradients(q, bank, target, g)
     assert not dq.any() and not dbank.any()
     check_device()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("n,v,d", [(300, 500, 64), (70, 129, 33)])
+def test_softmax_loss_rows_that_take_no_part_hold_anything(n, v, d, dt):
+    """Infinities and NaN in the queries of ignored rows reach neither dq nor dbank."""
+    q, bank, target, g = loss_inputs(n, v, d, dt, ignored=0.0, seed=n)
+    target[5], target[6], target[n - 1] = -1, v, -100
+    want = loss_gradients(q, bank, target, g)
+    q[5], q[6, 3], q[n - 1] = float("nan"), float("inf"), -float("inf")
+    got = loss_gradients(q, bank, target, g)
+    assert all(a.isfinite().all() and torch.equal(a, b) for a, b in zip(want, got))
+    got = loss_gradients(q, bank, torch.full_like(target, -1), g)
+    assert not got[0].any() and not got[1].any()
+    check_device()
