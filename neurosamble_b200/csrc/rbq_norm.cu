@@ -147,11 +147,12 @@ __device__ __forceinline__ float row_sum(float v, float* s_red)
   return t;
 }
 
-// sum / d, rounded as a division would: one correction of the product with 1 / d.
+// sum / d, rounded as a division would: the product with the rounded 1 / d, corrected once by its residual
+// (Markstein's method).  An infinite sum has no residual (infinity - infinity) and stays as it is.
 __device__ __forceinline__ float over(float sum, float d, float inv_d)
 {
-  const float q = sum * inv_d;
-  return fmaf(fmaf(-q, d, sum), inv_d, q);
+  const float q = sum * inv_d, rest = fmaf(-q, d, sum);
+  return rest == rest ? fmaf(rest, inv_d, q) : q;
 }
 
 // TPR threads to a row; thread i of a row holds CH pieces of VEC values, piece c at column

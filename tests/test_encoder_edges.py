@@ -3,7 +3,7 @@ bits and the tolerances are those of that file."""
 import pytest
 import torch
 
-from test_encoder_ops import BF16, F16, check_device, linear_check, linear_inputs, loss_inputs, ops
+from test_encoder_ops import BF16, F16, F32, check_device, linear_check, linear_inputs, loss_inputs, ops
 
 
 @pytest.mark.gpu
@@ -65,3 +65,34 @@ def test_softmax_loss_rows_that_take_no_part_hold_anything(n, v, d, dt):
     got = loss_gradients(q, bank, torch.full_like(target, -1), g)
     assert not got[0].any() and not got[1].any()
     check_device()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16, F32])
+@pytest.mark.parametrize("d", [5, 8, 40, 256, 771, 2048, 5001, 8192, 40000])
+def test_layer_norm_rows_with_infinities(d, dt):
+    """mean and rstd of rows with an infinity, with two of either sign and with a NaN are those of the definition at
+    every width; the other rows keep their bits."""
+    x = torch.randn((9, d), device="cuda", generator=torch.Generator(device="cuda").manual_seed(d)).to(dt)
+    w, b = torch.full((d,), 2.0, dtype=dt, device="cuda"), torch.ones(d, dtype=dt, device="cuda")
+    plain = ops().layer_norm(x, w, b)
+    x[2, 1], x[3, 0], x[5, 1], x[5, 2], x[7, 3] = float("inf"), -float("inf"), float("inf"), -float("inf"), float("nan")
+    y, mean, rstd = ops().layer_norm(x, w, b)
+    keep = [0, 1, 4, 6, 8]
+    assert all(torch.equal(a[keep], c[keep]) for a, c in zip((y, mean, rstd), plain))
+    bad = [2, 3, 5, 7]
+    want = x.double().mean(1)[bad].float()
+    assert torch.equal(mean[bad].nan_to_num(7.0), want.nan_to_num(7.0)) and torch.equal(mean[bad].isnan(), want.isnan())
+    assert y[bad].isnan().all() and rstd[bad].isnan().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [8, 256, 771, 40000])
+def test_layer_norm_sums_that_overflow(d):
+    """Values whose squares add up to infinity in 32 bits: rstd is 0 and y = b, as in the formula in 32 bits."""
+    x = torch.randn((4, d), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1))
+    x[1] *= 1e25
+    w, b = torch.ones(d, device="cuda"), torch.arange(d, device="cuda") / d
+    y, mean, rstd = ops().layer_norm(x, w, b)
+    assert rstd[1] == 0 and torch.equal(y[1], b) and mean[1].isfinite()
+    assert y.isfinite().all() and (rstd[[0, 2, 3]] > 0).all()
