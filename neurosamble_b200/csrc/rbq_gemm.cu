@@ -25,7 +25,7 @@
 // that owns the rows.
 //
 // Measured on one B200 (CUDA time; cuBLAS alone on the same product in brackets, where taken): linear
-// 819,200 x 256 -> 1,024 in fp16 0.47 ms without, 0.64 with GELU (0.50; HBM floor 0.32); 819,200 x 1,024
+// 819,200 x 256 -> 1,024 in fp16 0.47 ms without, 0.66 with GELU (0.50; HBM floor 0.32); 819,200 x 1,024
 // -> 256 0.41 (0.39); 8,192^3 0.82 (0.70: its tiles are better ordered for L2).  Loss of 8,192 queries
 // against 200,000 x 256: forward 0.72 ms (1.17 PFLOP/s), backward 2.4 ms.  In loops of these the card
 // runs into its 1,000 W limit at 1.3 to 1.7 GHz.
@@ -283,12 +283,21 @@ __device__ __forceinline__ float max_nan(float a, float b)
   return r;
 }
 
-// GELU z Phi(z) = max(z, 0) - w Phi(-w) and its slope Phi(z) + z phi(z) = [z > 0] - sign(z) (Phi(-w) -
-// w phi(w)), w = |z|.  Both tails are e^{-w^2 / 2} times a smooth function of w, and that is a
-// polynomial here: minimax fits on [0, 6] of the products' absolute error (own fits, weighted by the
-// exponential), good to 8e-7 for the value and 4e-6 for the slope, which is rounded to 16 bits
-// at once.  Past w = 8 the exponential is below 2^-46.  With erff and expf the layer took 1.74 ms on
-// 819,200 x 256 -> 1,024, with these 0.94 in the same kernel.
+// GELU z Phi(z) = max(z, 0) - t(w), w = |z|, with the tail t(w) = w Phi(-w); its slope Phi(z) + z phi(z) is
+// s(w) = Phi(-w) - w phi(w) for z <= 0 and 1 - s(w) for z > 0.  Both are e^{-w^2 / 2} times a smooth function of w,
+// whose zeros are taken out as factors:
+//   t(w) = e^{-w^2 / 2} w P(w),   s(w) = e^{-w^2 / 2} (w0 - w) Q(w),   s(w0) = 0
+// so that polynomials for P and Q hold the relative error of the tails, which 16-bit outputs show to the last
+// bit (at z = -5 an absolute error of 8e-7 is half the value).  Own minimax fits by linear programming, in
+// powers of -w.  What they add to the one rounding of the output, in units of that: 0.16 (value) and 0.18 (slope) up
+// to w = 5; past it, in fp16, as much and 0.32 down to the subnormal values (a value is 0 from w = 6, and a
+// slope past 8 times any gradient); in bf16, whose exponents reach w = 13.1, 0.66 and 0.82.  Their absolute error
+// stays under 2e-6 (1 + w).  From w = 13.2 on the exponential is 0.
+// bf16's value is a constant times the exponential past 9.5 (true to 0.5 %), and takes powers of 4.75 - w: so
+// many terms in powers of w would cancel to nothing.
+// On one B200, 819,200 x 256 -> 1,024 in fp16: 660 us; polynomials for an absolute error of 8e-7, one term shorter,
+// 641; erff and expf 1.85 times as long as those.  The slope's kernel, 51,200 x 256 -> 1,024: 66 us, 61 with an
+// absolute error of 4e-6.
 __device__ __forceinline__ uint64_t gauss2(uint64_t z)  // e^{-z^2 / 2}
 {
   const float c = -0.72134752f;  // -log2(e) / 2
@@ -303,31 +312,55 @@ __device__ __forceinline__ uint64_t horner2(const float (&c)[N], uint64_t x)
   for (int i = N - 2; i >= 0; --i) r = fma2(r, x, pair(c[i], c[i]));
   return r;
 }
-template <int ACT>
+// (-w, -w) of two values, w at most `end`
+__device__ __forceinline__ uint64_t minus_abs(float2 v, float end)
+{
+  return pair(fmaxf(-fabsf(v.x), -end), fmaxf(-fabsf(v.y), -end));
+}
+template <typename T, int ACT>
 __device__ __forceinline__ float2 act_of(uint64_t z)
 {
   const float2 v = split(z);
   if (ACT == RBQ_ACT_RELU) return make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
   if (ACT == RBQ_ACT_GELU) {
-    // in -w, so that every coefficient is positive
-    const float c[9] = {0.499963641f,  0.398381382f,   0.247026116f,   0.125212014f,  0.050794214f,
-                        0.0154364463f, 0.00319635496f, 0.000392604211f, 2.12489049e-05f};
-    const uint64_t nw = pair(fmaxf(-fabsf(v.x), -8.0f), fmaxf(-fabsf(v.y), -8.0f));
-    return split(fma2(mul2(gauss2(z), nw), horner2(c, nw), pair(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f))));
+    uint64_t nw, p;
+    if (std::is_same<T, __half>::value) {
+      const float c[10] = {0.499972373f,  0.398479819f, 0.247432157f,   0.126111999f,   0.0520200133f,
+                           0.0164886173f, 0.0037531869f, 0.000565699709f, 4.99067755e-05f, 1.93591131e-06f};
+      nw = minus_abs(v, 6.0f);
+      p = horner2(c, nw);
+    } else {
+      const float c[12] = {0.0806254521f,    0.0157307144f,   0.00298358826f,  0.000617415411f,
+                           8.76739214e-05f,  -7.04420836e-06f, 5.34964329e-06f, 3.19636297e-06f,
+                           -1.65086874e-07f, -1.24640735e-07f, 1.01854436e-08f, 3.03623016e-09f};
+      nw = minus_abs(v, 9.5f);
+      p = horner2(c, add2(nw, pair(4.75f, 4.75f)));
+    }
+    return split(fma2(mul2(gauss2(z), nw), p, pair(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f))));
   }
   return v;
 }
-template <int ACT>
+template <typename T, int ACT>
 __device__ __forceinline__ float2 act_slope(uint64_t z)
 {
   const float2 v = split(z);
   if (ACT == RBQ_ACT_RELU)
     return make_float2(v.x > 0.0f ? 1.0f : (v.x != v.x ? v.x : 0.0f), v.y > 0.0f ? 1.0f : (v.y != v.y ? v.y : 0.0f));
   if (ACT == RBQ_ACT_GELU) {
-    const float c[8] = {0.499996036f,  0.797662377f,  0.247959644f,   0.125826955f,
-                        0.0499400385f, 0.013923605f, 0.00231907005f, 0.000168557366f};
-    const uint64_t nw = pair(fmaxf(-fabsf(v.x), -8.0f), fmaxf(-fabsf(v.y), -8.0f));
-    const float2 t = split(mul2(gauss2(z), horner2(c, nw)));
+    const float root = 0.751791525f;
+    uint64_t nw, p;
+    if (std::is_same<T, __half>::value) {
+      const float c[10] = {0.66507566f,    0.176510572f,   0.096318841f,    0.0434494428f,   0.015321183f,
+                           0.00392379053f, 0.00068282726f, 7.52700944e-05f, 4.69856604e-06f, 1.25869008e-07f};
+      nw = minus_abs(v, 8.0f);
+      p = horner2(c, nw);
+    } else {
+      const float c[11] = {0.66507411f,    0.176427275f,    0.095736444f,    0.0421805046f,   0.0141140036f,  0.0033448264f,
+                           0.000535338011f, 5.57655512e-05f, 3.59613659e-06f, 1.29842135e-07f, 2.00207539e-09f};
+      nw = minus_abs(v, 13.25f);
+      p = horner2(c, nw);
+    }
+    const float2 t = split(mul2(mul2(gauss2(z), add2(nw, pair(root, root))), p));
     return make_float2(v.x > 0.0f ? 1.0f - t.x : t.x, v.y > 0.0f ? 1.0f - t.y : t.y);
   }
   return make_float2(1.0f, 1.0f);
@@ -857,11 +890,11 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
             for (int e = 0; e < 4; ++e) {
               const uint64_t z = fma2(pair(o[2 * e], o[2 * e + 1]), al, b[e]);
               if (EPI == kEpiActGrad) {
-                const float2 f = act_slope<ACT>(z), g = Pack<T>::get(xs[e]);
+                const float2 f = act_slope<T, ACT>(z), g = Pack<T>::get(xs[e]);
                 o[2 * e] = g.x * f.x;
                 o[2 * e + 1] = g.y * f.y;
               } else {
-                const float2 f = act_of<ACT>(z);
+                const float2 f = act_of<T, ACT>(z);
                 o[2 * e] = f.x;
                 o[2 * e + 1] = f.y;
                 if (a.has_extra) {

@@ -1,9 +1,12 @@
 """Corners of the read encoder's operators that tests/test_encoder_ops.py does not reach; the definitions in 64
 bits and the tolerances are those of that file."""
+import math
+
 import pytest
 import torch
 
-from test_encoder_ops import BF16, F16, F32, check_device, linear_check, linear_inputs, loss_inputs, ops
+from test_encoder_ops import (BF16, F16, F32, check_device, linear_check, linear_inputs, loss_inputs, ops, tiny, u,
+                              within)
 
 
 @pytest.mark.gpu
@@ -96,3 +99,39 @@ def test_layer_norm_sums_that_overflow(d):
     y, mean, rstd = ops().layer_norm(x, w, b)
     assert rstd[1] == 0 and torch.equal(y[1], b) and mean[1].isfinite()
     assert y.isfinite().all() and (rstd[[0, 2, 3]] > 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_gelu_keeps_its_tails(dt):
+    """Value and slope of GELU at every 16-bit z in [-13.1, 13.1], through a one-wide layer whose products are
+    exact: two roundings of the result, one for the output's own and one for everything before it, down to
+    fp16's subnormal values (two of their roundings) and bf16's smallest normal value."""
+    z = torch.arange(-2 ** 15, 2 ** 15, device="cuda").to(torch.int16).view(dt)
+    z = z[z.double().abs() <= 13.1].sort().values[:, None]
+    leaf = z.clone().requires_grad_()
+    y = ops().linear(leaf, torch.ones(1, 1, dtype=dt, device="cuda"), None, None, "gelu")
+    dx, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    check_device()
+    z = z.double()
+    w = z.abs()
+    gauss, mills = torch.exp(-0.5 * w * w), 0.5 * torch.special.erfcx(w / math.sqrt(2))  # Phi(-w) = gauss * mills
+    tail, fall = gauss * mills * w, gauss * (mills - w / math.sqrt(2 * math.pi))
+    few = 2 * tiny(F16) if dt == F16 else torch.finfo(dt).smallest_normal
+    for got, want, name in ((y, torch.where(z > 0, z - tail, -tail), "y"),
+                            (dx, torch.where(z > 0, 1 - fall, fall), "slope")):
+        within(got, want, 2 * u(dt) * want.abs() + few, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16])
+def test_gelu_far_out(dt):
+    """Infinities, NaN and the types' largest values: z or 0, and a slope of 1 or 0."""
+    big = torch.finfo(dt).max
+    z = torch.tensor([float("inf"), big, 14.0, 100.0, -float("inf"), -big, -14.0, -100.0, float("nan"), 0.0], device="cuda")
+    z = z.to(dt)[:, None]
+    leaf = z.clone().requires_grad_()
+    y = ops().linear(leaf, torch.ones(1, 1, dtype=dt, device="cuda"), None, None, "gelu")
+    dx, = torch.autograd.grad(y, leaf, torch.ones_like(y))
+    assert torch.equal(y[:4], z[:4]) and not y[4:8].any() and y[8].isnan() and y[9] == 0
+    assert (dx[:4] == 1).all() and not dx[4:8].any() and dx[8].isnan() and dx[9] == 0.5
