@@ -95,6 +95,14 @@ bool wants_grad(std::initializer_list<Tensor> ts)
   return false;
 }
 
+// There are no forward-mode derivatives: an input that carries a tangent is refused, since the tangent would be
+// dropped below autograd (and taken as zero by the caller).
+void no_tangents(std::initializer_list<Tensor> ts, const char* name)
+{
+  for (const Tensor& t : ts)
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "rbq: ", name, " has no forward-mode derivative");
+}
+
 // An output whose own gradient is refused (the backward passes are not differentiable again).
 template <size_t N>
 std::array<Tensor, N> once(std::array<Tensor, N> out, const char* name)
@@ -232,6 +240,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow("rbq::linear_backward", "")
                          .typed<decltype(linear_backward_kernel)>();
+    no_tangents({grads[0]}, "linear's gradient");
     const auto saved = ctx->get_saved_variables();
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
     const bool has_bias = saved[2].defined(), nb = has_bias && ctx->needs_input_grad(2);
@@ -251,6 +260,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
 Tensor linear_autograd(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& residual,
                        c10::string_view act)
 {
+  no_tangents({x, w, bias.value_or(Tensor()), residual.value_or(Tensor())}, "linear");
   if (!wants_grad({x, w, bias.value_or(Tensor()), residual.value_or(Tensor())})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return linear_op().call(x, w, bias, residual, act);
@@ -351,6 +361,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads)
   {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    no_tangents({grads[0]}, "layer_norm's gradient");
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow("rbq::layer_norm_backward", "")
                          .typed<decltype(layer_norm_backward_kernel)>();
@@ -369,6 +380,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
 
 Three layer_norm_autograd(const Tensor& x, const Tensor& w, const Tensor& b, double eps)
 {
+  no_tangents({x, w, b}, "layer_norm");
   if (!wants_grad({x, w, b})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return layer_norm_op().call(x, w, b, eps);
@@ -468,6 +480,7 @@ struct SoftmaxLossFunction : torch::autograd::Function<SoftmaxLossFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads)
   {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    no_tangents({grads[0]}, "softmax_loss's gradient");
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow("rbq::softmax_loss_backward", "")
                          .typed<decltype(softmax_loss_backward_kernel)>();
@@ -486,6 +499,7 @@ struct SoftmaxLossFunction : torch::autograd::Function<SoftmaxLossFunction> {
 
 Two softmax_loss_autograd(const Tensor& q, const Tensor& bank, const Tensor& target, double scale)
 {
+  no_tangents({q, bank}, "softmax_loss");
   if (!wants_grad({q, bank})) {
     at::AutoDispatchBelowADInplaceOrView below;
     return softmax_loss_op().call(q, bank, target, scale);

@@ -27,6 +27,7 @@ softmax_loss take float16 or bfloat16, layer_norm also float32, with w and b of 
 float32.  A row of softmax_loss whose target lies outside [0, v) is ignored: loss 0, no
 gradient.  mean, rstd and lse carry no gradient; the backward passes (linear_backward,
 layer_norm_backward, softmax_loss_backward) are operators too and are not differentiable again.
+Forward-mode derivatives (dual tensors, torch.func.jvp) are refused.
 
 ``h`` is the index handle as an int (``IndexIVFRaBitQ.handle.value``).  ``query_bits`` of search
 is the search mode: 4 (QUANT4), 8 (QUANT8), 16 (LUT16) or 32 (LUT32); ``bits`` of query_prep is

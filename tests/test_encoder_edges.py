@@ -4,11 +4,45 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as fw
 
 from test_encoder_ops import (BF16, F16, F32, check_device, linear_check, linear_inputs, loss_inputs, ops, tiny, u,
                               within)
 
 
+def meta(*s, dt=F16):
+    return torch.empty(*s, dtype=dt, device="meta")
+
+
+def forwards():
+    """Each operator as a function of its differentiable inputs, with fake ones (on the CPU: shapes only)."""
+    o, t = ops(), meta(4, dt=torch.int64)
+    return [(lambda x, w, b, r: o.linear(x, w, b, r, "gelu"), [meta(4, 16), meta(8, 16), meta(8), meta(4, 8)]),
+            (lambda x, w, b: o.layer_norm(x, w, b)[0], [meta(4, 16), meta(16), meta(16)]),
+            (lambda q, k: o.softmax_loss(q, k, t, 2.0)[0], [meta(4, 16), meta(9, 16)])]
+
+
+# -- on the CPU -------------------------------------------------------------------------------------
+def test_forward_mode_derivatives_are_refused():
+    """A tangent on any input, with and without gradients, and one on the gradient that goes back."""
+    for call, args in forwards():
+        for i in range(len(args)):
+            for leaf in (False, True):
+                with fw.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                    primal = args[i].detach().clone().requires_grad_(leaf)
+                    call(*args[:i], fw.make_dual(primal, torch.empty_like(args[i])), *args[i + 1:])
+            with fw.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call(*args[:i], fw.make_dual(args[i], torch.empty_like(args[i])), *args[i + 1:])
+        with pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            torch.func.jvp(call, tuple(args), tuple(torch.empty_like(a) for a in args))
+        leaves = [a.detach().clone().requires_grad_() for a in args]
+        with fw.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+            y = call(*leaves)
+            torch.autograd.grad(y, leaves, fw.make_dual(torch.empty_like(y), torch.empty_like(y)))
+        assert call(*leaves).requires_grad  # plain calls go on
+
+
+# -- on the GPU -------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,k,n,act", [(20000, 64, 517, "gelu"), (13331, 40, 1279, "relu"), (40001, 24, 333, "gelu")])
 def test_gradient_of_odd_widths_whose_last_tile_is_half_empty(m, k, n, act):
