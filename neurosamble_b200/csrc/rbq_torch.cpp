@@ -103,19 +103,19 @@ void no_tangents(std::initializer_list<Tensor> ts, const char* name)
     TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "rbq: ", name, " has no forward-mode derivative");
 }
 
-// An output whose own gradient is refused (the backward passes are not differentiable again).
+// Outputs of a backward pass, whose own gradient is refused.  The refusal hangs on what the pass read, so that
+// every way back from the outputs to one of those meets it: from a node with no way on, autograd.grad with such an
+// input would skip it and take its part of the derivative as zero.
 template <size_t N>
-std::array<Tensor, N> once(std::array<Tensor, N> out, const char* name)
+std::array<Tensor, N> once(std::array<Tensor, N> out, const char* name, std::initializer_list<Tensor> read)
 {
-  if (!at::GradMode::is_enabled()) return out;
+  if (!wants_grad(read)) return out;
   variable_list in;
-  for (Tensor& t : out)
-    if (t.defined() && t.numel() > 0) {
-      t = t.detach();
-      t.requires_grad_();
-      in.push_back(t);
-    }
+  for (const Tensor& t : out)
+    if (t.defined() && t.numel() > 0) in.push_back(t.detach());
   if (in.empty()) return out;
+  for (const Tensor& t : read)
+    if (t.defined() && t.requires_grad()) in.push_back(t);
   auto fn = std::make_shared<torch::autograd::DelayedError>(
       std::string("rbq: the gradient of ") + name + " cannot be differentiated again", (int64_t)in.size());
   variable_list wrapped = (*fn)(std::move(in));
@@ -252,7 +252,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
                                   ctx->saved_data["act"].toStringRef(), nx, nw, nb);
       d = {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor()};
     }
-    d = once(std::move(d), "linear");
+    d = once(std::move(d), "linear", {grads[0], saved[0], saved[1], saved[2]});
     return {d[0], d[1], d[2], nr ? grads[0] : Tensor(), Tensor()};
   }
 };
@@ -373,7 +373,7 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
       auto [dx, dw, db] = op.call(grads[0], s[0], s[1], s[2], s[3], nx, nw, nb);
       d = {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor()};
     }
-    d = once(std::move(d), "layer_norm");
+    d = once(std::move(d), "layer_norm", {grads[0], s[0], s[1]});
     return {d[0], d[1], d[2], Tensor()};
   }
 };
@@ -492,7 +492,7 @@ struct SoftmaxLossFunction : torch::autograd::Function<SoftmaxLossFunction> {
       auto [dq, dbank] = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(), nq, nk);
       d = {nq ? dq : Tensor(), nk ? dbank : Tensor()};
     }
-    d = once(std::move(d), "softmax_loss");
+    d = once(std::move(d), "softmax_loss", {grads[0], s[0], s[1]});
     return {d[0], d[1], Tensor(), Tensor()};
   }
 };

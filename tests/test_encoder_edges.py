@@ -15,17 +15,18 @@ def meta(*s, dt=F16):
 
 
 def forwards():
-    """Each operator as a function of its differentiable inputs, with fake ones (on the CPU: shapes only)."""
+    """Each operator as a function of its differentiable inputs, with meta tensors for them (shapes only), and the
+    number of inputs that its gradients read."""
     o, t = ops(), meta(4, dt=torch.int64)
-    return [(lambda x, w, b, r: o.linear(x, w, b, r, "gelu"), [meta(4, 16), meta(8, 16), meta(8), meta(4, 8)]),
-            (lambda x, w, b: o.layer_norm(x, w, b)[0], [meta(4, 16), meta(16), meta(16)]),
-            (lambda q, k: o.softmax_loss(q, k, t, 2.0)[0], [meta(4, 16), meta(9, 16)])]
+    return [(lambda x, w, b, r: o.linear(x, w, b, r, "gelu"), [meta(4, 16), meta(8, 16), meta(8), meta(4, 8)], 3),
+            (lambda x, w, b: o.layer_norm(x, w, b)[0], [meta(4, 16), meta(16), meta(16)], 2),
+            (lambda q, k: o.softmax_loss(q, k, t, 2.0)[0], [meta(4, 16), meta(9, 16)], 2)]
 
 
 # -- on the CPU -------------------------------------------------------------------------------------
 def test_forward_mode_derivatives_are_refused():
     """A tangent on any input, with and without gradients, and one on the gradient that goes back."""
-    for call, args in forwards():
+    for call, args, _ in forwards():
         for i in range(len(args)):
             for leaf in (False, True):
                 with fw.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
@@ -40,6 +41,29 @@ def test_forward_mode_derivatives_are_refused():
             y = call(*leaves)
             torch.autograd.grad(y, leaves, fw.make_dual(torch.empty_like(y), torch.empty_like(y)))
         assert call(*leaves).requires_grad  # plain calls go on
+
+
+def test_second_derivatives_are_refused_on_every_way_back():
+    """From each gradient to each input and to the gradient that went back, alone and beside a term that can be
+    differentiated: no part of a second derivative is taken as zero."""
+    for call, args, read in forwards():
+        leaves = [a.detach().clone().requires_grad_() for a in args]
+        y = call(*leaves)
+        g = torch.empty_like(y).requires_grad_()
+        grads = torch.autograd.grad(y, leaves, g, create_graph=True)
+        if len(args) == 4:  # the residual's gradient is g itself
+            assert torch.autograd.grad(grads[3].sum(), g, retain_graph=True)[0].shape == g.shape
+            grads = grads[:3]
+        for d in grads:
+            assert d.requires_grad
+            for t in (*leaves[:read], g):
+                for out in (d.sum(), d.sum() + t.sum()):
+                    with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+                        torch.autograd.grad(out, t, retain_graph=True)
+            with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+                (d.sum() + leaves[0].sum()).backward(retain_graph=True)
+        plain = torch.autograd.grad(call(*leaves), leaves, g.detach())
+        assert not any(d.requires_grad for d in plain)
 
 
 # -- on the GPU -------------------------------------------------------------------------------------
