@@ -224,6 +224,29 @@ c10::TypedOperatorHandle<decltype(linear_kernel)>& linear_op()
   return op;
 }
 
+c10::TypedOperatorHandle<decltype(linear_backward_kernel)>& linear_backward_op()
+{
+  static auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("rbq::linear_backward", "").typed<decltype(linear_backward_kernel)>();
+  return op;
+}
+
+// Refuses forward-mode and second derivatives; LinearFunction's backward pass and direct calls come here.
+std::tuple<Tensor, Tensor, Tensor> linear_backward_autograd(const Tensor& g, const Tensor& x, const Tensor& w,
+                                                            const OptTensor& bias, c10::string_view act, bool need_x,
+                                                            bool need_w, bool need_bias)
+{
+  const Tensor b = bias.value_or(Tensor());
+  no_tangents({g, x, w, b}, "linear_backward");
+  std::array<Tensor, 3> d;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    std::tie(d[0], d[1], d[2]) = linear_backward_op().call(g, x, w, bias, act, need_x, need_w, need_bias);
+  }
+  d = once(std::move(d), "linear", {g, x, w, b});
+  return {d[0], d[1], d[2]};
+}
+
 struct LinearFunction : torch::autograd::Function<LinearFunction> {
   // Absent optional inputs have no edge: those of bias and residual are numbered without them.
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const OptTensor& bias,
@@ -237,23 +260,15 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads)
   {
-    static auto op = c10::Dispatcher::singleton()
-                         .findSchemaOrThrow("rbq::linear_backward", "")
-                         .typed<decltype(linear_backward_kernel)>();
-    no_tangents({grads[0]}, "linear's gradient");
     const auto saved = ctx->get_saved_variables();
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1);
     const bool has_bias = saved[2].defined(), nb = has_bias && ctx->needs_input_grad(2);
     const bool nr = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(has_bias ? 3 : 2);
-    std::array<Tensor, 3> d;
-    if (nx || nw || nb) {
-      at::AutoDispatchBelowADInplaceOrView below;
-      auto [dx, dw, db] = op.call(grads[0], saved[0], saved[1], has_bias ? OptTensor(saved[2]) : OptTensor(),
-                                  ctx->saved_data["act"].toStringRef(), nx, nw, nb);
-      d = {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor()};
-    }
-    d = once(std::move(d), "linear", {grads[0], saved[0], saved[1], saved[2]});
-    return {d[0], d[1], d[2], nr ? grads[0] : Tensor(), Tensor()};
+    Tensor dx, dw, db;
+    if (nx || nw || nb)
+      std::tie(dx, dw, db) = linear_backward_autograd(grads[0], saved[0], saved[1], has_bias ? OptTensor(saved[2]) : OptTensor(),
+                                                      ctx->saved_data["act"].toStringRef(), nx, nw, nb);
+    return {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor(), nr ? grads[0] : Tensor(), Tensor()};
   }
 };
 
@@ -348,6 +363,27 @@ c10::TypedOperatorHandle<decltype(layer_norm_kernel)>& layer_norm_op()
   return op;
 }
 
+c10::TypedOperatorHandle<decltype(layer_norm_backward_kernel)>& layer_norm_backward_op()
+{
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("rbq::layer_norm_backward", "")
+                       .typed<decltype(layer_norm_backward_kernel)>();
+  return op;
+}
+
+Three layer_norm_backward_autograd(const Tensor& g, const Tensor& x, const Tensor& w, const Tensor& mean, const Tensor& rstd,
+                                   bool need_x, bool need_w, bool need_b)
+{
+  no_tangents({g, x, w, mean, rstd}, "layer_norm_backward");
+  std::array<Tensor, 3> d;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    std::tie(d[0], d[1], d[2]) = layer_norm_backward_op().call(g, x, w, mean, rstd, need_x, need_w, need_b);
+  }
+  d = once(std::move(d), "layer_norm", {g, x, w, mean, rstd});
+  return {d[0], d[1], d[2]};
+}
+
 struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Tensor& b, double eps)
   {
@@ -361,20 +397,10 @@ struct LayerNormFunction : torch::autograd::Function<LayerNormFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads)
   {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    no_tangents({grads[0]}, "layer_norm's gradient");
-    static auto op = c10::Dispatcher::singleton()
-                         .findSchemaOrThrow("rbq::layer_norm_backward", "")
-                         .typed<decltype(layer_norm_backward_kernel)>();
     const auto s = ctx->get_saved_variables();
     const bool nx = ctx->needs_input_grad(0), nw = ctx->needs_input_grad(1), nb = ctx->needs_input_grad(2);
-    std::array<Tensor, 3> d;
-    {
-      at::AutoDispatchBelowADInplaceOrView below;
-      auto [dx, dw, db] = op.call(grads[0], s[0], s[1], s[2], s[3], nx, nw, nb);
-      d = {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor()};
-    }
-    d = once(std::move(d), "layer_norm", {grads[0], s[0], s[1]});
-    return {d[0], d[1], d[2], Tensor()};
+    auto [dx, dw, db] = layer_norm_backward_autograd(grads[0], s[0], s[1], s[2], s[3], nx, nw, nb);
+    return {nx ? dx : Tensor(), nw ? dw : Tensor(), nb ? db : Tensor(), Tensor()};
   }
 };
 
@@ -466,6 +492,27 @@ c10::TypedOperatorHandle<decltype(softmax_loss_kernel)>& softmax_loss_op()
   return op;
 }
 
+c10::TypedOperatorHandle<decltype(softmax_loss_backward_kernel)>& softmax_loss_backward_op()
+{
+  static auto op = c10::Dispatcher::singleton()
+                       .findSchemaOrThrow("rbq::softmax_loss_backward", "")
+                       .typed<decltype(softmax_loss_backward_kernel)>();
+  return op;
+}
+
+Two softmax_loss_backward_autograd(const Tensor& g, const Tensor& q, const Tensor& bank, const Tensor& target,
+                                   const Tensor& loss, const Tensor& lse, double scale, bool need_q, bool need_bank)
+{
+  no_tangents({g, q, bank, loss, lse}, "softmax_loss_backward");
+  std::array<Tensor, 2> d;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    std::tie(d[0], d[1]) = softmax_loss_backward_op().call(g, q, bank, target, loss, lse, scale, need_q, need_bank);
+  }
+  d = once(std::move(d), "softmax_loss", {g, q, bank, loss, lse});
+  return {d[0], d[1]};
+}
+
 struct SoftmaxLossFunction : torch::autograd::Function<SoftmaxLossFunction> {
   static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& bank, const Tensor& target, double scale)
   {
@@ -480,20 +527,11 @@ struct SoftmaxLossFunction : torch::autograd::Function<SoftmaxLossFunction> {
   static variable_list backward(AutogradContext* ctx, variable_list grads)
   {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
-    no_tangents({grads[0]}, "softmax_loss's gradient");
-    static auto op = c10::Dispatcher::singleton()
-                         .findSchemaOrThrow("rbq::softmax_loss_backward", "")
-                         .typed<decltype(softmax_loss_backward_kernel)>();
     const auto s = ctx->get_saved_variables();
     const bool nq = ctx->needs_input_grad(0), nk = ctx->needs_input_grad(1);
-    std::array<Tensor, 2> d;
-    {
-      at::AutoDispatchBelowADInplaceOrView below;
-      auto [dq, dbank] = op.call(grads[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(), nq, nk);
-      d = {nq ? dq : Tensor(), nk ? dbank : Tensor()};
-    }
-    d = once(std::move(d), "softmax_loss", {grads[0], s[0], s[1]});
-    return {d[0], d[1], Tensor(), Tensor()};
+    auto [dq, dbank] = softmax_loss_backward_autograd(grads[0], s[0], s[1], s[2], s[3], s[4], ctx->saved_data["scale"].toDouble(),
+                                                      nq, nk);
+    return {nq ? dq : Tensor(), nk ? dbank : Tensor(), Tensor(), Tensor()};
   }
 };
 
@@ -544,8 +582,11 @@ TORCH_LIBRARY_IMPL(rbq, Meta, m)
 TORCH_LIBRARY_IMPL(rbq, Autograd, m)
 {
   m.impl("linear", linear_autograd);
+  m.impl("linear_backward", linear_backward_autograd);
   m.impl("layer_norm", layer_norm_autograd);
+  m.impl("layer_norm_backward", layer_norm_backward_autograd);
   m.impl("softmax_loss", softmax_loss_autograd);
+  m.impl("softmax_loss_backward", softmax_loss_backward_autograd);
 }
 
 }  // namespace

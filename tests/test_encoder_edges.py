@@ -66,6 +66,26 @@ def test_second_derivatives_are_refused_on_every_way_back():
         assert not any(d.requires_grad for d in plain)
 
 
+def test_backward_operators_called_directly_refuse_more_derivatives():
+    o, t = ops(), meta(4, dt=torch.int64)
+    per_row = lambda: meta(4, dt=F32)  # noqa: E731
+    for call, args in [
+        (lambda g, x, w, b: o.linear_backward(g, x, w, b, "gelu", True, True, True), [meta(4, 8), meta(4, 16), meta(8, 16), meta(8)]),
+        (lambda g, x, w, m, r: o.layer_norm_backward(g, x, w, m, r, True, True, True),
+         [meta(4, 16), meta(4, 16), meta(16), per_row(), per_row()]),
+        (lambda g, q, k, a, b: o.softmax_loss_backward(g, q, k, t, a, b, 2.0, True, True),
+         [per_row(), meta(4, 16), meta(9, 16), per_row(), per_row()]),
+    ]:
+        for i in range(len(args)):
+            with fw.dual_level(), pytest.raises(RuntimeError, match="no forward-mode derivative"):
+                call(*args[:i], fw.make_dual(args[i], torch.empty_like(args[i])), *args[i + 1:])
+            leaf = args[i].detach().clone().requires_grad_()
+            for d in call(*args[:i], leaf, *args[i + 1:]):
+                with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+                    torch.autograd.grad(d.sum() + leaf.sum(), leaf, retain_graph=True)
+        assert not any(d.requires_grad for d in call(*args))
+
+
 # -- on the GPU -------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,k,n,act", [(20000, 64, 517, "gelu"), (13331, 40, 1279, "relu"), (40001, 24, 333, "gelu")])
