@@ -85,6 +85,9 @@ Tensor scratch(const Tensor& like, int64_t bytes)
 {
   return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
+// Outputs for meta and fake tensors: dense rows whatever the input's strides, as the kernels write them.
+Tensor dense_meta(const Tensor& like) { return at::empty_symint(like.sym_sizes(), like.options()); }
+Tensor dense_meta_if(bool need, const Tensor& like) { return need ? dense_meta(like) : at::empty({0}, like.options()); }
 Tensor empty_if(bool need, const Tensor& like) { return need ? at::empty_like(like) : at::empty({0}, like.options()); }
 
 bool wants_grad(std::initializer_list<Tensor> ts)
@@ -214,7 +217,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward_kernel(const Tensor& g, const
 std::tuple<Tensor, Tensor, Tensor> linear_backward_meta(const Tensor&, const Tensor& x, const Tensor& w, const OptTensor&,
                                                         c10::string_view, bool need_x, bool need_w, bool need_bias)
 {
-  return {empty_if(need_x, x), empty_if(need_w, w),
+  return {dense_meta_if(need_x, x), dense_meta_if(need_w, w),
           need_bias ? at::empty_symint({w.sym_size(0)}, x.options()) : at::empty({0}, x.options())};
 }
 
@@ -326,7 +329,7 @@ Three layer_norm_meta(const Tensor& x, const Tensor&, const Tensor&, double)
 {
   c10::SymDimVector s(x.sym_sizes().begin(), x.sym_sizes().end() - 1);
   Tensor mean = at::empty_symint(s, x.options().dtype(at::kFloat));
-  return {at::empty_like(x), mean, at::empty_like(mean)};
+  return {dense_meta(x), mean, at::empty_like(mean)};
 }
 
 Three layer_norm_backward_kernel(const Tensor& g, const Tensor& x, const Tensor& w, const Tensor& mean, const Tensor& rstd,
@@ -354,7 +357,7 @@ Three layer_norm_backward_kernel(const Tensor& g, const Tensor& x, const Tensor&
 Three layer_norm_backward_meta(const Tensor&, const Tensor& x, const Tensor& w, const Tensor&, const Tensor&, bool need_x,
                                bool need_w, bool need_b)
 {
-  return {empty_if(need_x, x), empty_if(need_w, w), empty_if(need_b, w)};
+  return {dense_meta_if(need_x, x), dense_meta_if(need_w, w), dense_meta_if(need_b, w)};
 }
 
 c10::TypedOperatorHandle<decltype(layer_norm_kernel)>& layer_norm_op()
@@ -483,7 +486,7 @@ Two softmax_loss_backward_kernel(const Tensor& g, const Tensor& q, const Tensor&
 Two softmax_loss_backward_meta(const Tensor&, const Tensor& q, const Tensor& bank, const Tensor&, const Tensor&, const Tensor&,
                                double, bool need_q, bool need_bank)
 {
-  return {empty_if(need_q, q), empty_if(need_bank, bank)};
+  return {dense_meta_if(need_q, q), dense_meta_if(need_bank, bank)};
 }
 
 c10::TypedOperatorHandle<decltype(softmax_loss_kernel)>& softmax_loss_op()

@@ -86,6 +86,27 @@ def test_backward_operators_called_directly_refuse_more_derivatives():
         assert not any(d.requires_grad for d in call(*args))
 
 
+def strided_calls(device):
+    """Every operator on inputs whose rows are not dense (transposed, sliced, expanded)."""
+    o = ops()
+    e = lambda *s, dt=F16: torch.zeros(*s, dtype=dt, device=device)  # noqa: E731
+    x, w, g = e(2, 16, 6).transpose(1, 2), e(16, 8).t(), e(2, 8, 6).transpose(1, 2)
+    row, rows, t = e(32)[::2], e(3, 2, dt=F32).t(), e(8, dt=torch.int64)[::2]
+    xs, bank, each = e(16, 4).t(), e(16, 9).t(), e(1, dt=F32).expand(4)
+    xn, gn = e(2, 16, 3).transpose(1, 2), e(2, 16, 3).transpose(1, 2)
+    yield o.linear(x, w, e(16)[::2], g, "gelu")
+    yield from o.linear_backward(g, x, w, e(16)[::2], "gelu", True, True, True)
+    yield from o.layer_norm(xn, row, row)
+    yield from o.layer_norm_backward(gn, xn, row, rows, rows, True, True, True)
+    yield from o.softmax_loss(xs, bank, t, 2.0)
+    yield from o.softmax_loss_backward(each, xs, bank, t, each, each, 2.0, True, True)
+
+
+def test_meta_outputs_are_dense():
+    for t in strided_calls("meta"):
+        assert t.is_contiguous(), (t.shape, t.stride())
+
+
 # -- on the GPU -------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,k,n,act", [(20000, 64, 517, "gelu"), (13331, 40, 1279, "relu"), (40001, 24, 333, "gelu")])
@@ -213,3 +234,22 @@ def test_gelu_far_out(dt):
     dx, = torch.autograd.grad(y, leaf, torch.ones_like(y))
     assert torch.equal(y[:4], z[:4]) and not y[4:8].any() and y[8].isnan() and y[9] == 0
     assert (dx[:4] == 1).all() and not dx[4:8].any() and dx[8].isnan() and dx[9] == 0.5
+
+
+@pytest.mark.gpu
+def test_outputs_have_the_strides_that_meta_tensors_say():
+    for real, fake in zip(strided_calls("cuda"), strided_calls("meta"), strict=True):
+        assert real.shape == fake.shape and real.stride() == fake.stride() and real.dtype == fake.dtype
+    check_device()
+
+
+@pytest.mark.gpu
+def test_compiler_checks_of_the_operators():
+    """Schemas, fake tensors and ahead-of-time tracing of forward and backward, on strided inputs."""
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    r = lambda *s: torch.randn(s, generator=gen, device="cuda").to(F16).requires_grad_()  # noqa: E731
+    tests = ("test_schema", "test_faketensor", "test_aot_dispatch_dynamic")
+    o, t = ops(), torch.tensor([1, 0, 8, -1], device="cuda")
+    torch.library.opcheck(o.linear, (r(2, 16, 6).transpose(1, 2), r(16, 8).t(), r(8), r(2, 6, 8), "gelu"), test_utils=tests)
+    torch.library.opcheck(o.layer_norm, (r(2, 16, 3).transpose(1, 2), r(16), r(16), 1e-5), test_utils=tests)
+    torch.library.opcheck(o.softmax_loss, (r(16, 4).t(), r(16, 9).t(), t, 2.0), test_utils=tests)
