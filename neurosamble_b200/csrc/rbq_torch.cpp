@@ -55,12 +55,23 @@ std::string type_name(at::ScalarType t)
 
 int type_code(at::ScalarType t) { return t == at::kHalf ? RBQ_F16 : t == at::kBFloat16 ? RBQ_BF16 : RBQ_F32; }
 
+void check_type(const Tensor& t, at::ScalarType type, const char* name)
+{
+  TORCH_CHECK(t.scalar_type() == type, "rbq: ", name, " must be ", type_name(type), ", got ", type_name(t.scalar_type()));
+}
+void check_first_type(const Tensor& t, bool f32_too, const char* name)
+{
+  const auto s = t.scalar_type();
+  TORCH_CHECK(s == at::kHalf || s == at::kBFloat16 || (f32_too && s == at::kFloat), "rbq: ", name,
+              " must be torch.float16 or torch.bfloat16", f32_too ? " or torch.float32" : "", ", got ", type_name(s));
+}
+
 // t of the given type on like's device, dense and on a 16-byte boundary.
 Tensor operand(const Tensor& t, const Tensor& like, at::ScalarType type, const char* name)
 {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device(), "rbq: ", name, " must be a CUDA tensor on ", like.device(),
               ", got ", t.device());
-  TORCH_CHECK(t.scalar_type() == type, "rbq: ", name, " must be ", type_name(type), ", got ", type_name(t.scalar_type()));
+  check_type(t, type, name);
   Tensor d = t.contiguous();
   return reinterpret_cast<uintptr_t>(d.const_data_ptr()) % 16 == 0 ? d : d.clone();
 }
@@ -68,16 +79,24 @@ Tensor operand(const Tensor& t, const Tensor& like, at::ScalarType type, const c
 Tensor first(const Tensor& t, bool f32_too, const char* name)
 {
   TORCH_CHECK(t.is_cuda(), "rbq: ", name, " must be a CUDA tensor");
-  const auto s = t.scalar_type();
-  TORCH_CHECK(s == at::kHalf || s == at::kBFloat16 || (f32_too && s == at::kFloat), "rbq: ", name,
-              " must be torch.float16 or torch.bfloat16", f32_too ? " or torch.float32" : "", ", got ", type_name(s));
-  return operand(t, t, s, name);
+  check_first_type(t, f32_too, name);
+  return operand(t, t, t.scalar_type(), name);
 }
 
 void check_shape(const Tensor& t, at::IntArrayRef want, const char* name)
 {
   TORCH_CHECK(t.sizes() == want, "rbq: ", name, " must have shape ", want, ", got ", t.sizes());
 }
+
+// The same checks for meta and fake tensors, whose sizes may be symbols.
+void check_meta(const Tensor& t, at::ScalarType type, c10::SymIntArrayRef want, const char* name)
+{
+  check_type(t, type, name);
+  TORCH_CHECK(t.dim() == (int64_t)want.size(), "rbq: ", name, " must have shape ", want, ", got ", t.sym_sizes());
+  for (size_t i = 0; i < want.size(); ++i)
+    TORCH_SYM_CHECK(t.sym_size(i).sym_eq(want[i]), "rbq: ", name, " must have shape ", want, ", got ", t.sym_sizes());
+}
+c10::SymDimVector rows_of(const Tensor& x) { return c10::SymDimVector(x.sym_sizes().begin(), x.sym_sizes().end() - 1); }
 
 void* data(const Tensor& t) { return t.defined() ? const_cast<void*>(t.const_data_ptr()) : nullptr; }
 void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.device().index()).stream(); }
@@ -189,11 +208,26 @@ Tensor linear_kernel(const Tensor& x, const Tensor& w, const OptTensor& bias, co
   return y;
 }
 
-Tensor linear_meta(const Tensor& x, const Tensor& w, const OptTensor&, const OptTensor&, c10::string_view)
+c10::SymDimVector check_linear_meta(const Tensor& x, const Tensor& w, const OptTensor& bias, c10::string_view act)
 {
-  c10::SymDimVector s(x.sym_sizes().begin(), x.sym_sizes().end());
-  s.back() = w.sym_size(0);
-  return at::empty_symint(s, x.options());
+  check_first_type(x, false, "x");
+  check_type(w, x.scalar_type(), "w");
+  TORCH_CHECK(x.dim() >= 1 && w.dim() == 2, "rbq: linear takes x [..., k] and w [n, k], got ", x.sym_sizes(), " and ",
+              w.sym_sizes());
+  TORCH_SYM_CHECK(x.sym_size(-1).sym_eq(w.sym_size(1)), "rbq: linear takes x [..., k] and w [n, k], got ", x.sym_sizes(),
+                  " and ", w.sym_sizes());
+  if (bias.has_value() && bias->defined()) check_meta(*bias, x.scalar_type(), {w.sym_size(0)}, "bias");
+  activation(act);
+  c10::SymDimVector out = rows_of(x);
+  out.push_back(w.sym_size(0));
+  return out;
+}
+
+Tensor linear_meta(const Tensor& x, const Tensor& w, const OptTensor& bias, const OptTensor& residual, c10::string_view act)
+{
+  const auto out = check_linear_meta(x, w, bias, act);
+  if (residual.has_value() && residual->defined()) check_meta(*residual, x.scalar_type(), out, "residual");
+  return at::empty_symint(out, x.options());
 }
 
 std::tuple<Tensor, Tensor, Tensor> linear_backward_kernel(const Tensor& g, const Tensor& x, const Tensor& w,
@@ -214,9 +248,11 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward_kernel(const Tensor& g, const
   return {dx, dw, db};
 }
 
-std::tuple<Tensor, Tensor, Tensor> linear_backward_meta(const Tensor&, const Tensor& x, const Tensor& w, const OptTensor&,
-                                                        c10::string_view, bool need_x, bool need_w, bool need_bias)
+std::tuple<Tensor, Tensor, Tensor> linear_backward_meta(const Tensor& g, const Tensor& x, const Tensor& w,
+                                                        const OptTensor& bias, c10::string_view act, bool need_x, bool need_w,
+                                                        bool need_bias)
 {
+  check_meta(g, x.scalar_type(), check_linear_meta(x, w, bias, act), "g");
   return {dense_meta_if(need_x, x), dense_meta_if(need_w, w),
           need_bias ? at::empty_symint({w.sym_size(0)}, x.options()) : at::empty({0}, x.options())};
 }
@@ -293,13 +329,18 @@ struct NormArgs {
   int type, param_type;
 };
 
+void check_param_type(const Tensor& x, const Tensor& w)
+{
+  TORCH_CHECK(w.scalar_type() == x.scalar_type() || w.scalar_type() == at::kFloat, "rbq: w must be ",
+              type_name(x.scalar_type()), " or torch.float32, got ", type_name(w.scalar_type()));
+}
+
 NormArgs norm_args(const Tensor& x, const Tensor& w)
 {
   NormArgs a;
   a.x = first(x, true, "x");
   TORCH_CHECK(x.dim() >= 1 && x.size(-1) >= 1, "rbq: layer_norm takes x [..., d] with d >= 1, got ", x.sizes());
-  TORCH_CHECK(w.scalar_type() == x.scalar_type() || w.scalar_type() == at::kFloat, "rbq: w must be ",
-              type_name(x.scalar_type()), " or torch.float32, got ", type_name(w.scalar_type()));
+  check_param_type(x, w);
   a.w = operand(w, a.x, w.scalar_type(), "w");
   a.d = a.x.size(-1);
   TORCH_CHECK(a.d < (1ll << 31), "rbq: layer norm: bad sizes");
@@ -325,10 +366,19 @@ Three layer_norm_kernel(const Tensor& x, const Tensor& w, const Tensor& b, doubl
   return {y, mean, rstd};
 }
 
-Three layer_norm_meta(const Tensor& x, const Tensor&, const Tensor&, double)
+void check_norm_meta(const Tensor& x, const Tensor& w)
 {
-  c10::SymDimVector s(x.sym_sizes().begin(), x.sym_sizes().end() - 1);
-  Tensor mean = at::empty_symint(s, x.options().dtype(at::kFloat));
+  check_first_type(x, true, "x");
+  TORCH_CHECK(x.dim() >= 1, "rbq: layer_norm takes x [..., d] with d >= 1, got ", x.sym_sizes());
+  check_param_type(x, w);
+  check_meta(w, w.scalar_type(), {x.sym_size(-1)}, "w");
+}
+
+Three layer_norm_meta(const Tensor& x, const Tensor& w, const Tensor& b, double)
+{
+  check_norm_meta(x, w);
+  check_meta(b, w.scalar_type(), {x.sym_size(-1)}, "b");
+  Tensor mean = at::empty_symint(rows_of(x), x.options().dtype(at::kFloat));
   return {dense_meta(x), mean, at::empty_like(mean)};
 }
 
@@ -354,9 +404,13 @@ Three layer_norm_backward_kernel(const Tensor& g, const Tensor& x, const Tensor&
   return {dx, dw, db};
 }
 
-Three layer_norm_backward_meta(const Tensor&, const Tensor& x, const Tensor& w, const Tensor&, const Tensor&, bool need_x,
-                               bool need_w, bool need_b)
+Three layer_norm_backward_meta(const Tensor& g, const Tensor& x, const Tensor& w, const Tensor& mean, const Tensor& rstd,
+                               bool need_x, bool need_w, bool need_b)
 {
+  check_norm_meta(x, w);
+  check_meta(g, x.scalar_type(), x.sym_sizes(), "g");
+  check_meta(mean, at::kFloat, rows_of(x), "mean");
+  check_meta(rstd, at::kFloat, rows_of(x), "rstd");
   return {dense_meta_if(need_x, x), dense_meta_if(need_w, w), dense_meta_if(need_b, w)};
 }
 
@@ -457,8 +511,20 @@ Two softmax_loss_kernel(const Tensor& q, const Tensor& bank, const Tensor& targe
   return {loss, lse};
 }
 
-Two softmax_loss_meta(const Tensor& q, const Tensor&, const Tensor&, double)
+void check_loss_meta(const Tensor& q, const Tensor& bank, const Tensor& target)
 {
+  check_first_type(q, false, "q");
+  check_type(bank, q.scalar_type(), "bank");
+  TORCH_CHECK(q.dim() == 2 && bank.dim() == 2, "rbq: softmax_loss takes q [n, d] and bank [v, d] with v, d >= 1, got ",
+              q.sym_sizes(), " and ", bank.sym_sizes());
+  TORCH_SYM_CHECK(q.sym_size(1).sym_eq(bank.sym_size(1)), "rbq: softmax_loss takes q [n, d] and bank [v, d] with v, d >= 1, got ",
+                  q.sym_sizes(), " and ", bank.sym_sizes());
+  check_meta(target, at::kLong, {q.sym_size(0)}, "target");
+}
+
+Two softmax_loss_meta(const Tensor& q, const Tensor& bank, const Tensor& target, double)
+{
+  check_loss_meta(q, bank, target);
   Tensor loss = at::empty_symint({q.sym_size(0)}, q.options().dtype(at::kFloat));
   return {loss, at::empty_like(loss)};
 }
@@ -483,9 +549,13 @@ Two softmax_loss_backward_kernel(const Tensor& g, const Tensor& q, const Tensor&
   return {dq, dbank};
 }
 
-Two softmax_loss_backward_meta(const Tensor&, const Tensor& q, const Tensor& bank, const Tensor&, const Tensor&, const Tensor&,
-                               double, bool need_q, bool need_bank)
+Two softmax_loss_backward_meta(const Tensor& g, const Tensor& q, const Tensor& bank, const Tensor& target, const Tensor& loss,
+                               const Tensor& lse, double, bool need_q, bool need_bank)
 {
+  check_loss_meta(q, bank, target);
+  check_meta(g, at::kFloat, {q.sym_size(0)}, "g");
+  check_meta(loss, at::kFloat, {q.sym_size(0)}, "loss");
+  check_meta(lse, at::kFloat, {q.sym_size(0)}, "lse");
   return {dense_meta_if(need_q, q), dense_meta_if(need_bank, bank)};
 }
 

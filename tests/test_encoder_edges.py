@@ -107,6 +107,46 @@ def test_meta_outputs_are_dense():
         assert t.is_contiguous(), (t.shape, t.stride())
 
 
+def refusals(device):
+    """Calls that every device refuses, with what the message says."""
+    o = ops()
+    e = lambda *s, dt=F16: torch.zeros(s, dtype=dt, device=device)  # noqa: E731
+    x, w, y, t, f = e(4, 16), e(8, 16), e(4, 8), e(4, dt=torch.int64), e(4, dt=F32)
+    yes = (True, True, True)
+    return [
+        (lambda: o.linear(x.float(), w.float()), "float16 or torch.bfloat16"),
+        (lambda: o.linear(x, w.bfloat16()), "w must be torch.float16"),
+        (lambda: o.linear(x, e(8, 17)), r"x \[..., k\] and w \[n, k\]"),
+        (lambda: o.linear(e(), w), r"x \[..., k\] and w \[n, k\]"),
+        (lambda: o.linear(x, w[0]), r"x \[..., k\] and w \[n, k\]"),
+        (lambda: o.linear(x, w, w[0]), "bias must have shape"),
+        (lambda: o.linear(x, w, None, x), "residual must have shape"),
+        (lambda: o.linear(x, w, None, None, "tanh"), "act must be one of"),
+        (lambda: o.linear_backward(x, x, w, None, "none", *yes), "g must have shape"),
+        (lambda: o.linear_backward(y.float(), x, w, None, "none", *yes), "g must be torch.float16"),
+        (lambda: o.layer_norm(e(), w[0], w[0]), r"layer_norm takes x \[..., d\]"),
+        (lambda: o.layer_norm(x, w[0, :8], w[0]), "w must have shape"),
+        (lambda: o.layer_norm(x, w[0], w[0, :8]), "b must have shape"),
+        (lambda: o.layer_norm(x, w[0], w[0].float()), "b must be torch.float16"),
+        (lambda: o.layer_norm(x, w[0].double(), w[0].double()), "w must be torch.float16 or torch.float32"),
+        (lambda: o.layer_norm_backward(y, x, w[0], f, f, *yes), "g must have shape"),
+        (lambda: o.layer_norm_backward(x, x, w[0], f[:2], f, *yes), "mean must have shape"),
+        (lambda: o.layer_norm_backward(x, x, w[0], f, f.half(), *yes), "rstd must be torch.float32"),
+        (lambda: o.softmax_loss(x, e(8, 17), t, 1.0), "softmax_loss takes"),
+        (lambda: o.softmax_loss(x[None], w, t, 1.0), "softmax_loss takes"),
+        (lambda: o.softmax_loss(x, w, t.int(), 1.0), "target must be torch.int64"),
+        (lambda: o.softmax_loss(x, w, t[:2], 1.0), "target must have shape"),
+        (lambda: o.softmax_loss_backward(f[:2], x, w, t, f, f, 1.0, True, True), "g must have shape"),
+        (lambda: o.softmax_loss_backward(f, x, w, t, f, f.half(), 1.0, True, True), "lse must be torch.float32"),
+    ]
+
+
+def test_meta_tensors_are_checked():
+    for call, what in refusals("meta"):
+        with pytest.raises(RuntimeError, match=what):
+            call()
+
+
 # -- on the GPU -------------------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,k,n,act", [(20000, 64, 517, "gelu"), (13331, 40, 1279, "relu"), (40001, 24, 333, "gelu")])
@@ -253,3 +293,10 @@ def test_compiler_checks_of_the_operators():
     torch.library.opcheck(o.linear, (r(2, 16, 6).transpose(1, 2), r(16, 8).t(), r(8), r(2, 6, 8), "gelu"), test_utils=tests)
     torch.library.opcheck(o.layer_norm, (r(2, 16, 3).transpose(1, 2), r(16), r(16), 1e-5), test_utils=tests)
     torch.library.opcheck(o.softmax_loss, (r(16, 4).t(), r(16, 9).t(), t, 2.0), test_utils=tests)
+
+
+@pytest.mark.gpu
+def test_real_tensors_are_checked_alike():
+    for call, what in refusals("cuda"):
+        with pytest.raises(RuntimeError, match=what):
+            call()
