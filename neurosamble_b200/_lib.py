@@ -11,6 +11,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "librbq.so")
 TORCH_LIB_PATH = os.path.join(_HERE, "_lib", "librbq_torch.so")  # PyTorch operators over the C ABI
+TORCH_VERSION_PATH = TORCH_LIB_PATH + ".torch"  # the version of torch that it was compiled against
 
 RBQ_OK = 0
 ERRORS = {1: "invalid argument", 2: "CUDA error", 3: "out of device memory", 4: "I/O error",
@@ -127,6 +128,15 @@ def lib() -> ctypes.CDLL:
             fn.restype = _RESTYPES.get(name, ctypes.c_int)
         _lib = L
     return _lib
+
+
+def torch_version_built() -> str:
+    """The version of torch that librbq_torch.so was compiled against ("" if there is no record of it)."""
+    try:
+        with open(TORCH_VERSION_PATH) as f:
+            return f.read().strip()
+    except OSError:
+        return ""
 
 
 def check(status: int) -> None:

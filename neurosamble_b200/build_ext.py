@@ -17,6 +17,7 @@ CSRC = os.path.join(HERE, "csrc")
 OUT_DIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(OUT_DIR, "librbq.so")
 TORCH_LIB = os.path.join(OUT_DIR, "librbq_torch.so")
+TORCH_VERSION = TORCH_LIB + ".torch"  # the version of torch that it was compiled against
 
 SOURCES = ["rbq_host_math.cpp", "rbq_build.cu", "rbq_search.cu", "rbq_coarse_tc.cu", "rbq_gemm.cu", "rbq_norm.cu",
            "rbq_capi.cu"]
@@ -48,7 +49,23 @@ def _cxx() -> str:
     raise RuntimeError("g++ not found")
 
 
-def build_torch(env: dict) -> None:
+def _environment() -> dict:
+    env = dict(os.environ)
+    env.pop("CXX", None)
+    env.pop("CC", None)
+    return env
+
+
+def torch_version() -> str:
+    """The running torch's version, "" without torch."""
+    try:
+        import torch
+    except ImportError:
+        return ""
+    return str(torch.__version__)
+
+
+def build_torch() -> None:
     """Compile the PyTorch operators against the running torch's headers and link them to librbq.so beside them."""
     import torch
     root = os.path.dirname(torch.__file__)
@@ -59,28 +76,46 @@ def build_torch(env: dict) -> None:
                     "-I" + os.path.join(include, "torch", "csrc", "api", "include"), "-I/usr/local/cuda/include",
                     os.path.join(CSRC, TORCH_SOURCE), "-o", tmp, "-L" + os.path.join(root, "lib"), "-L" + OUT_DIR,
                     "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda", "-lrbq", "-Wl,-rpath,$ORIGIN"],
-                   check=True, env=env)
+                   check=True, env=_environment())
+    if os.path.exists(TORCH_VERSION):  # never beside a library of another version
+        os.remove(TORCH_VERSION)
     os.replace(tmp, TORCH_LIB)
+    with open(TORCH_VERSION, "w") as f:
+        f.write(torch_version() + "\n")
+
+
+def _older(path: str, sources) -> bool:
+    if not os.path.exists(path):
+        return True
+    t = os.path.getmtime(path)
+    return any(os.path.getmtime(os.path.join(CSRC, f)) > t for f in sources)
 
 
 def _stale() -> bool:
-    if not os.path.exists(LIB) or not os.path.exists(TORCH_LIB):
+    return _older(LIB, SOURCES + HEADERS)
+
+
+def _torch_stale() -> bool:
+    """librbq_torch.so is older than its sources, or was compiled against another torch than the running one."""
+    if _older(TORCH_LIB, [TORCH_SOURCE, HEADERS[-1]]) or not os.path.exists(TORCH_VERSION):
         return True
-    t = min(os.path.getmtime(LIB), os.path.getmtime(TORCH_LIB))
-    for f in SOURCES + HEADERS + [TORCH_SOURCE]:
-        if os.path.getmtime(os.path.join(CSRC, f)) > t:
-            return True
-    return False
+    with open(TORCH_VERSION) as f:
+        return f.read().strip() != torch_version()
 
 
 def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and not _stale():
-        return LIB
+    """Build what is out of date.  Without torch librbq.so is built alone: C users need no more."""
+    if force or _stale():
+        build_library(verbose)
+    if torch_version() and (force or _torch_stale()):
+        build_torch()
+    return LIB
+
+
+def build_library(verbose: bool = False) -> None:
     os.makedirs(OUT_DIR, exist_ok=True)
     nvcc = _nvcc()
-    env = dict(os.environ)
-    env.pop("CXX", None)
-    env.pop("CC", None)
+    env = _environment()
 
     def compile_one(src: str) -> str:
         obj = os.path.join(OUT_DIR, os.path.splitext(src)[0] + ".o")
@@ -104,8 +139,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.replace(tmp, LIB)
     for o in objs:
         os.remove(o)
-    build_torch(env)
-    return LIB
 
 
 if __name__ == "__main__":

@@ -43,6 +43,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import warnings
 from typing import Optional, Tuple
 
 import torch
@@ -240,8 +241,25 @@ def _(dist, ids):
     return dist.new_empty((n, k)), ids.new_empty((n, k))
 
 
-# linear, layer_norm, softmax_loss and their backward passes are registered by librbq_torch.so
-# (csrc/rbq_torch.cpp).  Before the libraries are built there is nothing to load: `_lib.lib()` says so
-# at the first call of any other entry point.
-if os.path.exists(_lib.TORCH_LIB_PATH):
-    torch.ops.load_library(_lib.TORCH_LIB_PATH)
+def _load_encoder_operators() -> bool:
+    """Register linear, layer_norm, softmax_loss and their backward passes (librbq_torch.so, csrc/rbq_torch.cpp).
+    The library holds torch's C++ classes as they were when it was compiled, so it is loaded into that version
+    only.  Without it the index and its operators go on: they need librbq.so alone.  Before the libraries are
+    built there is nothing to load: `_lib.lib()` says so at the first call of any entry point."""
+    if not os.path.exists(_lib.TORCH_LIB_PATH):
+        return False
+    built, why = _lib.torch_version_built(), ""
+    if built and built != str(torch.__version__):
+        why = f"it was compiled against torch {built}, this is {torch.__version__}"
+    else:
+        try:
+            torch.ops.load_library(_lib.TORCH_LIB_PATH)
+        except OSError as e:
+            why = str(e)
+    if why:
+        warnings.warn(f"neurosamble_b200: torch.ops.rbq.linear, layer_norm and softmax_loss are missing, since "
+                      f"{_lib.TORCH_LIB_PATH} was not loaded: {why}; run `python -m neurosamble_b200.build_ext`")
+    return not why
+
+
+_load_encoder_operators()
