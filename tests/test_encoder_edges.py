@@ -1,12 +1,13 @@
 """Corners of the read encoder's operators that tests/test_encoder_ops.py does not reach; the definitions in 64
 bits and the tolerances are those of that file."""
+import ctypes
 import math
 
 import pytest
 import torch
 import torch.autograd.forward_ad as fw
 
-from test_encoder_ops import (BF16, F16, F32, check_device, linear_check, linear_inputs, loss_inputs, ops, tiny, u,
+from test_encoder_ops import (ADD, BF16, F16, F32, check_device, linear_check, linear_inputs, loss_inputs, ops, tiny, u,
                               within)
 
 
@@ -300,3 +301,64 @@ def test_real_tensors_are_checked_alike():
     for call, what in refusals("cuda"):
         with pytest.raises(RuntimeError, match=what):
             call()
+
+
+def check_loss_gradients_by_rows(q, bank, target, scale, g, dq, dbank, rows=1024):
+    """test_encoder_ops.loss_check's gradients and tolerances, `rows` queries at a time."""
+    dt, (n, d), v = q.dtype, q.shape, bank.shape[0]
+    K = bank.double()
+    wdk, tdk = torch.zeros_like(K), torch.zeros_like(K)
+    top = g[(target >= 0) & (target < v)].abs().max().double()
+    for a in range(0, n, rows):
+        Q, t = q[a:a + rows].double(), target[a:a + rows]
+        s = scale * (Q @ K.t())
+        es = (d + 8) * ADD * scale * (Q.abs() @ K.abs().t()) + 4 * ADD * s.abs()
+        valid = (t >= 0) & (t < v)
+        weight = torch.where(valid, g[a:a + rows].double(), torch.zeros(1, dtype=torch.float64, device=q.device))
+        lse = torch.logsumexp(s, 1)
+        e = es.max(1).values + (v + 64) * ADD * 2 + 4 * ADD * lse.abs()
+        dl = torch.exp(s - lse[:, None])
+        at = torch.arange(len(t), device=q.device)[valid]
+        own = dl[at, t[valid]].clone()
+        dl[at, t[valid]] = 0.0
+        dl[at, t[valid]] = -dl[valid].sum(1)  # 1 - p without its cancellation
+        assert (own + dl[at, t[valid]].abs() - 1).abs().max() < 1e-9
+        dl *= weight[:, None]
+        el = (u(dt) + 8 * ADD) * dl.abs() + 2 * (e[:, None] + es) * dl.abs() * 1.01 + (2.0 ** -38 * top if dt == F16 else 0.0)
+        wdq = scale * dl @ K
+        within(dq[a:a + rows], wdq, (u(dt) + 4 * ADD) * wdq.abs() + 1.01 * scale * (el + (v + 72) * ADD * dl.abs()) @ K.abs() +
+               tiny(dt), f"dq from row {a}")
+        wdk += scale * dl.t() @ Q
+        tdk += 1.01 * scale * (el + (n + 72) * ADD * dl.abs()).t() @ Q.abs()
+    within(dbank, wdk, (u(dt) + 4 * ADD) * wdk.abs() + tdk + tiny(dt), "dbank")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,v,d,dt", [(8192, 80001, 40, F16), (200003, 4001, 24, BF16), (9001, 75003, 33, BF16)])
+def test_softmax_loss_gradient_in_several_pieces(n, v, d, dt):
+    """Banks whose logits' gradient does not fit the workspace at once: the queries' gradient is added up over the
+    pieces, the bank's written piece by piece, and the last piece is shorter and odd.  It repeats bit for
+    bit, alone and on two streams at once."""
+    from neurosamble_b200 import _lib
+    need = ctypes.c_int64()
+    _lib.call("rbq_softmax_loss_workspace", n, v, d, 0 if dt == F16 else 1, 1, ctypes.byref(need))
+    assert need.value < 2 * n * v  # not even the gradient of all logits
+    q, bank, target, g = loss_inputs(n, v, d, dt, seed=n)
+    target[:3] = torch.tensor([v - 1, v - 2, 0], device="cuda")  # in the last piece and in the first
+    loss, lse = ops().softmax_loss(q, bank, target, 5.0)
+    run = lambda: ops().softmax_loss_backward(g, q, bank, target, loss, lse, 5.0, True, True)  # noqa: E731
+    dq, dbank = run()
+    check_loss_gradients_by_rows(q, bank, target, 5.0, g, dq, dbank)
+    one = ops().softmax_loss_backward(g, q, bank, target, loss, lse, 5.0, True, False)[0]
+    other = ops().softmax_loss_backward(g, q, bank, target, loss, lse, 5.0, False, True)[1]
+    assert torch.equal(one, dq) and torch.equal(other, dbank)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(2):
+        for s in streams:
+            with torch.cuda.stream(s):
+                outs.append(run())
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, dq) and torch.equal(b, dbank) for a, b in outs)
+    check_device()
