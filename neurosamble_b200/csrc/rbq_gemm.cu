@@ -1231,17 +1231,6 @@ __global__ void grad_rows_kernel(const float* __restrict__ g, const int64_t* __r
 // ---------------------------------------------------------------------------------------
 // Host side.
 // ---------------------------------------------------------------------------------------
-int sm_count()
-{
-  static std::atomic<int> known[64];
-  int dev = 0, n = 0;
-  RBQ_CUDA(cudaGetDevice(&dev));
-  if (dev < 64 && (n = known[dev].load()) > 0) return n;
-  RBQ_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-  if (dev < 64) known[dev].store(n);
-  return n;
-}
-
 constexpr int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
 
 // A row-major matrix [rows, cols] with rows ld values apart.
@@ -1299,7 +1288,7 @@ void launch_gemm(GemmArgs& a, const CUtensorMap& ta, const CUtensorMap& tb, cons
     if (dev < 64) ready.fetch_or(1ull << dev);
   }
   cudaLaunchConfig_t cfg{};
-  if (EPI != kEpiSlab) a.ctas = std::min(a.units, sm_count() / CG);
+  if (EPI != kEpiSlab) a.ctas = std::min(a.units, device_sm_count() / CG);
   a.step_fast = a.ctas % a.len_fast;
   a.step_slow = a.ctas / a.len_fast;
   cfg.gridDim = dim3((unsigned)(CG * a.ctas));
@@ -1352,7 +1341,7 @@ void gemm(GemmArgs a, Matrix A, bool a_mn, Matrix B, bool b_mn, int cg, const CU
 
 // CTAs of a tile: pairs with 256 x 256 tiles where there is one for every SM pair, else single CTAs
 // with 128 x 128 tiles, which spread a small product over four times as many SMs.
-int group_size(int64_t M, int64_t N) { return N > 128 && ceil_div(M, 256) * ceil_div(N, 256) >= sm_count() / 2 ? 2 : 1; }
+int group_size(int64_t M, int64_t N) { return N > 128 && ceil_div(M, 256) * ceil_div(N, 256) >= device_sm_count() / 2 ? 2 : 1; }
 
 // Carves aligned pieces out of the caller's workspace; with no workspace it only counts.
 struct Carver {
@@ -1373,7 +1362,7 @@ void pad_rows(const void* src, int64_t rows, int cols, int ld, void* dst, const 
   int x = 8;  // threads to a row
   while (x < 256 && x < ld / 8) x *= 2;
   const dim3 block(x, 256 / x);
-  const int64_t blocks = std::min<int64_t>(ceil_div(rows, block.y), (int64_t)sm_count() * 16);
+  const int64_t blocks = std::min<int64_t>(ceil_div(rows, block.y), (int64_t)device_sm_count() * 16);
   pad_rows_kernel<<<(unsigned)blocks, block, 0, s>>>(static_cast<const uint16_t*>(src), rows, cols, ld,
                                                      static_cast<uint16_t*>(dst), weights);
   RBQ_LAUNCHED();
@@ -1402,7 +1391,7 @@ SlabPlan plan_slabs(int64_t M, int N, int64_t K, bool must_add)
 {
   SlabPlan p;
   p.cg = N > 128 && M > 128 ? 2 : 1;
-  const int64_t slots = sm_count() / p.cg, tm = ceil_div(M, kBM * p.cg), tiles = tm * ceil_div(N, 128 * p.cg);
+  const int64_t slots = device_sm_count() / p.cg, tm = ceil_div(M, kBM * p.cg), tiles = tm * ceil_div(N, 128 * p.cg);
   p.tiles_m = (int)tm;
   p.kblocks = (int)ceil_div(K, kBK);
   p.total = tiles * p.kblocks;
@@ -1431,7 +1420,7 @@ template <typename T>
 void add_slabs(const SlabPlan& p, const float* slabs, bool all, int64_t M, int N, float alpha, const float* alpha_dev, T* out,
                cudaStream_t s)
 {
-  const int64_t blocks = std::min<int64_t>(ceil_div(M * (p.ld / 4), 256), (int64_t)sm_count() * 8);
+  const int64_t blocks = std::min<int64_t>(ceil_div(M * (p.ld / 4), 256), (int64_t)device_sm_count() * 8);
   const SlabTiles st{p.slabs, 128 * p.cg, p.tiles_m, p.kblocks, all ? 0 : p.ctas, p.total};
   add_slabs_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(slabs, st, p.rows * p.ld, M, N, (int)p.ld, alpha, alpha_dev, out);
   RBQ_LAUNCHED();
@@ -1494,10 +1483,10 @@ void linear_backward(const T* g, const T* x, const T* w, const T* bias, T* dx, T
   // The gradient kernel's sums are 4 rows of n floats per CTA: less than a pass over dz from about 2,048 rows.
   const bool fused = act != RBQ_ACT_NONE && m >= 2048;
   const int64_t tiles_m = ceil_div(m, kBM * cg), tiles_n = ceil_div(n, 128 * cg);
-  const int ctas = (int)std::min<int64_t>(tiles_m * tiles_n, sm_count() / cg);
+  const int ctas = (int)std::min<int64_t>(tiles_m * tiles_n, device_sm_count() / cg);
   const int gx = (int)ceil_div(n, kColGroup * 8);
   const int parts = fused ? ctas * cg * 4
-                          : (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(m, 64), ceil_div(4 * sm_count(), gx)));
+                          : (int)std::max<int64_t>(1, std::min<int64_t>(ceil_div(m, 64), ceil_div(4 * device_sm_count(), gx)));
   float* part = ws.take<float>((int64_t)parts * n);
   if (act == RBQ_ACT_NONE) {
     Z = addressable(g, m, n, ws, run, s);
@@ -1549,7 +1538,7 @@ void loss_forward(const T* q, const T* bank, const int64_t* target, int64_t n, i
   const int cg = group_size(n, v);
   // Runs of up to 16 tiles write one partial row each, but leave enough of them to even out over the SMs.
   const int64_t tiles_m = ceil_div(n, kBM * cg), tiles_n = ceil_div(v, 128 * cg);
-  const int length = (int)std::max<int64_t>(1, std::min<int64_t>(16, tiles_m * tiles_n / (8 * (sm_count() / cg))));
+  const int length = (int)std::max<int64_t>(1, std::min<int64_t>(16, tiles_m * tiles_n / (8 * (device_sm_count() / cg))));
   const int64_t tiles = 2 * cg * ceil_div(tiles_n, length);
   float2* partial = ws.take<float2>(tiles * n);
   if (!run) return;
@@ -1574,7 +1563,7 @@ int64_t piece_columns(int64_t n, int64_t v)
 {
   const int64_t most = std::max<int64_t>(1, kPieceBytes / (2 * n) / 256);  // in tiles of 256 columns
   // whole rounds of the SM pairs for the bank's gradient, where a piece holds one; the last piece is shorter
-  const int64_t pairs = sm_count() / 2, whole = most >= pairs ? most / pairs * pairs : most;
+  const int64_t pairs = device_sm_count() / 2, whole = most >= pairs ? most / pairs * pairs : most;
   return std::min(whole, ceil_div(v, 256)) * 256;
 }
 

@@ -501,21 +501,11 @@ __global__ void __launch_bounds__(1024) norm_parts_kernel(const float* __restric
   }
 }
 
-int sms()
-{
-  static std::atomic<int> known[64];
-  int dev = 0, n = 0;
-  RBQ_CUDA(cudaGetDevice(&dev));
-  if (dev < 64 && (n = known[dev].load()) > 0) return n;
-  RBQ_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-  if (dev < 64) known[dev].store(n);
-  return n;
-}
-
 // How a row is shared: vec values per load (16 bytes, or one where the width or an address does not
-// allow that), tpr threads per row, ch loads per thread; tpr = 0: wider than the register paths.  ch is the
-// next size up, so that no thread steps over more than half of its loads (200 M values in rows of 1,953
-// fp32: 644 us with 32 loads, 293 with 8; of 2,048 fp16: 369 with 4, 166 with 1).
+// allow that), tpr threads per row, ch loads per thread; tpr = 0: wider than the register paths.  For rows that a
+// block holds ch is the next size up, so that no thread steps over more than half of its loads (200 M values in
+// rows of 1,953 fp32: 644 us with 32 loads, 293 with 8; of 2,048 fp16: 369 with 4, 166 with 1).  Narrower rows of
+// single values have one size for widths to 32 and one to 256, and step over more.
 struct Plan {
   int vec, tpr, ch;
 };
@@ -563,7 +553,7 @@ int blocks_for(K kernel, size_t smem, int64_t rows, int tpr, int rounds)
     n = std::max(1, std::min(n, kMostBlocks));
     per_sm.store(n);
   }
-  const int64_t work = ceil_div(rows, kNormThreads / tpr), wave = (int64_t)sms() * n;
+  const int64_t work = ceil_div(rows, kNormThreads / tpr), wave = (int64_t)device_sm_count() * n;
   const int64_t waves = rounds > 0 ? std::max<int64_t>(1, std::min<int64_t>(64, work / (wave * rounds))) : 1;
   return (int)std::max<int64_t>(1, std::min<int64_t>(work, wave * waves));
 }
@@ -579,7 +569,7 @@ void run_forward(const T* x, const P* w, const P* b, T* y, float* mean, float* r
       <<<blocks_for<Kernel<T, P, VEC, CH, TPR, 0>>(norm_kernel<T, P, VEC, CH, TPR>, 0, rows, TPR, kRounds), kNormThreads, 0, \
          s>>>(x, w, b, y, mean, rstd, rows, d, eps)
   if (p.tpr == 0)
-    norm_wide_kernel<T, P><<<(unsigned)std::min<int64_t>(rows, (int64_t)sms() * kMostBlocks), kNormThreads, 0, s>>>(
+    norm_wide_kernel<T, P><<<(unsigned)std::min<int64_t>(rows, (int64_t)device_sm_count() * kMostBlocks), kNormThreads, 0, s>>>(
         x, w, b, y, mean, rstd, rows, d, eps);
   else if (p.vec == 1 && p.tpr == 8)
     RBQ_NORM(1, 4, 8);
@@ -611,7 +601,7 @@ void run_backward(const T* g, const T* x, const P* w, const float* mean, const f
 {
   const Plan p = plan_of(d, (int)sizeof(T), vector, true);
   constexpr int V = 16 / (int)sizeof(T);
-  int blocks = (int)std::min<int64_t>(rows, (int64_t)sms() * kMostBlocks);  // of the wide kernels
+  int blocks = (int)std::min<int64_t>(rows, (int64_t)device_sm_count() * kMostBlocks);  // of the wide kernels
   const bool sums = dw != nullptr || db != nullptr;
   float* out = sums ? part : nullptr;
   const size_t smem = sums && p.tpr && p.tpr < kNormThreads ? (size_t)2 * d * sizeof(float) : 0;
@@ -684,7 +674,7 @@ void launch_layer_norm(const void* x, const void* w, const void* b, void* y, flo
 
 int64_t layer_norm_workspace(int64_t rows, int d)
 {
-  return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)sms() * kMostBlocks)) * 2 * d * (int64_t)sizeof(float);
+  return std::max<int64_t>(1, std::min<int64_t>(rows, (int64_t)device_sm_count() * kMostBlocks)) * 2 * d * (int64_t)sizeof(float);
 }
 
 void launch_layer_norm_backward(const void* g, const void* x, const void* w, const float* mean, const float* rstd, void* dx,

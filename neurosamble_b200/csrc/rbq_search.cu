@@ -9,6 +9,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "rbq_internal.cuh"
 
@@ -426,10 +427,14 @@ __global__ void __launch_bounds__(256) refine_all_kernel(const float* __restrict
 
 int device_sm_count()
 {
+  static std::atomic<int> known[64];  // asked several times per call: the attribute is read once per device
   int dev = 0, n = 0;
   RBQ_CUDA(cudaGetDevice(&dev));
+  if (dev < 64 && (n = known[dev].load()) > 0) return n;
   RBQ_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-  return n > 0 ? n : 1;
+  if (n < 1) n = 1;
+  if (dev < 64) known[dev].store(n);
+  return n;
 }
 
 void launch_refine_all(const float* A, int64_t nq, const float* C, int d, int K, int p, const int* unsafe,
