@@ -27,7 +27,8 @@ softmax_loss take float16 or bfloat16, layer_norm also float32, with w and b of 
 float32.  A row of softmax_loss whose target lies outside [0, v) is ignored: loss 0, no
 gradient.  mean, rstd and lse carry no gradient; the backward passes (linear_backward,
 layer_norm_backward, softmax_loss_backward) are operators too and are not differentiable again.
-Forward-mode derivatives (dual tensors, torch.func.jvp) are refused.
+Forward-mode derivatives (dual tensors, torch.func.jvp) are refused.  ``torch_ops.check_op_errors()``
+waits for the device and tells whether a kernel of theirs failed.
 
 ``h`` is the index handle as an int (``IndexIVFRaBitQ.handle.value``).  ``query_bits`` of search
 is the search mode: 4 (QUANT4), 8 (QUANT8), 16 (LUT16) or 32 (LUT32); ``bits`` of query_prep is
@@ -239,6 +240,13 @@ def merge_results(dist: Tensor, ids: Tensor) -> Pair:
 def _(dist, ids):
     _, n, k = dist.shape
     return dist.new_empty((n, k)), ids.new_empty((n, k))
+
+
+def check_op_errors() -> None:
+    """Raise RuntimeError if a kernel of linear or softmax_loss (or of their backward passes) on the current device
+    gave up on a wait since the last check: their outputs are then invalid.  The operators themselves do not wait
+    for the device and cannot tell.  Synchronises; the record is one for all threads, and reading clears it."""
+    _lib.call("rbq_check_op_errors")
 
 
 def _load_encoder_operators() -> bool:

@@ -7,8 +7,8 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fw
 
-from test_encoder_ops import (ADD, BF16, F16, F32, check_device, linear_check, linear_inputs, loss_inputs, ops, tiny, u,
-                              within)
+from test_encoder_ops import (ADD, BF16, F16, F32, check_device, linear_check, linear_inputs, loss_inputs,
+                              norm_check, norm_inputs, ops, tiny, u, within)
 
 
 def meta(*s, dt=F16):
@@ -146,6 +146,24 @@ def test_meta_tensors_are_checked():
     for call, what in refusals("meta"):
         with pytest.raises(RuntimeError, match=what):
             call()
+
+
+def test_errors_of_the_kernels_are_raised(monkeypatch):
+    """A failed wait that the library reports (its status is planted here, on the host) becomes a RuntimeError."""
+    from neurosamble_b200 import _lib, torch_ops
+
+    class Library:
+        @staticmethod
+        def rbq_check_op_errors():
+            return 2
+
+        @staticmethod
+        def rbq_last_error():
+            return b"a tensor-core pipeline wait timed out on the device"
+
+    monkeypatch.setattr(_lib, "lib", lambda: Library)
+    with pytest.raises(RuntimeError, match="timed out"):
+        torch_ops.check_op_errors()
 
 
 # -- on the GPU -------------------------------------------------------------------------------------
@@ -362,3 +380,19 @@ def test_softmax_loss_gradient_in_several_pieces(n, v, d, dt):
     torch.cuda.synchronize()
     assert all(torch.equal(a, dq) and torch.equal(b, dbank) for a, b in outs)
     check_device()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt,pdt", [(F16, F32), (BF16, BF16), (F32, F32)])
+@pytest.mark.parametrize("d", [1, 3, 7, 9, 31, 33, 65, 127, 255, 257])
+def test_layer_norm_narrow_odd_rows_in_rounds(d, dt, pdt):
+    """Widths that take single values, with more rows than the blocks hold at once."""
+    norm_check(*norm_inputs(40001, d, dt, pdt, seed=d))
+
+
+@pytest.mark.gpu
+def test_no_errors_were_recorded():
+    from neurosamble_b200 import torch_ops
+    x = torch.ones(256, 64, dtype=F16, device="cuda")
+    ops().linear(x, x)
+    assert torch_ops.check_op_errors() is None
