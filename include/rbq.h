@@ -388,7 +388,8 @@ int rbq_linear(const void* x_dev, const void* w_dev, const void* bias_dev, const
                int32_t k, int32_t n, int32_t dtype, int32_t act, void* workspace_dev, int64_t workspace_bytes, void* stream);
 /* Gradients from g [m, n] = dL/dy: dz = g * act'(x w^T + bias), recomputed; dx = dz w, dw = dz^T x,
  * dbias = column sums of dz (each may be NULL).  The residual's gradient is g itself.  dz is rounded
- * to dtype as the operand of both products; all sums are fp32 and each output is rounded once. */
+ * to dtype, as the operand of both products, and dbias adds the rounded values (act none: dz is g, with no
+ * rounding); all sums are fp32 and each output is rounded once. */
 int rbq_linear_backward(const void* g_dev, const void* x_dev, const void* w_dev, const void* bias_dev, void* dx_dev,
                         void* dw_dev, void* dbias_dev, int64_t m, int32_t k, int32_t n, int32_t dtype, int32_t act,
                         void* workspace_dev, int64_t workspace_bytes, void* stream);
@@ -416,13 +417,15 @@ int rbq_softmax_loss(const void* q_dev, const void* bank_dev, const int64_t* tar
                      int64_t workspace_bytes, void* stream);
 /* Gradients of sum_i g_i loss_i (g [n] fp32) from the forward pass's loss and lse: dq [n, d] and
  * dbank [v, d] (either may be NULL), in pieces of the bank.  The gradient of the logits is rounded to
- * dtype as the operand of both products, relative to the largest |g_i|. */
+ * dtype as the operand of both products, relative to the largest finite |g_i|: in RBQ_F16 entries p_ij |g_i|
+ * below 2^-27 of that lose bits.  An infinite or NaN g_i spoils its own row of dq and dbank. */
 int rbq_softmax_loss_backward(const float* g_dev, const void* q_dev, const void* bank_dev, const int64_t* target_dev,
                               const float* loss_dev, const float* lse_dev, int64_t n, int64_t v, int32_t d, float scale,
                               int32_t dtype, void* dq_dev, void* dbank_dev, void* workspace_dev, int64_t workspace_bytes,
                               void* stream);
 /* Synchronises the current device and returns RBQ_ERR_CUDA if a kernel of rbq_linear* or
- * rbq_softmax_loss* gave up on a wait since the last call (their results are then invalid). */
+ * rbq_softmax_loss* gave up on a wait since the last call, by any thread of the process, on this device (their
+ * results are then invalid).  The calls themselves do not synchronise and cannot tell. */
 int rbq_check_op_errors(void);
 
 /* ---- fault injection (tests) --------------------------------------------------------------- */

@@ -66,7 +66,9 @@ __device__ int g_op_err;
 // for as long as the CTA stays in one column of tiles.  Tiles run down the columns for that, so a CTA (or
 // pair) visits each column of tiles once at most and writes one row of sums for it:
 //   sums[((cta * CG + rank) * 4 + warp) * N + column]
-// A pass of its own over the output took as long as a third of the gradient kernel.
+// A pass of its own over the output took as long as a third of the gradient kernel.  What is added is the output as
+// rounded to 16 bits, the operand of the two products: one rounding of either sign per term, which the sum
+// averages out.  (The fp32 values lie a row to a thread; their sums would take a transposition of their own.)
 enum Epilogue {
   kEpiLinear,  // out = act(alpha * acc + bias) + extra
   kEpiActGrad, // out = extra * act'(acc + bias)

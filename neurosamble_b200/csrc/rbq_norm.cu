@@ -546,7 +546,8 @@ struct Kernel;  // names a kernel
 template <typename Name, typename K>
 int blocks_for(K kernel, size_t smem, int64_t rows, int tpr, int rounds)
 {
-  static std::atomic<int> per_sm{0};  // one for every Name; smem is that of its widest rows
+  // one for every Name and all devices (the library runs on one architecture); smem is that of its widest rows
+  static std::atomic<int> per_sm{0};
   int n = per_sm.load();
   if (n == 0) {
     RBQ_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, kNormThreads, smem));
