@@ -291,18 +291,19 @@ __device__ __forceinline__ float max_nan(float a, float b)
 //   t(w) = e^{-w^2 / 2} w P(w),   s(w) = e^{-w^2 / 2} (w0 - w) Q(w),   s(w0) = 0
 // so that polynomials for P and Q hold the relative error of the tails, which 16-bit outputs show to the last
 // bit (at z = -5 an absolute error of 8e-7 is half the value).  Own minimax fits by linear programming, in
-// powers of -w.  What they add to the one rounding of the output, in units of that: 0.16 (value) and 0.18 (slope) up
-// to w = 5; past it, in fp16, as much and 0.32 down to the subnormal values (a value is 0 from w = 6, and a
-// slope past 8 times any gradient); in bf16, whose exponents reach w = 13.1, 0.66 and 0.82.  Their absolute error
-// stays under 2e-6 (1 + w).  From w = 13.2 on the exponential is 0.
-// bf16's value is a constant times the exponential past 9.5 (true to 0.5 %), and takes powers of 4.75 - w: so
-// many terms in powers of w would cancel to nothing.
+// powers of -w.  What they add to the one rounding of the output, in units of that: 0.14 (value) and 0.16 (slope) in
+// fp16, 0.21 and 0.18 in bf16 up to w = 5; past it, in fp16, as much and 0.32 down to the subnormal values (a value is
+// 0 from w = 6, and a slope past 8 times any gradient); in bf16, whose exponents reach w = 13.1, 0.79 and 0.82.
+// Their absolute error stays under 3e-6 (1 + w).  From w = 13.2 on the exponential is 0.
+// bf16's value past w = 6.5 is a constant times an exponential: w P(w) rises by 1.8 % from there to 13, and the
+// exponential of (1 - 2.6e-4) w^2 / 2 rises along with it (P on [0, 6.5] makes up for that).  Without that the
+// polynomial took two terms more, in powers of 4.75 - w to keep it from cancelling: 15 % more of the layer's time
+// than the absolute fit named below, where this one takes 3 %.
 // On one B200, 819,200 x 256 -> 1,024 in fp16: 660 us; polynomials for an absolute error of 8e-7, one term shorter,
 // 641; erff and expf 1.85 times as long as those.  The slope's kernel, 51,200 x 256 -> 1,024: 66 us, 61 with an
 // absolute error of 4e-6.
-__device__ __forceinline__ uint64_t gauss2(uint64_t z)  // e^{-z^2 / 2}
+__device__ __forceinline__ uint64_t gauss2(uint64_t z, float c = -0.72134752f)  // 2^{c z^2}, e^{-z^2 / 2} unless told
 {
-  const float c = -0.72134752f;  // -log2(e) / 2
   const float2 t = split(mul2(mul2(z, z), pair(c, c)));
   return pair(ex2(t.x), ex2(t.y));
 }
@@ -325,20 +326,14 @@ __device__ __forceinline__ float2 act_of(uint64_t z)
   const float2 v = split(z);
   if (ACT == RBQ_ACT_RELU) return make_float2(max_nan(v.x, 0.0f), max_nan(v.y, 0.0f));
   if (ACT == RBQ_ACT_GELU) {
-    uint64_t nw, p;
-    if (std::is_same<T, __half>::value) {
-      const float c[10] = {0.499972373f,  0.398479819f, 0.247432157f,   0.126111999f,   0.0520200133f,
-                           0.0164886173f, 0.0037531869f, 0.000565699709f, 4.99067755e-05f, 1.93591131e-06f};
-      nw = minus_abs(v, 6.0f);
-      p = horner2(c, nw);
-    } else {
-      const float c[12] = {0.0806254521f,    0.0157307144f,   0.00298358826f,  0.000617415411f,
-                           8.76739214e-05f,  -7.04420836e-06f, 5.34964329e-06f, 3.19636297e-06f,
-                           -1.65086874e-07f, -1.24640735e-07f, 1.01854436e-08f, 3.03623016e-09f};
-      nw = minus_abs(v, 9.5f);
-      p = horner2(c, add2(nw, pair(4.75f, 4.75f)));
-    }
-    return split(fma2(mul2(gauss2(z), nw), p, pair(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f))));
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    const float half[10] = {0.499972373f,  0.398479819f,  0.247432157f,   0.126111999f,   0.0520200133f,
+                            0.0164886173f, 0.0037531869f, 0.000565699709f, 4.99067755e-05f, 1.93591131e-06f};
+    const float bf16[10] = {0.499914378f,  0.397714943f,   0.244145826f,   0.119834676f,   0.0455746762f,
+                            0.0126912659f, 0.00243611634f, 0.000300497486f, 2.12530103e-05f, 6.51733785e-07f};
+    const uint64_t nw = minus_abs(v, kHalf ? 6.0f : 6.5f), g = kHalf ? gauss2(z) : gauss2(z, -0.721159995f);
+    const uint64_t p = kHalf ? horner2(half, nw) : horner2(bf16, nw);
+    return split(fma2(mul2(g, nw), p, pair(fmaxf(v.x, 0.0f), fmaxf(v.y, 0.0f))));
   }
   return v;
 }
