@@ -388,8 +388,8 @@ int rbq_linear(const void* x_dev, const void* w_dev, const void* bias_dev, const
                int32_t k, int32_t n, int32_t dtype, int32_t act, void* workspace_dev, int64_t workspace_bytes, void* stream);
 /* Gradients from g [m, n] = dL/dy: dz = g * act'(x w^T + bias), recomputed; dx = dz w, dw = dz^T x,
  * dbias = column sums of dz (each may be NULL).  The residual's gradient is g itself.  dz is rounded
- * to dtype, as the operand of both products, and dbias adds the rounded values (act none: dz is g, with no
- * rounding); all sums are fp32 and each output is rounded once. */
+ * to dtype as the operand of both products (act none: dz is g), not for dbias; all sums are fp32 and each
+ * output is rounded once. */
 int rbq_linear_backward(const void* g_dev, const void* x_dev, const void* w_dev, const void* bias_dev, void* dx_dev,
                         void* dw_dev, void* dbias_dev, int64_t m, int32_t k, int32_t n, int32_t dtype, int32_t act,
                         void* workspace_dev, int64_t workspace_bytes, void* stream);

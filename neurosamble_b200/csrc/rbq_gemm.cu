@@ -61,14 +61,16 @@ constexpr float kGradScale = 16384.0f;        // power of two, see GradRows
 
 __device__ int g_op_err;
 
-// Column sums of the gradient kernel's output (the bias's gradient) come from its staging tiles: in a
-// group, thread t adds columns 2 (t % 32) and the next over the 32 rows of warp t / 32, in registers
-// for as long as the CTA stays in one column of tiles.  Tiles run down the columns for that, so a CTA (or
-// pair) visits each column of tiles once at most and writes one row of sums for it:
+// Column sums of the gradient kernel's output (the bias's gradient) are taken in fp32, before its rounding to 16
+// bits: a sum of many terms of either sign may be small beside them, and their roundings are not.  A row's values lie
+// in one thread, so the 32 rows of a warp pass 16 columns at a time through the staging rows that held the extra
+// input of these columns (consumed by then): lane l adds columns 2 (l % 8) and the next over rows 8 (l / 8).., in
+// registers for as long as the CTA stays in one column of tiles.  Tiles run down the columns for that, so a CTA (or
+// pair) visits each column of tiles once at most and writes one row of sums per warp for it:
 //   sums[((cta * CG + rank) * 4 + warp) * N + column]
-// A pass of its own over the output took as long as a third of the gradient kernel.  What is added is the output as
-// rounded to 16 bits, the operand of the two products: one rounding of either sign per term, which the sum
-// averages out.  (The fp32 values lie a row to a thread; their sums would take a transposition of their own.)
+// Rows past the last add zeros: g is 0 there, and the slope finite but in columns whose bias is NaN, of which nothing
+// is left anyway.  51,200 x 256 -> 1,024 with GELU: 72 us, 67 with sums of the rounded values; four columns to a lane
+// spill (74).  A pass of its own over the output took a third of the kernel.
 enum Epilogue {
   kEpiLinear,  // out = act(alpha * acc + bias) + extra
   kEpiActGrad, // out = extra * act'(acc + bias)
@@ -96,7 +98,7 @@ struct GemmArgs {
   int64_t ld_extra = 0, ld_out = 0;  // of the warps' own moves
   float alpha = 1.0f;
   const float* alpha_dev = nullptr;  // further factor held on the device
-  float* sums = nullptr;  // kEpiActGrad: column sums of out, see above
+  float* sums = nullptr;  // kEpiActGrad: column sums of out before its rounding, see above
   int slab_rows = 0;     // rows between slabs
   int slab_add = 0;      // add to what the slab holds
   // softmax loss: rows are queries, columns bank rows col0 + n
@@ -690,13 +692,23 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
     };
     Walk w(a, first_unit);
     read_ahead(w);
-    float2 sums = make_float2(0.0f, 0.0f);
-    int sums_n = -1;  // the column of tiles that they belong to
+    uint64_t sums[4] = {};  // of columns 16 i + 2 (lane % 8) and the next of the group, over the lane's rows
+    int sums_n = -1;        // the column of tiles that they belong to
+    const int sum_at = quarter * 4096 + (lane >> 3) * 1024 + (lane & 7) * 8;  // first of the lane's 8 rows
     auto write_sums = [&]() {
-      const int col = sums_n * BN + wg * 64 + lane * 2;
-      float* at = a.sums + ((int64_t)(first_unit * CG + rank) * 4 + quarter) * a.N + col;
-      if (col < a.N) at[0] = sums.x;
-      if (col + 1 < a.N) at[1] = sums.y;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 two = split(sums[i]);
+        float e[2] = {two.x, two.y};
+        const int col = sums_n * BN + wg * 64 + i * 16 + (lane & 7) * 2;
+        float* at = a.sums + ((int64_t)(first_unit * CG + rank) * 4 + quarter) * a.N + col;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+#pragma unroll
+          for (int o = 8; o < 32; o <<= 1) e[k] += __shfl_xor_sync(0xffffffffu, e[k], o);
+          if (lane < 8 && col + k < a.N) at[k] = e[k];
+        }
+      }
     };
     if (kElement) {
       if (gt < 64) bias[gt] = next_bias;
@@ -849,6 +861,12 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
           __syncwarp();
         }
       }
+      if (EPI == kEpiActGrad && a.sums != nullptr && tl.n != sums_n) {
+        if (sums_n >= 0 && !dead) write_sums();
+        sums_n = tl.n;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sums[i] = 0;
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float v[32];
@@ -902,25 +920,34 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
               }
             }
           }
-          at[slot] = make_uint4(Pack<T>::two(o[0], o[1]), Pack<T>::two(o[2], o[3]), Pack<T>::two(o[4], o[5]),
-                                Pack<T>::two(o[6], o[7]));
+          if (EPI != kEpiActGrad)
+            at[slot] = make_uint4(Pack<T>::two(o[0], o[1]), Pack<T>::two(o[2], o[3]), Pack<T>::two(o[4], o[5]),
+                                  Pack<T>::two(o[6], o[7]));
         }
-      }
-      if (EPI == kEpiActGrad && a.sums != nullptr && tl.n != sums_n) {
-        if (sums_n >= 0 && !dead) write_sums();
-        sums_n = tl.n;
-        sums = make_float2(0.0f, 0.0f);
-      }
-      if (EPI == kEpiActGrad && a.sums != nullptr) {  // before the barrier: a warp reads its own rows only
-        __syncwarp();
-        const int rows = dead ? 0 : (int)min((int64_t)32, a.M - m0 - quarter * 32);
-#pragma unroll 8
-        for (int r = 0; r < rows; ++r) {
-          const int at = quarter * 32 + r;
-          const float2 f = Pack<T>::get(
-              *reinterpret_cast<const uint32_t*>(buf + at * 128 + (((lane >> 2) ^ (at & 7)) << 4) + (lane & 3) * 4));
-          sums.x += f.x;
-          sums.y += f.y;
+        if (EPI == kEpiActGrad) {
+          if (a.sums != nullptr) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+              if (q == 1) __syncwarp();  // the columns before have been read
+              float4* to = reinterpret_cast<float4*>(at);
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                const float* e = v + q * 16 + k * 4;
+                to[(h * 4 + k) ^ (gt & 7)] = make_float4(e[0], e[1], e[2], e[3]);
+              }
+              __syncwarp();
+#pragma unroll
+              for (int r = 0; r < 8; ++r)
+                sums[h * 2 + q] = add2(sums[h * 2 + q], *reinterpret_cast<const uint64_t*>(buf + (sum_at ^ (h * 64) ^ (r * 16)) + r * 128));
+            }
+            __syncwarp();
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float* o = v + k * 8;
+            at[(h * 4 + k) ^ (gt & 7)] = make_uint4(Pack<T>::two(o[0], o[1]), Pack<T>::two(o[2], o[3]),
+                                                    Pack<T>::two(o[4], o[5]), Pack<T>::two(o[6], o[7]));
+          }
         }
       }
       if (a.out_tma) {
@@ -1477,8 +1504,8 @@ void linear_backward(const T* g, const T* x, const T* w, const T* bias, T* dx, T
   const Matrix X = addressable(x, m, k, ws, run, s), W = addressable(w, n, k, ws, run, s);
   Matrix Z;
   const int cg = group_size(m, n);
-  // The gradient kernel's sums are 4 rows of n floats per CTA: less than a pass over dz from about 2,048 rows.
-  const bool fused = act != RBQ_ACT_NONE && m >= 2048;
+  // With an activation the gradient kernel leaves 4 rows of n sums per CTA; without one dz is g, summed by a pass.
+  const bool fused = act != RBQ_ACT_NONE;
   const int64_t tiles_m = ceil_div(m, kBM * cg), tiles_n = ceil_div(n, 128 * cg);
   const int ctas = (int)std::min<int64_t>(tiles_m * tiles_n, device_sm_count() / cg);
   const int gx = (int)ceil_div(n, kColGroup * 8);

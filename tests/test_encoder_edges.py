@@ -396,3 +396,26 @@ def test_no_errors_were_recorded():
     x = torch.ones(256, 64, dtype=F16, device="cuda")
     ops().linear(x, x)
     assert torch_ops.check_op_errors() is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [F16, BF16])
+@pytest.mark.parametrize("m,k,n", [(65, 8, 40), (1001, 8, 37), (5001, 16, 300), (20000, 8, 517)])
+def test_bias_gradients_that_cancel(m, k, n, dt):
+    """Bias gradients far smaller than their terms, which a last row cancels: they are sums of fp32 terms,
+    rounded once, without the rounding to 16 bits that the products' operand has."""
+    x, w, b, _, g = linear_inputs(m, k, n, dt, seed=m)
+    w, x[-1] = w.abs(), 60.0  # the last row's slope is 1 in every column
+    z = x.double() @ w.double().t() + b.double()
+    slope = torch.special.ndtr(z) + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    assert (slope[-1] == 1).all()
+    g[-1] = 0
+    g[-1] = -(g.double() * slope).sum(0).to(dt)
+    dz = g.double() * slope
+    want = dz.sum(0)
+    db = ops().linear_backward(g, x, w, b, "gelu", True, True, True)[2]
+    check_device()
+    # an error of z's sum and of the slope (|gelu''| <= 0.8), and fp32 additions; one rounding of the result
+    ez = (k + 8) * ADD * (x.double().abs() @ w.double().abs().t() + b.double().abs())
+    tol = ((0.8 * ez + 4e-6 * (1 + z.abs())) * g.double().abs() * (slope != 1)).sum(0) + (m + 8) * ADD * dz.abs().sum(0)
+    within(db, want, (u(dt) + ADD) * want.abs() + 1.01 * tol + tiny(dt), "db")
