@@ -417,7 +417,7 @@ int rbq_softmax_loss(const void* q_dev, const void* bank_dev, const int64_t* tar
                      int64_t workspace_bytes, void* stream);
 /* Gradients of sum_i g_i loss_i (g [n] fp32) from the forward pass's loss and lse: dq [n, d] and
  * dbank [v, d] (either may be NULL), in pieces of the bank.  The gradient of the logits is rounded to
- * dtype as the operand of both products, relative to the largest finite |g_i|: in RBQ_F16 entries p_ij |g_i|
+ * dtype as the operand of both products (but for the targets' entries in dq), relative to the largest finite |g_i|: in RBQ_F16 entries p_ij |g_i|
  * below 2^-27 of that lose bits.  An infinite or NaN g_i spoils its own row of dq and dbank. */
 int rbq_softmax_loss_backward(const float* g_dev, const void* q_dev, const void* bank_dev, const int64_t* target_dev,
                               const float* loss_dev, const float* lse_dev, int64_t n, int64_t v, int32_t d, float scale,

@@ -113,10 +113,11 @@ struct GemmArgs {
 // scale of at most kGradScale (0: the row takes no part) and the value at the target, expm1(-loss) * w.
 //   d loss_i / d s_ij = p_ij - [j = t_i],   p_ij - 1 = expm1(-loss_i) at the target
 // The gradient of the logits is rounded to the operands' 16 bits, since it is the operand of the two
-// products that follow.  |p - 1| <= 1, so with |w| <= 2^14 nothing overflows in fp16 and
+// products that follow; what that takes off the target's entry, the largest of its row, is added to dq by
+// itself (at_rest, see loss_operands_kernel).  |p - 1| <= 1, so with |w| <= 2^14 nothing overflows in fp16 and
 // probabilities down to 2^-27 keep all 11 bits; the factor max|g| * scale / w returns in fp32.
 struct GradRows {
-  float lse2, w, at_target, unused;
+  float lse2, w, at_target, at_rest;
 };
 
 __device__ __forceinline__ float ex2(float x)
@@ -997,24 +998,24 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
 // ---------------------------------------------------------------------------------------
 
 // Rows of `cols` 16-bit values -> rows `ld` apart (ld a multiple of 8, so that TMA can address them).  A thread
-// makes 16 bytes of the copy.  With `weights` (GradRows) a row of weight 0 is zeros in the copy, whatever it holds.
+// makes 16 bytes of the copy.
 __global__ void pad_rows_kernel(const uint16_t* __restrict__ src, int64_t rows, int cols, int ld,
-                                uint16_t* __restrict__ dst, const float4* __restrict__ weights)
+                                uint16_t* __restrict__ dst)
 {
   const int per = ld / 8;
   for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < rows; r += (int64_t)gridDim.x * blockDim.y) {
-    const bool kept = weights == nullptr || weights[r].y != 0.0f;
     for (int i = threadIdx.x; i < per; i += blockDim.x) {
       uint32_t v[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = kept && i * 8 + e < cols ? src[r * cols + i * 8 + e] : 0u;
+      for (int e = 0; e < 8; ++e) v[e] = i * 8 + e < cols ? src[r * cols + i * 8 + e] : 0u;
       *reinterpret_cast<uint4*>(dst + r * ld + i * 8) =
           make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
     }
   }
 }
 
-// out[m, n] = alpha * sum over the tile's slabs in ascending order; slab rows are ld (multiple of 4) apart.
+// out[m, n] = alpha * sum over the tile's slabs in ascending order, + extra [m, n] if there is one; slab rows are ld
+// (multiple of 4) apart.
 // With `ctas` the slabs of a tile are those of the CTAs that had a part of it (RangeWalk), else all of them.
 struct SlabTiles {
   int slabs, tile, tiles_m, kblocks, ctas;  // tile: rows and columns of one
@@ -1022,7 +1023,8 @@ struct SlabTiles {
 };
 template <typename T>
 __global__ void add_slabs_kernel(const float* __restrict__ slabs, SlabTiles st, int64_t slab_stride, int64_t rows, int cols,
-                                 int ld, float alpha, const float* __restrict__ alpha_dev, T* __restrict__ out)
+                                 int ld, float alpha, const float* __restrict__ alpha_dev, const T* __restrict__ extra,
+                                 T* __restrict__ out)
 {
   if (alpha_dev != nullptr) alpha *= __ldg(alpha_dev);
   const int quads = ld / 4;
@@ -1042,14 +1044,18 @@ __global__ void add_slabs_kernel(const float* __restrict__ slabs, SlabTiles st, 
       sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
     }
     T* o = out + r * cols + c;
-    const float e[4] = {sum.x, sum.y, sum.z, sum.w};
+    float e[4] = {alpha * sum.x, alpha * sum.y, alpha * sum.z, alpha * sum.w};
     if ((cols & 3) == 0) {
-      *reinterpret_cast<uint2*>(o) =
-          make_uint2(Pack<T>::two(alpha * e[0], alpha * e[1]), Pack<T>::two(alpha * e[2], alpha * e[3]));
+      if (extra != nullptr) {
+        const uint2 x = *reinterpret_cast<const uint2*>(extra + r * cols + c);
+        const float2 a = Pack<T>::get(x.x), b = Pack<T>::get(x.y);
+        e[0] += a.x, e[1] += a.y, e[2] += b.x, e[3] += b.y;
+      }
+      *reinterpret_cast<uint2*>(o) = make_uint2(Pack<T>::two(e[0], e[1]), Pack<T>::two(e[2], e[3]));
     } else {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (c + j < cols) o[j] = Pack<T>::from(alpha * e[j]);
+        if (c + j < cols) o[j] = Pack<T>::from(extra != nullptr ? e[j] + Pack<T>::one(extra[r * cols + c + j]) : e[j]);
     }
   }
 }
@@ -1183,9 +1189,9 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(const float2* __restric
 }
 
 // Largest finite |g| of the rows that take part (1 if all are 0), and the scale of the logits' gradient: kGradScale times one
-// of eight factors in (1/2, 1].  A row's gradient is mostly its target's entry, so its rounding does
-// not average out the way the others' do; rows that have learnt about as much have entries of about
-// one mantissa, and a factor that moves it up towards the next power of two halves the rounding.  The
+// of eight factors in (1/2, 1].  A bank row's gradient is mostly the entries of the queries that it is the target
+// of, whose rounding does not average out the way the others' do; rows that have learnt about as much have entries
+// of about one mantissa, and a factor that moves it up towards the next power of two halves the rounding.  The
 // factor is the one with the least squared rounding of the target's entries over the first rows.  A row whose g
 // is infinite or NaN has a weight that is: its own gradient and the bank's are lost, the other rows' are not.
 constexpr int kScaleTries = 8;
@@ -1240,6 +1246,7 @@ __global__ void __launch_bounds__(1024) grad_top_kernel(const float* __restrict_
     out[2] = kGradScale * factor;
   }
 }
+template <typename T>
 __global__ void grad_rows_kernel(const float* __restrict__ g, const int64_t* __restrict__ target,
                                  const float* __restrict__ loss, const float* __restrict__ lse, int64_t n, int64_t v,
                                  const float* __restrict__ top, float4* __restrict__ rows)
@@ -1249,7 +1256,64 @@ __global__ void grad_rows_kernel(const float* __restrict__ g, const int64_t* __r
   const int64_t t = target[i];
   float w = 0.0f;
   if (t >= 0 && t < v && g[i] != 0.0f) w = g[i] / top[0] * top[2];
-  rows[i] = make_float4(lse[i] * kLog2e, w, w == 0.0f ? 0.0f : expm1f(-loss[i]) * w, 0.0f);
+  const float at = w == 0.0f ? 0.0f : expm1f(-loss[i]) * w;
+  rows[i] = make_float4(lse[i] * kLog2e, w, at, at - Pack<T>::one(Pack<T>::from(at)));
+}
+
+// What the products of the loss's gradient read beside the logits' gradient:
+//   kept [n, ld]: q with zeros in the rows that take no part.  They meet zeros of the logits' gradient in the bank's
+//     sums, and zero times an infinity or NaN that such a row may hold (a batch's padding) would spoil every row of
+//     dbank.  Rows ld apart, a multiple of 8.
+//   rest [n, d]: what the rounding of the target's entry takes off dq, at_rest * k_target times the products' factor.
+//     That entry is as large as all the others of its row together, so its rounding does not average out as theirs
+//     do, and where a bank's rows lie close to the target the products' sum is far smaller than the entry: without
+//     this dq was up to 1.8 times as far off as fp32 torch's.  (The bank's gradient keeps the rounding: there such
+//     entries come from different queries.)
+// A thread has eight values of a row.
+template <typename T>
+__global__ void loss_operands_kernel(const T* __restrict__ q, const T* __restrict__ bank, const int64_t* __restrict__ target,
+                                     const float4* __restrict__ rows, const float* __restrict__ top, int64_t n, int d, int ld,
+                                     uint16_t* __restrict__ kept, T* __restrict__ rest)
+{
+  const int per = ld / 8;
+  const bool whole = d == ld;  // rows of whole 16-byte pieces
+  for (int64_t r = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; r < n; r += (int64_t)gridDim.x * blockDim.y) {
+    const float4 row = rows[r];
+    const float f = row.w * top[1];
+    const bool add = row.w != 0.0f;  // the row takes part, so its target lies in the bank
+    const uint16_t* from = reinterpret_cast<const uint16_t*>(q) + r * d;
+    const uint16_t* key = reinterpret_cast<const uint16_t*>(bank) + (add ? target[r] * d : 0);
+    for (int i = threadIdx.x; i < per; i += blockDim.x) {
+      uint4 x = make_uint4(0, 0, 0, 0), k = x;
+      uint32_t *xs = &x.x, *ks = &k.x;
+      if (whole) {
+        if (row.y != 0.0f) x = *reinterpret_cast<const uint4*>(from + i * 8);
+        if (add) k = *reinterpret_cast<const uint4*>(key + i * 8);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool in = i * 8 + e < d;
+          if (in && row.y != 0.0f) xs[e / 2] |= (uint32_t)from[i * 8 + e] << (e & 1) * 16;
+          if (in && add) ks[e / 2] |= (uint32_t)key[i * 8 + e] << (e & 1) * 16;
+        }
+      }
+      *reinterpret_cast<uint4*>(kept + r * ld + i * 8) = x;
+      if (rest == nullptr) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 two = Pack<T>::get(ks[e]);
+        ks[e] = add ? Pack<T>::two(f * two.x, f * two.y) : 0u;
+      }
+      uint16_t* to = reinterpret_cast<uint16_t*>(rest) + r * d + i * 8;
+      if (whole) {
+        *reinterpret_cast<uint4*>(to) = k;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i * 8 + e < d) to[e] = (uint16_t)(ks[e / 2] >> (e & 1) * 16);
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------
@@ -1381,14 +1445,24 @@ struct Carver {
   }
 };
 
-void pad_rows(const void* src, int64_t rows, int cols, int ld, void* dst, const float4* weights, cudaStream_t s)
+// Blocks of 256 threads, each with eight values of a row.
+struct RowBlocks {
+  dim3 block;
+  unsigned blocks;
+  RowBlocks(int64_t rows, int ld)
+  {
+    int x = 8;  // threads to a row
+    while (x < 256 && x < ld / 8) x *= 2;
+    block = dim3(x, 256 / x);
+    blocks = (unsigned)std::min<int64_t>(ceil_div(rows, block.y), (int64_t)device_sm_count() * 16);
+  }
+};
+
+void pad_rows(const void* src, int64_t rows, int cols, int ld, void* dst, cudaStream_t s)
 {
-  int x = 8;  // threads to a row
-  while (x < 256 && x < ld / 8) x *= 2;
-  const dim3 block(x, 256 / x);
-  const int64_t blocks = std::min<int64_t>(ceil_div(rows, block.y), (int64_t)device_sm_count() * 16);
-  pad_rows_kernel<<<(unsigned)blocks, block, 0, s>>>(static_cast<const uint16_t*>(src), rows, cols, ld,
-                                                     static_cast<uint16_t*>(dst), weights);
+  const RowBlocks l(rows, ld);
+  pad_rows_kernel<<<l.blocks, l.block, 0, s>>>(static_cast<const uint16_t*>(src), rows, cols, ld,
+                                               static_cast<uint16_t*>(dst));
   RBQ_LAUNCHED();
 }
 
@@ -1398,7 +1472,7 @@ Matrix addressable(const void* p, int64_t rows, int cols, Carver& ws, bool run, 
   if (cols % 8 == 0) return Matrix{p, rows, cols, cols};
   const int ld = (int)round_up(cols, 8);
   uint16_t* copy = ws.take<uint16_t>(rows * ld);
-  if (run) pad_rows(p, rows, cols, ld, copy, nullptr, s);
+  if (run) pad_rows(p, rows, cols, ld, copy, s);
   return Matrix{copy, rows, cols, ld};
 }
 
@@ -1441,28 +1515,35 @@ void slab_gemm(const SlabPlan& p, Matrix A, bool a_mn, Matrix B, bool b_mn, floa
 }
 // `all`: every slab holds a sum (of zeros at least), else those of RangeWalk.
 template <typename T>
-void add_slabs(const SlabPlan& p, const float* slabs, bool all, int64_t M, int N, float alpha, const float* alpha_dev, T* out,
-               cudaStream_t s)
+void add_slabs(const SlabPlan& p, const float* slabs, bool all, int64_t M, int N, float alpha, const float* alpha_dev,
+               const T* extra, T* out, cudaStream_t s)
 {
   const int64_t blocks = std::min<int64_t>(ceil_div(M * (p.ld / 4), 256), (int64_t)device_sm_count() * 8);
   const SlabTiles st{p.slabs, 128 * p.cg, p.tiles_m, p.kblocks, all ? 0 : p.ctas, p.total};
-  add_slabs_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(slabs, st, p.rows * p.ld, M, N, (int)p.ld, alpha, alpha_dev, out);
+  add_slabs_kernel<T><<<(unsigned)blocks, 256, 0, s>>>(slabs, st, p.rows * p.ld, M, N, (int)p.ld, alpha, alpha_dev,
+                                                         extra, out);
   RBQ_LAUNCHED();
 }
 
-// out[M, N] (dense) = alpha_dev * A B^T, written by the product's own epilogue.
+// out[M, N] (dense) = alpha_dev * A B^T (+ extra [M, N]), written by the product's own epilogue.
 template <typename T>
-void store_gemm(Matrix A, bool a_mn, Matrix B, bool b_mn, int cg, const float* alpha_dev, T* out, cudaStream_t s)
+void store_gemm(Matrix A, bool a_mn, Matrix B, bool b_mn, int cg, const float* alpha_dev, const T* extra, T* out,
+                cudaStream_t s)
 {
   const int64_t M = a_mn ? A.cols : A.rows, N = b_mn ? B.cols : B.rows;
   GemmArgs a;
   a.alpha_dev = alpha_dev;
+  a.extra = extra;
+  a.has_extra = extra != nullptr;
   a.out = out;
-  a.ld_out = N;
-  a.out_tma = N % 8 == 0;
-  CUtensorMap to{};
-  if (a.out_tma) to = matrix_map<T>(Matrix{out, M, N, N}, kBM);
-  gemm<kEpiLinear, T>(a, A, a_mn, B, b_mn, cg, nullptr, a.out_tma ? &to : nullptr, s);
+  a.ld_extra = a.ld_out = N;
+  a.extra_tma = a.out_tma = N % 8 == 0;
+  CUtensorMap tx{}, to{};
+  if (a.out_tma) {
+    to = matrix_map<T>(Matrix{out, M, N, N}, kBM);
+    tx = extra ? matrix_map<T>(Matrix{extra, M, N, N}, kBM) : to;
+  }
+  gemm<kEpiLinear, T>(a, A, a_mn, B, b_mn, cg, a.out_tma ? &tx : nullptr, a.out_tma ? &to : nullptr, s);
 }
 
 template <typename T>
@@ -1537,11 +1618,11 @@ void linear_backward(const T* g, const T* x, const T* w, const T* bias, T* dx, T
   const SlabPlan plan = plan_slabs(n, k, m, false);
   float* slabs = ws.take<float>(plan.floats());
   if (!run) return;
-  if (dx) store_gemm<T>(Z, false, W, true, group_size(m, k), nullptr, dx, s);
-  if (dw && plan.direct) store_gemm<T>(Z, true, X, true, plan.cg, nullptr, dw, s);
+  if (dx) store_gemm<T>(Z, false, W, true, group_size(m, k), nullptr, nullptr, dx, s);
+  if (dw && plan.direct) store_gemm<T>(Z, true, X, true, plan.cg, nullptr, nullptr, dw, s);
   if (dw && !plan.direct) {
     slab_gemm<T>(plan, Z, true, X, true, slabs, false, s);
-    add_slabs<T>(plan, slabs, false, n, k, 1.0f, nullptr, dw, s);
+    add_slabs<T>(plan, slabs, false, n, k, 1.0f, nullptr, nullptr, dw, s);
   }
   if (dbias) {
     if (!fused) {
@@ -1595,11 +1676,9 @@ template <typename T>
 void loss_backward(const float* g, const T* q, const T* bank, const int64_t* target, const float* loss, const float* lse,
                    int64_t n, int64_t v, int d, float scale, T* dq, T* dbank, Carver& ws, bool run, cudaStream_t s)
 {
-  // q with zeros in the rows that take no part: they meet zeros of the logits' gradient in the bank's sums, and
-  // zero times an infinity or NaN that such a row may hold (a batch's padding) would spoil every row of dbank.  It is
-  // the padded copy too where the width wants one.
   const int ldq = (int)round_up(d, 8);
   uint16_t* kept = ws.take<uint16_t>(n * ldq);
+  T* rest = ws.take<T>(n * d);
   const Matrix Q{kept, n, d, ldq}, B = addressable(bank, v, d, ws, run, s);
   const int64_t piece = std::min(piece_columns(n, v), round_up(v, 8));
   float* top = ws.take<float>(3);
@@ -1618,9 +1697,11 @@ void loss_backward(const float* g, const T* q, const T* bank, const int64_t* tar
   if (!run) return;
   grad_top_kernel<T><<<1, 1024, 0, s>>>(g, target, loss, n, v, scale, top);
   RBQ_LAUNCHED();
-  grad_rows_kernel<<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(g, target, loss, lse, n, v, top, rows);
+  grad_rows_kernel<T><<<(unsigned)ceil_div(n, 256), 256, 0, s>>>(g, target, loss, lse, n, v, top, rows);
   RBQ_LAUNCHED();
-  pad_rows(q, n, d, ldq, kept, rows, s);
+  const RowBlocks l(n, ldq);
+  loss_operands_kernel<T><<<l.blocks, l.block, 0, s>>>(q, bank, target, rows, top, n, d, ldq, kept, dq ? rest : nullptr);
+  RBQ_LAUNCHED();
   if (dq && pieces) RBQ_CUDA(cudaMemsetAsync(slabs_q, 0, pq.floats() * sizeof(float), s));
   for (int64_t v0 = 0; v0 < v; v0 += piece) {
     const int64_t cols = std::min(piece, v - v0);
@@ -1634,19 +1715,19 @@ void loss_backward(const float* g, const T* q, const T* bank, const int64_t* tar
     const CUtensorMap to = matrix_map<T>(P, kBM);
     gemm<kEpiProb, T>(a, Q, false, Bp, false, group_size(n, cols), nullptr, &to, s);
     const bool at_last = v0 + piece >= v;
-    if (dq && pq.direct) store_gemm<T>(P, false, Bp, true, pq.cg, top + 1, dq, s);
+    if (dq && pq.direct) store_gemm<T>(P, false, Bp, true, pq.cg, top + 1, rest, dq, s);
     if (dq && !pq.direct) slab_gemm<T>(at_last ? pq_last : pq, P, false, Bp, true, slabs_q, pieces, s);
     if (dbank) {
       const SlabPlan& p = at_last ? pb_last : pb;
       if (p.direct) {
-        store_gemm<T>(P, true, Q, true, p.cg, top + 1, dbank + v0 * d, s);
+        store_gemm<T>(P, true, Q, true, p.cg, top + 1, nullptr, dbank + v0 * d, s);
       } else {
         slab_gemm<T>(p, P, true, Q, true, slabs_b, false, s);
-        add_slabs<T>(p, slabs_b, false, cols, d, 1.0f, top + 1, dbank + v0 * d, s);
+        add_slabs<T>(p, slabs_b, false, cols, d, 1.0f, top + 1, nullptr, dbank + v0 * d, s);
       }
     }
   }
-  if (dq && !pq.direct) add_slabs<T>(pq, slabs_q, pieces, n, d, 1.0f, top + 1, dq, s);
+  if (dq && !pq.direct) add_slabs<T>(pq, slabs_q, pieces, n, d, 1.0f, top + 1, rest, dq, s);
 }
 
 }  // namespace

@@ -419,3 +419,24 @@ def test_bias_gradients_that_cancel(m, k, n, dt):
     ez = (k + 8) * ADD * (x.double().abs() @ w.double().abs().t() + b.double().abs())
     tol = ((0.8 * ez + 4e-6 * (1 + z.abs())) * g.double().abs() * (slope != 1)).sum(0) + (m + 8) * ADD * dz.abs().sum(0)
     within(db, want, (u(dt) + ADD) * want.abs() + 1.01 * tol + tiny(dt), "db")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,v,d", [(1, 512, 8), (700, 512, 40), (40, 1024, 64), (33, 1024, 33), (300, 2048, 24)])
+def test_query_gradients_that_cancel(n, v, d):
+    """A bank of equal rows: every probability is 1 / v, the target's entry cancels all the others and dq is 0.
+    The others are powers of two, which 16 bits hold; the target's, 1 - 1 / v, takes more bits than bf16 has,
+    and what its rounding leaves is not in dq."""
+    q, bank, target, _ = loss_inputs(n, v, d, BF16, ignored=0.0, seed=v)
+    bank, scale = bank[:1].expand(v, d).contiguous(), 4.0
+    dq, _ = loss_gradients(q, bank, target, torch.ones(n, device="cuda"), scale)
+    check_device()
+    s = scale * (q.double() @ bank[0].double())
+    es = (d + 8) * ADD * scale * (q.double().abs() @ bank[0].double().abs()) + 4 * ADD * s.abs()
+    e = es + (v + 64) * ADD * 2 + 4 * ADD * (s + math.log(v)).abs()
+    assert (2 * (e + es) < u(BF16) / 2).all()  # the others round to 1 / v whatever their error
+    # the target's entry, expm1(-loss): the loss's error times 1 / v, and fp32; a sum of v products whose
+    # magnitudes add up to 2; and the rounding of what the entry's own rounding left
+    each = 2 * e / v + 8 * ADD + 2 * (v + 72) * ADD + u(BF16) ** 2
+    tol = 1.01 * scale * each[:, None] * bank[0].double().abs()
+    within(dq, torch.zeros_like(q, dtype=torch.float64), tol + tiny(BF16), "dq")
