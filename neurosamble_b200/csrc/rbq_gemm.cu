@@ -303,7 +303,7 @@ __device__ __forceinline__ float max_nan(float a, float b)
 // polynomial took two terms more, in powers of 4.75 - w to keep it from cancelling: 15 % more of the layer's time
 // than the absolute fit named below, where this one takes 3 %.
 // On one B200, 819,200 x 256 -> 1,024 in fp16: 660 us; polynomials for an absolute error of 8e-7, one term shorter,
-// 641; erff and expf 1.85 times as long as those.  The slope's kernel, 51,200 x 256 -> 1,024: 66 us, 61 with an
+// 641; erff and expf 1.85 times as long as those.  The slope's kernel, 51,200 x 256 -> 1,024: 72 us, 67 with one for an
 // absolute error of 4e-6.
 __device__ __forceinline__ uint64_t gauss2(uint64_t z, float c = -0.72134752f)  // 2^{c z^2}, e^{-z^2 / 2} unless told
 {
@@ -939,7 +939,8 @@ __global__ void __launch_bounds__(Shape<EPI, CG>::kThreads, 1)
               __syncwarp();
 #pragma unroll
               for (int r = 0; r < 8; ++r)
-                sums[h * 2 + q] = add2(sums[h * 2 + q], *reinterpret_cast<const uint64_t*>(buf + (sum_at ^ (h * 64) ^ (r * 16)) + r * 128));
+                sums[h * 2 + q] = add2(sums[h * 2 + q], *reinterpret_cast<const uint64_t*>(
+                                                            buf + (sum_at ^ (h * 64) ^ (r * 16)) + r * 128));
             }
             __syncwarp();
           }
@@ -1188,8 +1189,8 @@ __global__ void __launch_bounds__(1024) loss_rows_kernel(const float2* __restric
   }
 }
 
-// Largest finite |g| of the rows that take part (1 if all are 0), and the scale of the logits' gradient: kGradScale times one
-// of eight factors in (1/2, 1].  A bank row's gradient is mostly the entries of the queries that it is the target
+// Largest finite |g| of the rows that take part (1 if all are 0), and the scale of the logits' gradient: kGradScale
+// times one of eight factors in (1/2, 1].  A bank row's gradient is mostly the entries of the queries that it is the target
 // of, whose rounding does not average out the way the others' do; rows that have learnt about as much have entries
 // of about one mantissa, and a factor that moves it up towards the next power of two halves the rounding.  The
 // factor is the one with the least squared rounding of the target's entries over the first rows.  A row whose g
